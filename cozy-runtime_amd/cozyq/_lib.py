@@ -133,6 +133,32 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         c_int, [c_int, c_int, _P, _P, _P, _P, _P, _P, _P, _P, c_int64, c_int64, c_int64, _P, _P]
     ),
     "cozyq_bake_rotate_factor": (c_int, [c_int, _P, _P, c_int64, c_int64, _P]),
+    "cozyq_head_norm_rope": (
+        c_int,
+        [c_int, _P, _P, c_int, c_int64, c_int, c_int, c_int, c_int64, c_int64, c_int64, c_int64, c_int, _P, _P,
+         c_int, c_float, _P, _P, c_int64, c_int, c_int, _P, _P, _P, _P],
+    ),
+    "cozyq_cache_most_requests": (c_int, []),
+    "cozyq_cache_runs": (c_int64, [c_int64, c_int, c_int]),
+    "cozyq_cache_plan": (
+        c_int,
+        [c_int, _P, c_int, c_int, _P, c_int, _P, _P, _P, c_int64, c_int, _P, _P, _P, _P, _P, _P, _P, _P],
+    ),
+    "cozyq_cache_append": (
+        c_int,
+        [c_int, c_int, _P, _P, c_int, c_int64, c_int64, c_int64, c_int64, c_int64, _P, _P, _P, _P, c_int, c_int,
+         c_int, c_int, _P, c_int64, _P],
+    ),
+    "cozyq_cache_read": (
+        c_int,
+        [c_int, c_int, _P, _P, _P, _P, c_int, c_int, c_int, c_int, _P, c_int64, _P, _P, c_int, _P],
+    ),
+    "cozyq_cache_attend_workspace_bytes": (c_int64, [c_int64, c_int, c_int, c_int, c_int, c_int64]),
+    "cozyq_cache_attend": (
+        c_int,
+        [c_int, c_int, _P, c_int, c_int64, c_int, c_int64, c_int64, _P, _P, _P, _P, c_int, c_int, c_int, c_int, _P,
+         c_int, c_int, _P, _P, c_int64, c_float, c_int, c_int, _P, _P, _P],
+    ),
     "cozyq_host_e4m3": (None, [_P, _P, c_int64]),
     "cozyq_host_mx_byte": (None, [_P, _P, c_int64]),
     "cozyq_probe_div": (c_int, [c_int, _P, _P, _P, c_int64, _P]),

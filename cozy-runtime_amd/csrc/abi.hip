@@ -691,6 +691,145 @@ int cozyq_bake_stats(int device, int form, const void* before, const void* after
                              static_cast<int>(rank), partial, on(stream));
 }
 
+int cozyq_head_norm_rope(int device, const void* q, const void* k, int half, int64_t tokens, int q_heads,
+                         int k_heads, int width, int64_t q_token, int64_t q_head, int64_t k_token,
+                         int64_t k_head, int norm, const void* q_gain, const void* k_gain, int gain_wide,
+                         float eps, const float* cos, const float* sin, int64_t table_rows, int rotated,
+                         int interleaved, const int* positions, void* q_out, void* k_out, void* stream) {
+    if (tokens < 0 || tokens > cozyq::kMostTokens || q_heads < 0 || k_heads < 0 || q_heads > 4096 ||
+        k_heads > 4096 || width < 16 || width > 256 || width % 16 || rotated < 0 || rotated > width ||
+        rotated % 16)
+        return hipErrorInvalidValue;
+    if (tokens == 0 || q_heads + k_heads == 0) return hipSuccess;
+    if ((q_heads && (!q || !q_out || !aligned16(q) || !aligned16(q_out) || q_token % 8 || q_head % 8)) ||
+        (k_heads && (!k || !k_out || !aligned16(k) || !aligned16(k_out) || k_token % 8 || k_head % 8)) ||
+        !aligned16(q_gain) || !aligned16(k_gain))
+        return hipErrorInvalidValue;
+    if (rotated && (!cos || !sin || !aligned16(cos) || !aligned16(sin) || table_rows < 1 ||
+                    table_rows > cozyq::kMostTokens || (!positions && table_rows < tokens)))
+        return hipErrorInvalidValue;
+    const OnDevice guard(device);
+    if (guard.error() != hipSuccess) return guard.error();
+    return cozyq::head_norm_rope({static_cast<const uint16_t*>(q), static_cast<const uint16_t*>(k),
+                                  static_cast<uint16_t*>(q_out), static_cast<uint16_t*>(k_out), q_gain, k_gain,
+                                  cos, sin, positions, q_token, q_head, k_token, k_head, static_cast<int>(tokens),
+                                  q_heads, k_heads, width, rotated, static_cast<int>(table_rows), 0, eps, half != 0,
+                                  norm != 0, gain_wide != 0, interleaved != 0},
+                                 on(stream));
+}
+
+// log2 of a page's tokens, or -1 for a size that the cache does not take.
+static int page_shift(int page) {
+    for (int shift = 4; shift <= 8; ++shift)
+        if (page == 1 << shift) return shift;
+    return -1;
+}
+
+int cozyq_cache_most_requests(void) { return cozyq::kMostRequests; }
+
+int64_t cozyq_cache_runs(int64_t tokens, int requests, int page) {
+    if (tokens < 0 || tokens > cozyq::kMostTokens || requests < 0 || requests > cozyq::kMostRequests ||
+        page_shift(page) < 0)
+        return -1;
+    const int64_t runs = tokens / page + 2 * static_cast<int64_t>(requests);
+    return runs < tokens ? runs : tokens;
+}
+
+int cozyq_cache_plan(int device, int* table, int requests, int width, const int* free, int free_count,
+                     const int* spare, const int* held, const int* fresh, int64_t tokens, int page, int* starts,
+                     int* lengths, int* positions, int* requests_out, int* slots, int* runs, int* spare_out,
+                     void* stream) {
+    const int64_t most = cozyq_cache_runs(tokens, requests, page);
+    if (most < 0 || requests < 1 || width < 1 || width > cozyq::kMostTokens / page || free_count < 0)
+        return hipErrorInvalidValue;
+    if (!table || (!free && free_count) || !spare || !held || !fresh || !starts || !lengths || !spare_out ||
+        (tokens && (!positions || !requests_out || !slots || !runs || !aligned16(runs))))
+        return hipErrorInvalidValue;
+    const OnDevice guard(device);
+    if (guard.error() != hipSuccess) return guard.error();
+    return cozyq::cache_plan({table, free, spare, held, fresh, starts, lengths, positions, requests_out, slots, runs,
+                              spare_out, requests, width, free_count, static_cast<int>(tokens), static_cast<int>(most),
+                              page, page_shift(page)},
+                             on(stream));
+}
+
+static bool cache_shape(int pages, int heads, int page, int width) {
+    return pages >= 1 && heads >= 1 && heads <= 4096 && page_shift(page) >= 0 && pages <= cozyq::kMostTokens / page &&
+           (width == 64 || width == 128 || width == 256);
+}
+
+int cozyq_cache_append(int device, int fp8, const void* k, const void* v, int half, int64_t tokens, int64_t k_token,
+                       int64_t k_head, int64_t v_token, int64_t v_head, void* k_codes, void* v_codes, float* k_scale,
+                       float* v_scale, int pages, int heads, int page, int width, const int* runs, int64_t runs_most,
+                       void* stream) {
+    if (!cache_shape(pages, heads, page, width) || tokens < 0 || tokens > cozyq::kMostTokens || runs_most < 0 ||
+        runs_most > cozyq::kMostTokens)
+        return hipErrorInvalidValue;
+    if (tokens == 0 || runs_most == 0) return hipSuccess;
+    if (!k || !v || !aligned16(k) || !aligned16(v) || k_token % 8 || k_head % 8 || v_token % 8 || v_head % 8 ||
+        !k_codes || !v_codes || !aligned16(k_codes) || !aligned16(v_codes) || !k_scale || !v_scale || !runs ||
+        !aligned16(runs))
+        return hipErrorInvalidValue;
+    const OnDevice guard(device);
+    if (guard.error() != hipSuccess) return guard.error();
+    return cozyq::cache_append({static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v),
+                                static_cast<uint8_t*>(k_codes), static_cast<uint8_t*>(v_codes), k_scale, v_scale, runs,
+                                k_token, k_head, v_token, v_head, static_cast<int>(tokens),
+                                static_cast<int>(runs_most), pages, heads, width, page, half != 0},
+                               fp8 != 0, on(stream));
+}
+
+int cozyq_cache_read(int device, int fp8, const void* k_codes, const void* v_codes, const float* k_scale,
+                     const float* v_scale, int pages, int heads, int page, int width, const int* numbers,
+                     int64_t count, void* k_out, void* v_out, int half, void* stream) {
+    if (!cache_shape(pages, heads, page, width) || count < 0 || count > cozyq::kMostTokens) return hipErrorInvalidValue;
+    if (count == 0) return hipSuccess;
+    if (!k_codes || !v_codes || !aligned16(k_codes) || !aligned16(v_codes) || !k_scale || !v_scale || !numbers ||
+        !k_out || !v_out || !aligned16(k_out) || !aligned16(v_out))
+        return hipErrorInvalidValue;
+    const OnDevice guard(device);
+    if (guard.error() != hipSuccess) return guard.error();
+    return cozyq::cache_read({static_cast<const uint8_t*>(k_codes), static_cast<const uint8_t*>(v_codes), k_scale,
+                              v_scale, numbers, static_cast<uint16_t*>(k_out), static_cast<uint16_t*>(v_out),
+                              static_cast<int>(count), pages, heads, width, page, half != 0},
+                             fp8 != 0, on(stream));
+}
+
+static bool attend_shape(int64_t tokens, int q_heads, int requests, int table_width, int pages, int heads, int page,
+                         int width) {
+    return cache_shape(pages, heads, page, width) && tokens >= 0 && tokens <= cozyq::kMostTokens / 16 && q_heads >= 1 &&
+           q_heads <= 4096 && q_heads % heads == 0 && q_heads / heads <= 64 && requests >= 1 &&
+           requests <= cozyq::kMostRequests && table_width >= 1 && table_width <= cozyq::kMostTokens / page;
+}
+
+int64_t cozyq_cache_attend_workspace_bytes(int64_t tokens, int q_heads, int requests, int heads, int width,
+                                           int64_t most) {
+    if (!attend_shape(tokens, q_heads, requests, 1, 1, heads, 16, width) || most < 0) return -1;
+    return 0;
+}
+
+int cozyq_cache_attend(int device, int fp8, const void* q, int half, int64_t tokens, int q_heads, int64_t q_token,
+                       int64_t q_head, const void* k_codes, const void* v_codes, const float* k_scale,
+                       const float* v_scale, int pages, int heads, int page, int width, const int* table,
+                       int requests, int table_width, const int* starts, const int* lengths, int64_t most, float scale,
+                       int causal, int window, void* out, void* workspace, void* stream) {
+    if (!attend_shape(tokens, q_heads, requests, table_width, pages, heads, page, width) || most < 0 || window < 0 ||
+        (window && !causal))
+        return hipErrorInvalidValue;
+    if (tokens == 0) return hipSuccess;
+    if (!q || !aligned16(q) || q_token % 8 || q_head % 8 || !k_codes || !v_codes || !aligned16(k_codes) ||
+        !aligned16(v_codes) || !k_scale || !v_scale || !table || !starts || !lengths || !out || !aligned16(out))
+        return hipErrorInvalidValue;
+    const OnDevice guard(device);
+    if (guard.error() != hipSuccess) return guard.error();
+    return cozyq::cache_attend({static_cast<const uint16_t*>(q), static_cast<uint16_t*>(out),
+                                static_cast<const uint8_t*>(k_codes), static_cast<const uint8_t*>(v_codes), k_scale,
+                                v_scale, table, starts, lengths, q_token, q_head, static_cast<int>(tokens), requests,
+                                table_width, pages, heads, q_heads, q_heads / heads, width, page, page_shift(page),
+                                window, scale, half != 0, causal != 0},
+                               fp8 != 0, on(stream));
+}
+
 void cozyq_host_e4m3(const float* in, uint8_t* out, int64_t n) {
     for (int64_t i = 0; i < n; ++i) out[i] = cozyq::e4m3_rn(in[i]);
 }

@@ -297,6 +297,95 @@ hipError_t bake_stats(int form, const BakeStats& st, const float* up, const floa
 // out = each 256-group of down times H256 / 16; `groups` = rank · cols / 256.
 hipError_t rotate_factor(const float* down, float* out, int64_t groups, hipStream_t s);
 
+
+// Queries and keys [tokens, heads, width] (16-bit, rows `*_token` and heads `*_head` elements apart)
+// normed a head (RMS, eps inside the root, times `gain` [width] in x's type or, with gain_wide,
+// float32) and rotated over their first `rotated` elements by the cos / sin tables' row
+// positions[token] (or token), into contiguous q_out / k_out. `lanes` is the launcher's.
+struct HeadRows {
+    const uint16_t* q;
+    const uint16_t* k;
+    uint16_t* q_out;
+    uint16_t* k_out;
+    const void* q_gain;
+    const void* k_gain;
+    const float* cos;
+    const float* sin;
+    const int* positions;
+    int64_t q_token, q_head, k_token, k_head;
+    int tokens, q_heads, k_heads, width, rotated, table_rows, lanes;
+    float eps;
+    bool half, norm, gain_wide, interleaved;
+};
+hipError_t head_norm_rope(HeadRows rows, hipStream_t s);
+
+// The most rows, table rows or cache slots that the head and cache kernels index: int32 with room.
+constexpr int kMostTokens = 1 << 30;
+// The most requests a plan takes: four prefix sums of them in 64 KiB of LDS.
+constexpr int kMostRequests = 4000;
+// A step's plan (cozyq_cache_plan); page = 1 << shift.
+struct CachePlan {
+    int* table;
+    const int* free;
+    const int* spare;
+    const int* held;
+    const int* fresh;
+    int* starts;
+    int* lengths;
+    int* positions;
+    int* requests_out;
+    int* slots;
+    int* runs;
+    int* spare_out;
+    int requests, width, free_count, tokens, runs_most, page, shift;
+};
+hipError_t cache_plan(const CachePlan& p, hipStream_t s);
+// New keys and values into the pages of a plan's runs (cozyq_cache_append).
+struct CacheAppend {
+    const uint16_t* k;
+    const uint16_t* v;
+    uint8_t* k_codes;
+    uint8_t* v_codes;
+    float* k_scale;
+    float* v_scale;
+    const int* runs;
+    int64_t k_token, k_head, v_token, v_head;
+    int tokens, runs_most, pages, heads, width, page;
+    bool half;
+};
+hipError_t cache_append(const CacheAppend& p, bool fp8, hipStream_t s);
+// Listed pages as 16-bit numbers (cozyq_cache_read).
+struct CacheRead {
+    const uint8_t* k_codes;
+    const uint8_t* v_codes;
+    const float* k_scale;
+    const float* v_scale;
+    const int* numbers;
+    uint16_t* k_out;
+    uint16_t* v_out;
+    int count, pages, heads, width, page;
+    bool half;
+};
+hipError_t cache_read(const CacheRead& p, bool fp8, hipStream_t s);
+// Attention over the cache (cozyq_cache_attend): q [tokens, q_heads, head_width] against `heads` key
+// heads, `group` query heads each; table [requests, width].
+struct CacheAttend {
+    const uint16_t* q;
+    uint16_t* out;
+    const uint8_t* k_codes;
+    const uint8_t* v_codes;
+    const float* k_scale;
+    const float* v_scale;
+    const int* table;
+    const int* starts;
+    const int* lengths;
+    int64_t q_token, q_head;
+    int tokens, requests, width, pages, heads, q_heads, group, head_width, page, shift, window;
+    float scale;
+    bool half, causal;
+};
+hipError_t cache_attend(const CacheAttend& p, bool fp8, hipStream_t s);
+
 }  // namespace cozyq
 
 namespace cozyq {

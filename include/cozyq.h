@@ -477,6 +477,85 @@ int cozyq_bake_stats(int device, int form, const void* before, const void* after
 int cozyq_bake_rotate_factor(int device, const float* down, float* out, int64_t rank,
                              int64_t cols, void* stream);
 
+/* Queries and keys between the QKV projection and attention (reference: its fused RMS norm and rotary
+ * kernel, kernels/csrc/norm/rms_rope.cu, is outside the quantized-linear path): every head of q
+ * [tokens, q_heads, width] and k [tokens, k_heads, width] (16-bit, rows *_token and heads *_head
+ * elements apart, both multiples of 8, elements dense), in float32, rounded once:
+ *   y = x · rsqrt(mean(x²) + eps) · gain  (norm; q_gain / k_gain [width] or NULL, in x's type or, with
+ *   gain_wide, float32), then the first `rotated` elements in pairs, halves (i, i + rotated/2) or with
+ *   `interleaved` neighbours (2i, 2i + 1): (a, b) -> (a·cos − b·sin, b·cos + a·sin), with cos / sin
+ *   float32 [table_rows, rotated/2] of row positions[token] (int32; NULL: the token's own number; one
+ *   outside the table reads its nearest row).
+ * q_out, k_out: contiguous. width % 16 == 0 up to 256, rotated % 16 == 0 up to width (0: none).
+ * q_heads or k_heads may be 0. Pointers of 16-byte alignment. */
+int cozyq_head_norm_rope(int device, const void* q, const void* k, int half, int64_t tokens, int q_heads,
+                         int k_heads, int width, int64_t q_token, int64_t q_head, int64_t k_token,
+                         int64_t k_head, int norm, const void* q_gain, const void* k_gain, int gain_wide,
+                         float eps, const float* cos, const float* sin, int64_t table_rows, int rotated,
+                         int interleaved, const int* positions, void* q_out, void* k_out, void* stream);
+
+/* The paged 8-bit cache of keys and values (no reference counterpart: the reference's LM keeps a static
+ * 16-bit cache). `pages` pages of `page` tokens (16, 32, 64, 128 or 256) of every key head: k_codes
+ * [pages, heads, page, width], v_codes [pages, heads, width, page] (values stand transposed), int8 or
+ * E4M3 bytes, 16-byte aligned; k_scale, v_scale float32 [pages, heads], positive; value = code · scale.
+ * width 64, 128 or 256.
+ *
+ * The step's plan, from the requests' lengths, on the GPU. `held` [requests] int32: tokens each holds;
+ * `fresh` [requests] int32: tokens it brings. The step's rows are the requests' new tokens one request
+ * after another; `tokens` rows in all, those past the last request's belonging to none (a request whose
+ * tokens would pass the last row has its count cut there). A page that a request does not hold yet comes
+ * off the end of `free` [free_count], of which spare[0] are free, in row order. Negative counts are 0.
+ * Writes: the new pages into `table` [requests, width]; starts [requests + 1] (each request's first
+ * row), lengths [requests] (tokens held after the step); positions, requests_out, slots [tokens] (the
+ * token's position, request and page · page size + place in the page; 0, -1 and -1 for a row of none, slot
+ * -1 where no page was left); runs [cozyq_cache_runs(tokens, requests, page), 4] (a page's new tokens:
+ * first row, count, page or -1, first place in the page; 0, 0, -1, 0 past the last); spare_out [2] (free
+ * pages left; pages wanted and not got, for want of free ones or of room in `table`). cozyq_cache_runs:
+ * min(tokens, tokens / page + 2 · requests), -1 for a bad argument. Up to cozyq_cache_most_requests()
+ * requests. */
+int cozyq_cache_most_requests(void);
+int64_t cozyq_cache_runs(int64_t tokens, int requests, int page);
+int cozyq_cache_plan(int device, int* table, int requests, int width, const int* free, int free_count,
+                     const int* spare, const int* held, const int* fresh, int64_t tokens, int page, int* starts,
+                     int* lengths, int* positions, int* requests_out, int* slots, int* runs, int* spare_out,
+                     void* stream);
+
+/* New keys and values [tokens, heads, width] (16-bit, strides as cozyq_head_norm_rope's) into the pages
+ * of `runs` [runs_most, 4]. For each run and head, keys and values apart: scale = max(the page's own,
+ * amax / 127 or 448, 1e-12), without the page's own where the run begins the page (first place 0); code =
+ * x / scale rounded to nearest even. Where the scale grows, the codes that the page holds are rounded
+ * again as code · (old / new); a page that a run begins is cleared past its tokens. An infinity or NaN
+ * makes that page's scale for the head so (every row that sees the page is then NaN); codes stay
+ * finite. Runs whose page is not in the cache are skipped. */
+int cozyq_cache_append(int device, int fp8, const void* k, const void* v, int half, int64_t tokens, int64_t k_token,
+                       int64_t k_head, int64_t v_token, int64_t v_head, void* k_codes, void* v_codes, float* k_scale,
+                       float* v_scale, int pages, int heads, int page, int width, const int* runs, int64_t runs_most,
+                       void* stream);
+
+/* Pages `numbers` [count] as numbers: k_out, v_out [count, heads, page, width] 16-bit, code · scale
+ * rounded once; zeros for a number that is no page of the cache. */
+int cozyq_cache_read(int device, int fp8, const void* k_codes, const void* v_codes, const float* k_scale,
+                     const float* v_scale, int pages, int heads, int page, int width, const int* numbers,
+                     int64_t count, void* k_out, void* v_out, int half, void* stream);
+
+/* Attention over the cache: q [tokens, q_heads, width] (16-bit, strides as above), query heads in equal
+ * groups of up to 64 a key head; request r's rows are starts[r] .. starts[r + 1] − 1, its last tokens of
+ * lengths[r]. out [tokens, q_heads, width], contiguous, in q's type: softmax(scale · q·k) · v over the
+ * tokens that the row sees: causal, those up to its own, with a window > 0 the last `window` of them;
+ * otherwise all of the request's. Tokens whose table entry is no page of the cache are not seen; a row
+ * that sees none, or belongs to no request, is 0. What pages hold past a request's tokens is not read
+ * into any result. `most`: the most rows a request has, as far as the caller knows (0: not at all); it
+ * sets the launch's shape and speed, never its results. The workspace is of
+ * cozyq_cache_attend_workspace_bytes bytes, uninitialised (NULL where that is 0; -1 for a bad
+ * argument). */
+int64_t cozyq_cache_attend_workspace_bytes(int64_t tokens, int q_heads, int requests, int heads, int width,
+                                           int64_t most);
+int cozyq_cache_attend(int device, int fp8, const void* q, int half, int64_t tokens, int q_heads, int64_t q_token,
+                       int64_t q_head, const void* k_codes, const void* v_codes, const float* k_scale,
+                       const float* v_scale, int pages, int heads, int page, int width, const int* table,
+                       int requests, int table_width, const int* starts, const int* lengths, int64_t most, float scale,
+                       int causal, int window, void* out, void* workspace, void* stream);
+
 /* Test entries (no reference counterpart): the kernels' scalar conversions run on the host,
  * so CPU tests can hold the device code's arithmetic against torch without a GPU. */
 void cozyq_host_e4m3(const float* in, uint8_t* out, int64_t n);
