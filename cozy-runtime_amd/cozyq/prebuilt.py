@@ -1227,7 +1227,8 @@ class Prebuilt:
         if off_card(self.index, cache.k, cache.v, cache.k_scale, cache.v_scale, q, table, starts, lengths):
             raise ValueError(f"attend: every tensor must be on cuda:{self.index}")
         out = torch.empty((tokens, q_heads, width), dtype=q.dtype, device=q.device)
-        size = self._lib.cozyq_cache_attend_workspace_bytes(tokens, q_heads, requests, heads, width, plan.most)
+        size = self._lib.cozyq_cache_attend_workspace_bytes(tokens, q_heads, requests, heads, page, width,
+                                                            table_width, plan.most)
         work = torch.empty(size, dtype=torch.uint8, device=q.device) if size > 0 else None
         code = self._lib.cozyq_cache_attend(
             self.index, fp8, q.data_ptr(), half, tokens, q_heads, q_token, q_head, cache.k.data_ptr(),

@@ -802,10 +802,10 @@ static bool attend_shape(int64_t tokens, int q_heads, int requests, int table_wi
            requests <= cozyq::kMostRequests && table_width >= 1 && table_width <= cozyq::kMostTokens / page;
 }
 
-int64_t cozyq_cache_attend_workspace_bytes(int64_t tokens, int q_heads, int requests, int heads, int width,
-                                           int64_t most) {
-    if (!attend_shape(tokens, q_heads, requests, 1, 1, heads, 16, width) || most < 0) return -1;
-    return 0;
+int64_t cozyq_cache_attend_workspace_bytes(int64_t tokens, int q_heads, int requests, int heads, int page, int width,
+                                           int table_width, int64_t most) {
+    if (!attend_shape(tokens, q_heads, requests, table_width, 1, heads, page, width) || most < 0) return -1;
+    return cozyq::cache_attend_work(tokens, q_heads / heads, requests, heads, table_width, page, width, most);
 }
 
 int cozyq_cache_attend(int device, int fp8, const void* q, int half, int64_t tokens, int q_heads, int64_t q_token,
@@ -818,7 +818,10 @@ int cozyq_cache_attend(int device, int fp8, const void* q, int half, int64_t tok
         return hipErrorInvalidValue;
     if (tokens == 0) return hipSuccess;
     if (!q || !aligned16(q) || q_token % 8 || q_head % 8 || !k_codes || !v_codes || !aligned16(k_codes) ||
-        !aligned16(v_codes) || !k_scale || !v_scale || !table || !starts || !lengths || !out || !aligned16(out))
+        !aligned16(v_codes) || !k_scale || !v_scale || !table || !starts || !lengths || !out || !aligned16(out) ||
+        !aligned16(workspace))
+        return hipErrorInvalidValue;
+    if (!workspace && cozyq_cache_attend_workspace_bytes(tokens, q_heads, requests, heads, page, width, table_width, most))
         return hipErrorInvalidValue;
     const OnDevice guard(device);
     if (guard.error() != hipSuccess) return guard.error();
@@ -826,8 +829,8 @@ int cozyq_cache_attend(int device, int fp8, const void* q, int half, int64_t tok
                                 static_cast<const uint8_t*>(k_codes), static_cast<const uint8_t*>(v_codes), k_scale,
                                 v_scale, table, starts, lengths, q_token, q_head, static_cast<int>(tokens), requests,
                                 table_width, pages, heads, q_heads, q_heads / heads, width, page, page_shift(page),
-                                window, scale, half != 0, causal != 0},
-                               fp8 != 0, on(stream));
+                                window, scale, half != 0, causal != 0, static_cast<float*>(workspace), 0, 0},
+                               most, fp8 != 0, on(stream));
 }
 
 void cozyq_host_e4m3(const float* in, uint8_t* out, int64_t n) {

@@ -548,8 +548,8 @@ int cozyq_cache_read(int device, int fp8, const void* k_codes, const void* v_cod
  * sets the launch's shape and speed, never its results. The workspace is of
  * cozyq_cache_attend_workspace_bytes bytes, uninitialised (NULL where that is 0; -1 for a bad
  * argument). */
-int64_t cozyq_cache_attend_workspace_bytes(int64_t tokens, int q_heads, int requests, int heads, int width,
-                                           int64_t most);
+int64_t cozyq_cache_attend_workspace_bytes(int64_t tokens, int q_heads, int requests, int heads, int page, int width,
+                                           int table_width, int64_t most);
 int cozyq_cache_attend(int device, int fp8, const void* q, int half, int64_t tokens, int q_heads, int64_t q_token,
                        int64_t q_head, const void* k_codes, const void* v_codes, const float* k_scale,
                        const float* v_scale, int pages, int heads, int page, int width, const int* table,
