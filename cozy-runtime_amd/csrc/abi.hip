@@ -829,7 +829,7 @@ int cozyq_cache_attend(int device, int fp8, const void* q, int half, int64_t tok
                                 static_cast<const uint8_t*>(k_codes), static_cast<const uint8_t*>(v_codes), k_scale,
                                 v_scale, table, starts, lengths, q_token, q_head, static_cast<int>(tokens), requests,
                                 table_width, pages, heads, q_heads, q_heads / heads, width, page, page_shift(page),
-                                window, scale, half != 0, causal != 0, static_cast<float*>(workspace), 0, 0},
+                                window, scale, half != 0, causal != 0, static_cast<float*>(workspace)},
                                most, fp8 != 0, on(stream));
 }
 

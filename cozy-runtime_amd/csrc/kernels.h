@@ -383,11 +383,10 @@ struct CacheAttend {
     int tokens, requests, width, pages, heads, q_heads, group, head_width, page, shift, window;
     float scale;
     bool half, causal;
-    float* work;        // cache_attend_work bytes
-    int tiles, shares;  // the launcher's
+    float* work;  // cache_attend_work bytes
 };
 int64_t cache_attend_work(int64_t tokens, int group, int requests, int heads, int columns, int page, int width, int64_t most);
-hipError_t cache_attend(CacheAttend p, int64_t most, bool fp8, hipStream_t s);
+hipError_t cache_attend(const CacheAttend& p, int64_t most, bool fp8, hipStream_t s);
 
 }  // namespace cozyq
 

@@ -94,10 +94,17 @@ __device__ __forceinline__ T wave_prefix(T x) {
     return x;
 }
 
-// ------------------------------------------------------------------- few rows a request
+// --------------------------------------------------------------------- sharing the work out
 
-constexpr int kStep = 64;       // tokens a wave takes at a time
+constexpr int kStep = 64;       // tokens taken at a time
 constexpr int kMinSteps = 16;   // steps a workgroup takes at the least
+
+// Which requests a launch takes: those of more than `over` and up to `upto` rows, in row tiles shared
+// out over `shares` workgroups a head.
+struct Part {
+    int over, upto, shares;
+    float* work;  // places of kRows · (width + 4) floats: a row's sums, its reference, its denominator
+};
 
 // A request's part of the work: row tiles, and the 64-token steps that any of its rows sees.
 struct Extent {
@@ -105,56 +112,91 @@ struct Extent {
 };
 
 template <int kRows>
-__device__ __forceinline__ Extent extent(const CacheAttend& p, int r) {
-    const int fresh = row_start(p, r + 1) - row_start(p, r), length = p.lengths[r];
+__device__ __forceinline__ Extent extent(const CacheAttend& p, const Part& part, int r) {
+    const int fresh = row_start(p, r + 1) - row_start(p, r), length = p.lengths[r], rows = fresh * p.group;
+    if (rows <= part.over || rows > part.upto) return {0, 0};
     const int low = p.window > 0 ? max(0, length - fresh + 1 - p.window) : 0;
     const int steps = (max(length, 0) + kStep - 1) / kStep - low / kStep;
-    return {(fresh * p.group + kRows - 1) / kRows, max(steps, 0)};
+    return {(rows + kRows - 1) / kRows, max(steps, 0)};
 }
 
-// Tile `tile` of request `request`, its steps split in `splits` workgroups, this one number `split`,
-// whose partial results stand `split` places after place `first`.
+// Tile `tile` of request `request`, its steps split over `splits` workgroups, of which this is number
+// `split`; with more than one they leave their sums in that many places from `place` on.
 struct Share {
-    int request, tile, split, splits, first;
+    int request, tile, split, splits, place;
 };
 
 // All the row tiles' steps are shared out evenly: with N steps in all (a head), a workgroup takes
-// c = max(kMinSteps, ⌈N / shares⌉) of one row tile's, so that there are at most shares + tiles
-// workgroups, whatever the requests' lengths are, and the host can size the launch without knowing
-// them. Finds workgroup `id`'s share (kById), or row tile `id`'s first; false past the last. Every wave
-// scans all requests, 64 at a time.
+// c = max(kMinSteps, N / shares) of one row tile's, so that there are at most shares + tiles workgroups
+// and at most 2 · shares places (a tile of more than c steps splits into less than 2 · steps / c),
+// whatever the requests' lengths are: the host sizes the launch and the workspace without knowing them.
+// Finds workgroup `id`'s share (kById), or row tile `id`'s first; false past the last. A request's last
+// tile comes first: where causal it has the most to do. Every wave scans all requests, 64 at a time.
 template <int kRows, bool kById>
-__device__ bool find_share(const CacheAttend& p, int id, Share& out) {
+__device__ bool find_share(const CacheAttend& p, const Part& part, int id, Share& out) {
     const int lane = threadIdx.x & 63;
     float work = 0.0f;  // in float32, which no number of steps overflows; the margin is over its rounding
     for (int base = 0; base < p.requests; base += 64) {
         Extent e = {0, 0};
-        if (base + lane < p.requests) e = extent<kRows>(p, base + lane);
+        if (base + lane < p.requests) e = extent<kRows>(p, part, base + lane);
         const float sum = wave_prefix(static_cast<float>(e.tiles) * static_cast<float>(e.steps));
         work += __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, sum), 63));
     }
-    const int c = max(kMinSteps, static_cast<int>(work * 1.001f / static_cast<float>(p.shares)) + 1);
-    int groups_before = 0, tiles_before = 0;
+    const int c = max(kMinSteps, static_cast<int>(work * 1.001f / static_cast<float>(part.shares)) + 1);
+    int ids_before = 0, places_before = 0;
     for (int base = 0; base < p.requests; base += 64) {
         Extent e = {0, 0};
-        if (base + lane < p.requests) e = extent<kRows>(p, base + lane);
+        if (base + lane < p.requests) e = extent<kRows>(p, part, base + lane);
         const int splits = max(1, (e.steps + c - 1) / c);
-        const int groups = wave_prefix(e.tiles * splits), tiles = wave_prefix(e.tiles);
-        const int mine = kById ? groups_before + groups : tiles_before + tiles;
-        const uint64_t past = __ballot(mine > id);
+        const int ids = wave_prefix(kById ? e.tiles * splits : e.tiles);
+        const int places = wave_prefix(splits > 1 ? e.tiles * splits : 0);
+        const uint64_t past = __ballot(ids_before + ids > id);
         if (past) {
             const int at = __ffsll(static_cast<unsigned long long>(past)) - 1;
             const int n = __builtin_amdgcn_readlane(splits, at), t = __builtin_amdgcn_readlane(e.tiles, at);
-            const int g0 = groups_before + __builtin_amdgcn_readlane(groups, at) - t * n;
-            const int t0 = tiles_before + __builtin_amdgcn_readlane(tiles, at) - t;
-            const int tile = kById ? (id - g0) / n : id - t0;
-            out = {base + at, tile, kById ? (id - g0) % n : 0, n, g0 + tile * n};
+            const int from = id - ids_before - __builtin_amdgcn_readlane(ids, at) + (kById ? t * n : t);
+            const int tile = kById ? from / n : from;
+            const int first = places_before + __builtin_amdgcn_readlane(places, at) - (n > 1 ? t * n : 0);
+            out = {base + at, t - 1 - tile, kById ? from % n : 0, n, first + tile * n};
             return true;
         }
-        groups_before += __builtin_amdgcn_readlane(groups, 63);
-        tiles_before += __builtin_amdgcn_readlane(tiles, 63);
+        ids_before += __builtin_amdgcn_readlane(ids, 63);
+        places_before += __builtin_amdgcn_readlane(places, 63);
     }
     return false;
+}
+
+// Rows of the step that no request has (past the last one's) are zeros: the workgroups past the last
+// share, one at the least, write them.
+__device__ void clear_rest(const CacheAttend& p, int width, int group, int groups) {
+    const int64_t row = static_cast<int64_t>(p.q_heads) * width / 8;
+    const int64_t from = row_start(p, p.requests) * row, to = p.tokens * row;
+    for (int64_t i = from + static_cast<int64_t>(group) * blockDim.x + threadIdx.x; i < to; i += static_cast<int64_t>(groups) * blockDim.x)
+        reinterpret_cast<i32x4*>(p.out)[i] = i32x4{0, 0, 0, 0};
+}
+
+__device__ void clear_rest(const CacheAttend& p, int width) {
+    const int groups = min(static_cast<int>(gridDim.x), 256), mine = gridDim.x - 1 - blockIdx.x;
+    if (mine < groups) clear_rest(p, width, mine, groups);
+}
+
+// Where a row tile's tokens lie: steps [begin, end) of the share; rows see tokens from low_least on and
+// before high_most, and all of them those in [low_most, high_least).
+struct Span {
+    int begin, end, low_least, low_most, high_least, high_most;
+};
+
+__device__ __forceinline__ Span span_of(const CacheAttend& p, int row0, int rows, int fresh, int length, int split, int splits) {
+    const int before = length - fresh, t0 = row0 / p.group, t1 = (rows - 1) / p.group;
+    Span s;
+    s.low_least = p.window > 0 ? max(0, before + t0 + 1 - p.window) : 0;
+    s.low_most = p.window > 0 ? max(0, before + t1 + 1 - p.window) : 0;
+    s.high_least = p.causal ? before + t0 + 1 : length;
+    s.high_most = p.causal ? before + t1 + 1 : length;
+    const int from = s.low_least / kStep, steps = max(0, (s.high_most + kStep - 1) / kStep - from);
+    s.begin = from + static_cast<int>(static_cast<int64_t>(steps) * split / splits);
+    s.end = from + static_cast<int>(static_cast<int64_t>(steps) * (split + 1) / splits);
+    return s;
 }
 
 // What a workgroup keeps of a page of its tokens: its number (-1: none of the cache's), the keys'
@@ -163,6 +205,46 @@ struct PageScales {
     int page;
     float keys, values_log, values_inv;
 };
+
+constexpr int kStage = 128;  // steps whose pages a workgroup stages at a time
+constexpr int kEntries = kStage * kStep / 16 + 1;
+
+// Stages the pages of steps [from, to) of a request, the first of them number `page_first`.
+__device__ __forceinline__ void stage_pages(const CacheAttend& p, PageScales* entries, const int* table, int length, int kv,
+                                            int page_first, int to) {
+    const int pages = ((to * kStep - 1) >> p.shift) - page_first + 1;
+    for (int i = threadIdx.x; i < pages; i += blockDim.x) {
+        const int index = page_first + i;
+        const int page = index < p.width && (index << p.shift) < length ? table[index] : -1;
+        PageScales e = {-1, 0.0f, 0.0f, 0.0f};
+        if (page >= 0 && page < p.pages) {
+            const int64_t at = static_cast<int64_t>(page) * p.heads + kv;
+            const float values = nan_max(or_nan(p.v_scale[at]), 1e-30f);
+            e = {page, or_nan(p.k_scale[at]), __builtin_amdgcn_logf(values), 1.0f / values};
+        }
+        entries[i] = e;
+    }
+}
+
+// The largest magnitude's bits of a query row -> the exponents of the power of two that brings it to
+// about 2^12 and of its inverse, both of normal numbers.
+__device__ __forceinline__ void row_unit(uint32_t most, float& unit, float& down) {
+    const int e = min(max(static_cast<int>(most >> 23) - 12, 10), 240);
+    unit = float_of(static_cast<uint32_t>(e) << 23);
+    down = float_of(static_cast<uint32_t>(254 - e) << 23);
+}
+
+__device__ __forceinline__ void widen8(const CacheAttend& p, const uint16_t* x, float* v, uint32_t& most) {
+    const i32x4 raw = *reinterpret_cast<const i32x4*>(x);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const uint16_t h = static_cast<uint16_t>(static_cast<uint32_t>(raw[i / 2]) >> (16 * (i & 1)));
+        v[i] = p.half ? widen<true>(h) : widen<false>(h);
+        most = max(most, bits_of(v[i]) & 0x7fffffffu);
+    }
+}
+
+// ------------------------------------------------------------------------ few rows a request
 
 // Four waves take a row tile of 16 rows (kTiles of them) of one key head, the heads that share it token
 // by token, over the workgroup's share of its tokens: each wave every fourth step of 64. Both products
@@ -174,16 +256,18 @@ struct PageScales {
 // unit; nothing of the cache passes through LDS but its pages' numbers and scales, read once a share.
 // A step's keys are loaded over the previous step's second product and its values over its first.
 template <int kWidth, int kTiles, bool kFp8>
-__global__ __launch_bounds__(256, kWidth == 256 ? 1 : 2) void few_kernel(CacheAttend p) {
+__global__ __launch_bounds__(256, kWidth == 256 ? 1 : 2) void few_kernel(CacheAttend p, Part part, bool clears) {
     constexpr int kWaves = 4, kBlocks = kWidth / 64, kOut = kWidth / 16, kRows = 16 * kTiles;
-    constexpr int kStage = 128, kEntries = kStage * kStep / 16 + 1;
     __shared__ PageScales entries[kEntries];
     __shared__ float merged[kWaves][16][kWidth + 4];
     __shared__ float tops[kWaves][16], totals[kWaves][16];
     const int thread = threadIdx.x, lane = thread & 63, wave = thread >> 6, col = lane & 15, g = lane >> 4;
     const int kv = blockIdx.x % p.heads, id = blockIdx.x / p.heads;
     Share share;
-    if (!find_share<kRows, true>(p, id, share)) return;
+    if (!find_share<kRows, true>(p, part, id, share)) {
+        if (clears) clear_rest(p, kWidth);
+        return;
+    }
     const int first = row_start(p, share.request), fresh = row_start(p, share.request + 1) - first;
     const int length = p.lengths[share.request], rows = fresh * p.group;
 
@@ -200,14 +284,7 @@ __global__ __launch_bounds__(256, kWidth == 256 ? 1 : 2) void few_kernel(CacheAt
         high[n] = live[n] ? (p.causal ? position + 1 : length) : 0;
         low[n] = live[n] ? (p.window > 0 ? max(0, position + 1 - p.window) : 0) : 0x7fffffff;
     }
-    const int t_first = kRows * share.tile / p.group, t_last = min(rows, kRows * (share.tile + 1)) - 1;
-    const int low_least = p.window > 0 ? max(0, length - fresh + t_first + 1 - p.window) : 0;
-    const int low_most = p.window > 0 ? max(0, length - fresh + t_last / p.group + 1 - p.window) : 0;
-    const int high_least = p.causal ? length - fresh + t_first + 1 : length;
-    const int high_most = p.causal ? length - fresh + t_last / p.group + 1 : length;
-    const int steps_from = low_least / kStep, steps = max(0, (high_most + kStep - 1) / kStep - steps_from);
-    const int begin = steps_from + static_cast<int>(static_cast<int64_t>(steps) * share.split / share.splits);
-    const int end = steps_from + static_cast<int>(static_cast<int64_t>(steps) * (share.split + 1) / share.splits);
+    const Span span = span_of(p, kRows * share.tile, min(rows, kRows * (share.tile + 1)), fresh, length, share.split, share.splits);
 
     // Each row brought to a largest magnitude of about 2^12; a lane holds elements 64b + 16g .. + 15 of
     // each block of 64, as two operands.
@@ -216,28 +293,17 @@ __global__ __launch_bounds__(256, kWidth == 256 ? 1 : 2) void few_kernel(CacheAt
 #pragma unroll
     for (int n = 0; n < kTiles; ++n) {
         const uint16_t* x = p.q + (first + token[n]) * p.q_token + head[n] * p.q_head;
-        float v[kBlocks][16];
+        float v[kBlocks][16], unit, down;
         uint32_t most = 0;
 #pragma unroll
         for (int b = 0; b < kBlocks; ++b) {
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                const i32x4 raw = *reinterpret_cast<const i32x4*>(x + 64 * b + 16 * g + 8 * c);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const uint16_t h = static_cast<uint16_t>(static_cast<uint32_t>(raw[i / 2]) >> (16 * (i & 1)));
-                    const float f = p.half ? widen<true>(h) : widen<false>(h);
-                    v[b][8 * c + i] = f;
-                    most = max(most, bits_of(f) & 0x7fffffffu);
-                }
-            }
+            widen8(p, x + 64 * b + 16 * g, v[b], most);
+            widen8(p, x + 64 * b + 16 * g + 8, v[b] + 8, most);
         }
         most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), 16)));
         most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), 32)));
-        // 2^(exponent − 12) and its inverse, both normal numbers.
-        const int e = min(max(static_cast<int>(most >> 23) - 12, 10), 240);
-        sharp[n] = float_of(static_cast<uint32_t>(e) << 23) * p.scale * kLog2e;
-        const float down = float_of(static_cast<uint32_t>(254 - e) << 23);
+        row_unit(most, unit, down);
+        sharp[n] = unit * p.scale * kLog2e;
 #pragma unroll
         for (int b = 0; b < kBlocks; ++b) {
 #pragma unroll
@@ -264,22 +330,11 @@ __global__ __launch_bounds__(256, kWidth == 256 ? 1 : 2) void few_kernel(CacheAt
     const int64_t page_bytes = static_cast<int64_t>(p.heads) * p.page * kWidth;
 
     i32x4 kc[4][kBlocks], vc[kOut];
-    for (int stage = begin; stage < end; stage += kStage) {
-        const int stage_end = min(end, stage + kStage);
+    for (int stage = span.begin; stage < span.end; stage += kStage) {
+        const int stage_end = min(span.end, stage + kStage);
         const int page_first = stage * kStep >> p.shift;
-        const int pages = ((stage_end * kStep - 1) >> p.shift) - page_first + 1;
-        if (stage != begin) __syncthreads();
-        for (int i = thread; i < pages; i += 256) {
-            const int index = page_first + i;
-            const int page = index < p.width && (index << p.shift) < length ? table[index] : -1;
-            PageScales e = {-1, 0.0f, 0.0f, 0.0f};
-            if (page >= 0 && page < p.pages) {
-                const int64_t at = static_cast<int64_t>(page) * p.heads + kv;
-                const float values = nan_max(or_nan(p.v_scale[at]), 1e-30f);
-                e = {page, or_nan(p.k_scale[at]), __builtin_amdgcn_logf(values), 1.0f / values};
-            }
-            entries[i] = e;
-        }
+        if (stage != span.begin) __syncthreads();
+        stage_pages(p, entries, table, length, kv, page_first, stage_end);
         __syncthreads();
 
         const auto load_keys = [&](int step) {
@@ -307,7 +362,7 @@ __global__ __launch_bounds__(256, kWidth == 256 ? 1 : 2) void few_kernel(CacheAt
         for (; step < stage_end; step += kWaves) {
             const int t0 = step * kStep, mine = t0 + 16 * g;
             const PageScales page = entries[(mine >> p.shift) - page_first];
-            const bool whole = t0 >= low_most && t0 + kStep <= high_least && __all(page.page >= 0);
+            const bool whole = t0 >= span.low_most && t0 + kStep <= span.high_least && __all(page.page >= 0);
             f32x4 s[kTiles][4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -426,110 +481,389 @@ __global__ __launch_bounds__(256, kWidth == 256 ? 1 : 2) void few_kernel(CacheAt
                 const int t = (row0 + r) / p.group, h = kv * p.group + (row0 + r) - t * p.group;
                 store_row(p, first + t, h, kWidth, d, v, sum);
             } else {
-                const int64_t at = (static_cast<int64_t>(share.first + share.split) * p.heads + kv) * kRows + 16 * n + r;
-                *reinterpret_cast<f32x4*>(p.work + at * (kWidth + 4) + d) = v;
+                float* to = part.work + ((static_cast<int64_t>(share.place + share.split) * p.heads + kv) * kRows + 16 * n + r) * (kWidth + 4);
+                *reinterpret_cast<f32x4*>(to + d) = v;
                 if (d == 0) {
-                    p.work[at * (kWidth + 4) + kWidth] = best;
-                    p.work[at * (kWidth + 4) + kWidth + 1] = sum;
+                    to[kWidth] = best;
+                    to[kWidth + 1] = sum;
                 }
             }
         }
     }
 }
 
-// Joins the parts of the row tiles that several workgroups took: one workgroup a row tile and head,
-// every part brought to the largest reference, in the order of their tokens.
-template <int kWidth, int kTiles>
-__global__ __launch_bounds__(256) void join_kernel(CacheAttend p) {
-    constexpr int kRows = 16 * kTiles;
-    const int kv = blockIdx.y;
+// ----------------------------------------------------------------------- many rows a request
+
+// A step's keys and values as f16 in LDS, in 16-byte chunks whose place in a row is exclusive-or'ed with
+// the row's number, so that the eight rows that a read of 128 bytes takes lie in different banks.
+// Row m of a half's 32 keys holds token π(m), m with bits 2 and 3 exchanged.
+__device__ __forceinline__ int exchanged(int m) { return (m & ~12) | ((m & 4) << 1) | ((m & 8) >> 1); }
+
+// kWaves waves take a tile of 32 rows each of one key head, and the workgroup's share of its tokens 64 at
+// a time: codes become f16 once for all of them, on their way through registers into LDS, a step ahead of
+// their use. Products as in few_kernel, on v_mfma_f32_32x32x16_f16: lane l holds row l%32, and with row m of
+// the keys at token π(m), score register 8a + e of half h = l/32 is that of token 16a + 8h + e, in the order
+// that the second product reads its weights in. Bytes past the request's tokens and pages that the cache has
+// not become zeros on the way to LDS.
+template <int kWidth, int kWaves, bool kFp8>
+__global__ __launch_bounds__(64 * kWaves, kWidth == 256 ? 1 : 2) void many_kernel(CacheAttend p, Part part, bool clears) {
+    constexpr int kRows = 32 * kWaves, kThreads = 64 * kWaves, kOut = kWidth / 32, kDepth = kWidth / 16;
+    constexpr int kKeyBytes = kStep * kWidth * 2, kChunks = kStep * kWidth / 16 / kThreads;
+    __shared__ PageScales entries[kEntries];
+    __shared__ __attribute__((aligned(16))) uint8_t tiles[2][2 * kKeyBytes];
+    const int thread = threadIdx.x, lane = thread & 63, wave = thread >> 6, col = lane & 31, h = lane >> 5;
+    const int kv = blockIdx.x % p.heads, id = blockIdx.x / p.heads;
     Share share;
-    if (!find_share<kRows, false>(p, blockIdx.x, share) || share.splits == 1) return;
-    const int first = row_start(p, share.request), rows = (row_start(p, share.request + 1) - first) * p.group;
-    const int row0 = kRows * share.tile, count = min(kRows, rows - row0);
-    for (int i = threadIdx.x; i < count * (kWidth / 4); i += 256) {
-        const int r = i / (kWidth / 4), d = 4 * (i - r * (kWidth / 4));
-        const float* part = p.work + ((static_cast<int64_t>(share.first) * p.heads + kv) * kRows + r) * (kWidth + 4);
-        const int64_t next = static_cast<int64_t>(p.heads) * kRows * (kWidth + 4);
-        float best = kNoScore, sum = 0.0f;
-        for (int s = 0; s < share.splits; ++s) best = nan_max(best, part[s * next + kWidth]);
-        f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (int s = 0; s < share.splits; ++s) {
-            const float factor = __builtin_amdgcn_exp2f(part[s * next + kWidth] - best);
-            const f32x4 one = *reinterpret_cast<const f32x4*>(part + s * next + d);
+    if (!find_share<kRows, true>(p, part, id, share)) {
+        if (clears) clear_rest(p, kWidth);
+        return;
+    }
+    const int first = row_start(p, share.request), fresh = row_start(p, share.request + 1) - first;
+    const int length = p.lengths[share.request], rows = fresh * p.group;
+    const int row0 = kRows * share.tile, mine0 = row0 + 32 * wave, row = mine0 + col;
+    const Span span = span_of(p, row0, min(rows, row0 + kRows), fresh, length, share.split, share.splits);
+    // The wave's own rows; one without rows only helps to load.
+    const bool busy = mine0 < rows;
+    const Span own = span_of(p, busy ? mine0 : 0, min(rows, mine0 + 32), fresh, length, 0, 1);
+    const bool live = row < rows;
+    const int token = live ? row / p.group : 0, head = kv * p.group + (live ? row - token * p.group : 0);
+    const int position = length - fresh + token;
+    const int high = live ? (p.causal ? position + 1 : length) : 0;
+    const int low = live ? (p.window > 0 ? max(0, position + 1 - p.window) : 0) : 0x7fffffff;
+
+    f16x8 q[kDepth];
+    float sharp;
+    {
+        const uint16_t* x = p.q + (first + token) * p.q_token + head * p.q_head + 8 * h;
+        float unit, down;
+        uint32_t most = 0;
+        float v[kDepth][8];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] = __builtin_fmaf(one[j], factor, v[j]);
-            sum = __builtin_fmaf(part[s * next + kWidth + 1], factor, sum);
+        for (int b = 0; b < kDepth; ++b) widen8(p, x + 16 * b, v[b], most);
+        most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), 32)));
+        row_unit(most, unit, down);
+        sharp = unit * p.scale * kLog2e;
+#pragma unroll
+        for (int b = 0; b < kDepth; ++b) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) q[b][i] = static_cast<_Float16>(v[b][i] * down);
         }
-        const int t = (row0 + r) / p.group, h = kv * p.group + (row0 + r) - t * p.group;
-        store_row(p, first + t, h, kWidth, d, v, sum);
+    }
+
+    f32x16 acc[kOut];
+#pragma unroll
+    for (int o = 0; o < kOut; ++o) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[o][i] = 0.0f;
+    }
+    float ref = 0.0f, bound = -__builtin_inff(), total = 0.0f;
+    const int* table = p.table + static_cast<int64_t>(share.request) * p.width;
+    const int within = p.page - 1;
+    const int64_t page_bytes = static_cast<int64_t>(p.heads) * p.page * kWidth;
+    const uint8_t* k_head = p.k_codes + static_cast<int64_t>(kv) * p.page * kWidth;
+    const uint8_t* v_head = p.v_codes + static_cast<int64_t>(kv) * p.page * kWidth;
+
+    i32x4 kc[kChunks], vc[kChunks];
+    int page_first = 0;
+    // Chunk c of the step's codes: 16 channels of token c / (width/16); 16 tokens of channel c / 4.
+    const auto load = [&](int step) {
+#pragma unroll
+        for (int i = 0; i < kChunks; ++i) {
+            const int c = thread + i * kThreads;
+            const int tk = step * kStep + c / (kWidth / 16), tv = step * kStep + 16 * (c & 3);
+            const int pk = max(entries[(tk >> p.shift) - page_first].page, 0);
+            const int pv = max(entries[(tv >> p.shift) - page_first].page, 0);
+            kc[i] = *reinterpret_cast<const i32x4*>(k_head + pk * page_bytes + (tk & within) * kWidth + 16 * (c % (kWidth / 16)));
+            vc[i] = *reinterpret_cast<const i32x4*>(v_head + pv * page_bytes + (c / 4) * p.page + (tv & within));
+        }
+    };
+    const auto put = [&](int step, uint8_t* keys) {
+        uint8_t* values = keys + kKeyBytes;
+#pragma unroll
+        for (int i = 0; i < kChunks; ++i) {
+            const int c = thread + i * kThreads;
+            const int t = c / (kWidth / 16), part16 = c % (kWidth / 16);
+            const int m = (t & 32) | exchanged(t & 31);
+            uint8_t* k = keys + m * (2 * kWidth);
+            *reinterpret_cast<f16x8*>(k + 16 * ((2 * part16) ^ (m & (kWidth / 8 - 1) & 15))) = codes8<kFp8>(kc[i][0], kc[i][1]);
+            *reinterpret_cast<f16x8*>(k + 16 * ((2 * part16 + 1) ^ (m & (kWidth / 8 - 1) & 15))) = codes8<kFp8>(kc[i][2], kc[i][3]);
+            const int d = c / 4, tv = step * kStep + 16 * (c & 3);
+            i32x4 x = vc[i];
+            if (tv + 16 > length || entries[(tv >> p.shift) - page_first].page < 0) {
+                const bool there = entries[(tv >> p.shift) - page_first].page >= 0;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int n = there ? length - tv - 4 * j : 0;
+                    x[j] &= n >= 4 ? -1 : n <= 0 ? 0 : (1 << (8 * n)) - 1;
+                }
+            }
+            uint8_t* v = values + d * (2 * kStep);
+            *reinterpret_cast<f16x8*>(v + 16 * ((2 * (c & 3)) ^ (d & 7))) = codes8<kFp8>(x[0], x[1]);
+            *reinterpret_cast<f16x8*>(v + 16 * ((2 * (c & 3) + 1) ^ (d & 7))) = codes8<kFp8>(x[2], x[3]);
+        }
+    };
+
+    for (int stage = span.begin; stage < span.end; stage += kStage) {
+        const int stage_end = min(span.end, stage + kStage);
+        page_first = stage * kStep >> p.shift;
+        if (stage != span.begin) __syncthreads();
+        stage_pages(p, entries, table, length, kv, page_first, stage_end);
+        __syncthreads();
+        load(stage);
+        put(stage, tiles[0]);
+        __syncthreads();
+        for (int step = stage; step < stage_end; ++step) {
+            const uint8_t* keys = tiles[(step - stage) & 1];
+            const uint8_t* values = keys + kKeyBytes;
+            const bool more = step + 1 < stage_end;
+            if (more) load(step + 1);
+            const int t0 = step * kStep;
+            if (busy && t0 < own.high_most && t0 + kStep > own.low_least) {
+                PageScales page[4];
+#pragma unroll
+                for (int a = 0; a < 4; ++a) page[a] = entries[((t0 + 16 * a) >> p.shift) - page_first];
+                const bool whole = t0 >= own.low_most && t0 + kStep <= own.high_least && page[0].page >= 0 &&
+                                   page[1].page >= 0 && page[2].page >= 0 && page[3].page >= 0;
+                f32x16 s[2];
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) s[half][i] = 0.0f;
+                    const uint8_t* k = keys + (32 * half + col) * (2 * kWidth);
+#pragma unroll
+                    for (int b = 0; b < kDepth; ++b) {
+                        const f16x8 x = *reinterpret_cast<const f16x8*>(k + 16 * ((2 * b + h) ^ (col & (kWidth / 8 - 1) & 15)));
+                        s[half] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, q[b], s[half], 0, 0, 0);
+                    }
+                }
+                float most = -__builtin_inff();
+#pragma unroll
+                for (int a = 0; a < 4; ++a) {
+                    const float mul = sharp * page[a].keys, add = page[a].values_log - ref;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        float x = __builtin_fmaf(s[a / 2][8 * (a & 1) + e], mul, add);
+                        const int t = t0 + 16 * a + 8 * h + e;
+                        if (!whole && (page[a].page < 0 || t < low || t >= high)) x = -__builtin_inff();
+                        s[a / 2][8 * (a & 1) + e] = x;
+                        most = fmaxf(most, x);
+                    }
+                }
+                if (__any(most > bound)) {
+                    most = fmaxf(most, __shfl_xor(most, 32));
+                    const float up = most > bound ? most - kLift : 0.0f;
+                    const float shrink = bound > 0.0f ? __builtin_amdgcn_exp2f(-up) : 0.0f;
+                    if (most > bound) bound = 15.0f;
+                    ref += up;
+                    total *= shrink;
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) s[i / 16][i % 16] -= up;
+#pragma unroll
+                    for (int o = 0; o < kOut; ++o) {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) acc[o][i] *= shrink;
+                    }
+                }
+                f16x8 w[4];
+#pragma unroll
+                for (int a = 0; a < 4; ++a) {
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const float x = __builtin_amdgcn_exp2f(s[a / 2][8 * (a & 1) + e]);
+                        sum += x;
+                        w[a][e] = static_cast<_Float16>(x);
+                    }
+                    total += sum == 0.0f ? 0.0f : sum * page[a].values_inv;
+                }
+#pragma unroll
+                for (int o = 0; o < kOut; ++o) {
+                    const uint8_t* v = values + (32 * o + col) * (2 * kStep);
+#pragma unroll
+                    for (int a = 0; a < 4; ++a) {
+                        const f16x8 x = *reinterpret_cast<const f16x8*>(v + 16 * ((2 * a + h) ^ (col & 7)));
+                        acc[o] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, w[a], acc[o], 0, 0, 0);
+                    }
+                }
+            }
+            if (more) put(step + 1, tiles[(step + 1 - stage) & 1]);
+            __syncthreads();
+        }
+    }
+
+    if (!live) return;
+    total += __shfl_xor(total, 32);
+    float* to = share.splits == 1 ? nullptr : part.work + ((static_cast<int64_t>(share.place + share.split) * p.heads + kv) * kRows + 32 * wave + col) * (kWidth + 4);
+#pragma unroll
+    for (int o = 0; o < kOut; ++o) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const f32x4 v = {acc[o][4 * i], acc[o][4 * i + 1], acc[o][4 * i + 2], acc[o][4 * i + 3]};
+            const int d = 32 * o + 8 * i + 4 * h;
+            if (to) *reinterpret_cast<f32x4*>(to + d) = v;
+            else store_row(p, first + token, head, kWidth, d, v, total);
+        }
+    }
+    if (to && h == 0) {
+        to[kWidth] = bound > 0.0f ? ref : kNoScore;
+        to[kWidth + 1] = total;
     }
 }
 
-// Rows of the step that no request has (past the last one's tokens) are zeros.
-__global__ __launch_bounds__(256) void rest_kernel(CacheAttend p) {
-    const int first = row_start(p, p.requests);
-    const int64_t row = static_cast<int64_t>(p.q_heads) * p.head_width / 8;
-    const int64_t all = (p.tokens - first) * row;
-    i32x4* out = reinterpret_cast<i32x4*>(p.out) + first * row;
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < all; i += 256 * gridDim.x) out[i] = i32x4{0, 0, 0, 0};
+// ------------------------------------------------------------------------------------- join
+
+// Joins the parts of the row tiles that several workgroups took: a workgroup takes one row (and every
+// kRowGroups-th after it) of a tile and head, its threads kWidth/4 of them a part, all parts brought to the
+// largest reference. Which thread sums which parts is fixed by their number: a call's result does not vary.
+template <int kWidth, int kRows>
+__global__ __launch_bounds__(256) void join_kernel(CacheAttend p, Part part, int row_groups, int items) {
+    constexpr int kQuads = kWidth / 4, kParts = 256 / kQuads;
+    __shared__ float tops[4];
+    __shared__ f32x4 sums[kParts][kQuads];
+    __shared__ float totals[kParts];
+    const int thread = threadIdx.x, slice = thread / kQuads, quad = thread % kQuads;
+    for (int item = blockIdx.x; item < items; item += gridDim.x) {
+        const int kv = item % p.heads, group = item / p.heads % row_groups;
+        Share share;
+        if (!find_share<kRows, false>(p, part, item / (p.heads * row_groups), share)) return;
+        if (share.splits == 1) continue;
+        const int first = row_start(p, share.request), rows = (row_start(p, share.request + 1) - first) * p.group;
+        const int row0 = kRows * share.tile, count = min(kRows, rows - row0);
+        const int64_t next = static_cast<int64_t>(p.heads) * kRows * (kWidth + 4);
+        for (int r = group; r < count; r += row_groups) {
+            const float* at = part.work + ((static_cast<int64_t>(share.place) * p.heads + kv) * kRows + r) * (kWidth + 4);
+            float best = kNoScore;
+            for (int s = thread; s < share.splits; s += 256) best = nan_max(best, at[s * next + kWidth]);
+            best = wave_max_nan(best);
+            if ((thread & 63) == 0) tops[thread >> 6] = best;
+            __syncthreads();
+            best = nan_max(nan_max(tops[0], tops[1]), nan_max(tops[2], tops[3]));
+            float sum = 0.0f;
+            f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+            for (int s = slice; s < share.splits; s += kParts) {
+                const float* one = at + s * next;
+                const f32x4 x = *reinterpret_cast<const f32x4*>(one + 4 * quad);
+                const float factor = __builtin_amdgcn_exp2f(one[kWidth] - best);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[j] = __builtin_fmaf(x[j], factor, v[j]);
+                sum = __builtin_fmaf(one[kWidth + 1], factor, sum);
+            }
+            sums[slice][quad] = v;
+            if (quad == 0) totals[slice] = sum;
+            __syncthreads();
+            if (thread < kQuads) {
+#pragma unroll
+                for (int s = 1; s < kParts; ++s) {
+                    v += sums[s][quad];
+                    sum += totals[s];
+                }
+                const int t = (row0 + r) / p.group, h = kv * p.group + (row0 + r) - t * p.group;
+                store_row(p, first + t, h, kWidth, 4 * quad, v, sum);
+            }
+            __syncthreads();
+        }
+    }
 }
 
-struct AttendShape {
-    int tiles, shares;
-    int64_t row_tiles;
-    bool splits;
+// ----------------------------------------------------------------------------------- launch
+
+// One of a call's launches: its row tiles' rows, their number at the most, and where its places begin.
+struct Launch {
+    bool on;
+    int rows, over, upto, shares, row_groups;
+    int64_t tiles, offset;
 };
 
-int64_t few_tiles(const CacheAttend& p, int rows) {
-    return (static_cast<int64_t>(p.tokens) * p.group + rows - 1) / rows + p.requests;
+// Eight waves share a step's tiles; at width 64 those are too small for so many, at 256 a wave takes 512
+// registers.
+constexpr int many_waves(int width) { return width == 128 ? 8 : 4; }
+
+struct AttendShape {
+    Launch few, many;
+    bool splits;
+    int64_t floats;
+};
+
+constexpr int kFewRows = 64;      // up to here a request's rows are taken by few_kernel alone
+constexpr int kBesideRows = 16;   // and up to here beside requests of more
+
+// The shape of a call, which its workspace goes by too. Where a request may have more than kFewRows
+// rows, those of more than kBesideRows go to many_kernel and the others, if there are others, to few_kernel.
+AttendShape shape_of(int64_t tokens, int group, int requests, int heads, int columns, int page, int width, int64_t most) {
+    const int64_t rows = (most > 0 && most < tokens ? most : tokens) * group;
+    const int all = 0x7fffffff;
+    AttendShape a = {};
+    a.few.on = rows <= kFewRows || requests > 1;
+    a.many.on = rows > kFewRows;
+    a.few.rows = rows > 16 && !a.many.on ? 32 : 16;
+    a.few.upto = a.many.on ? kBesideRows : all;
+    a.few.shares = max(1, 2 * 512 / heads);
+    a.few.tiles = a.many.on ? requests : (tokens * group + a.few.rows - 1) / a.few.rows + requests;
+    a.few.row_groups = static_cast<int>(rows < a.few.rows ? rows : a.few.rows);
+    a.many.rows = 32 * many_waves(width);
+    a.many.over = a.few.on ? kBesideRows : 0;
+    a.many.upto = all;
+    a.many.shares = max(1, 256 / heads);
+    a.many.tiles = (tokens * group + a.many.rows - 1) / a.many.rows + requests;
+    a.many.row_groups = 8;
+    a.splits = static_cast<int64_t>(columns) * page > kMinSteps * kStep;
+    if (a.splits) {
+        if (a.few.on) a.floats += 2ll * a.few.shares * heads * a.few.rows * (width + 4);
+        a.many.offset = a.floats;
+        if (a.many.on) a.floats += 2ll * a.many.shares * heads * a.many.rows * (width + 4);
+    }
+    return a;
 }
 
-template <int kWidth, int kTiles, bool kFp8>
-hipError_t few(const CacheAttend& p, hipStream_t s) {
-    const int64_t tiles = few_tiles(p, 16 * kTiles);
-    few_kernel<kWidth, kTiles, kFp8><<<static_cast<unsigned>((p.shares + tiles) * p.heads), 256, 0, s>>>(p);
-    const hipError_t error = hipGetLastError();
-    if (error != hipSuccess || !p.work) return error;
-    join_kernel<kWidth, kTiles><<<dim3(static_cast<unsigned>(tiles), static_cast<unsigned>(p.heads)), 256, 0, s>>>(p);
+template <int kWidth, int kRows>
+hipError_t join(const CacheAttend& p, const Launch& l, const Part& part, hipStream_t s) {
+    const int64_t items = l.tiles * p.heads * l.row_groups;
+    join_kernel<kWidth, kRows><<<static_cast<unsigned>(items < 8192 ? items : 8192), 256, 0, s>>>(p, part, l.row_groups, static_cast<int>(items));
     return hipGetLastError();
 }
 
-template <bool kFp8>
-hipError_t attend(const CacheAttend& p, hipStream_t s) {
-    const bool one = p.tiles == 1;
-    if (p.head_width == 64) return one ? few<64, 1, kFp8>(p, s) : few<64, 2, kFp8>(p, s);
-    if (p.head_width == 128) return one ? few<128, 1, kFp8>(p, s) : few<128, 2, kFp8>(p, s);
-    return one ? few<256, 1, kFp8>(p, s) : few<256, 2, kFp8>(p, s);
+template <int kWidth, int kTiles, bool kFp8>
+hipError_t few(const CacheAttend& p, const AttendShape& a, hipStream_t s) {
+    const Launch& l = a.few;
+    const Part part = {l.over, l.upto, l.shares, p.work + l.offset};
+    few_kernel<kWidth, kTiles, kFp8><<<static_cast<unsigned>((l.shares + l.tiles + 1) * p.heads), 256, 0, s>>>(p, part, !a.many.on);
+    const hipError_t error = hipGetLastError();
+    if (error != hipSuccess || !a.splits) return error;
+    return join<kWidth, 16 * kTiles>(p, l, part, s);
 }
 
-// The launch's shape, which the workspace goes by too.
-AttendShape shape_of(int64_t tokens, int group, int requests, int heads, int columns, int page, int64_t most) {
-    AttendShape a;
-    a.tiles = most > 0 && most * group <= 16 ? 1 : 2;
-    a.row_tiles = (tokens * group + 16 * a.tiles - 1) / (16 * a.tiles) + requests;
-    // Two workgroups a CU at a time, and twice as many for the requests' different lengths.
-    a.shares = max(1, 2 * 512 / heads);
-    a.splits = static_cast<int64_t>(columns) * page > kMinSteps * kStep;
-    return a;
+template <int kWidth, bool kFp8>
+hipError_t attend(const CacheAttend& p, const AttendShape& a, hipStream_t s) {
+    hipError_t error = hipSuccess;
+    if (a.many.on) {
+        constexpr int kWaves = many_waves(kWidth);
+        const Launch& l = a.many;
+        const Part part = {l.over, l.upto, l.shares, p.work + l.offset};
+        many_kernel<kWidth, kWaves, kFp8><<<static_cast<unsigned>((l.shares + l.tiles + 1) * p.heads), 64 * kWaves, 0, s>>>(p, part, true);
+        error = hipGetLastError();
+        if (error == hipSuccess && a.splits) error = join<kWidth, 32 * kWaves>(p, l, part, s);
+    }
+    if (error != hipSuccess || !a.few.on) return error;
+    return a.few.rows == 16 ? few<kWidth, 1, kFp8>(p, a, s) : few<kWidth, 2, kFp8>(p, a, s);
+}
+
+template <bool kFp8>
+hipError_t attend(const CacheAttend& p, const AttendShape& a, hipStream_t s) {
+    if (p.head_width == 64) return attend<64, kFp8>(p, a, s);
+    if (p.head_width == 128) return attend<128, kFp8>(p, a, s);
+    return attend<256, kFp8>(p, a, s);
 }
 
 }  // namespace
 
 int64_t cache_attend_work(int64_t tokens, int group, int requests, int heads, int columns, int page, int width, int64_t most) {
-    const AttendShape a = shape_of(tokens, group, requests, heads, columns, page, most);
-    return a.splits ? (a.shares + a.row_tiles) * heads * 16 * a.tiles * (width + 4) * 4 : 0;
+    return 4 * shape_of(tokens, group, requests, heads, columns, page, width, most).floats;
 }
 
-hipError_t cache_attend(CacheAttend p, int64_t most, bool fp8, hipStream_t s) {
-    const AttendShape a = shape_of(p.tokens, p.group, p.requests, p.heads, p.width, p.page, most);
-    p.tiles = a.tiles;
-    p.shares = a.shares;
-    if (!a.splits) p.work = nullptr;
-    rest_kernel<<<64, 256, 0, s>>>(p);
-    const hipError_t error = hipGetLastError();
-    if (error != hipSuccess) return error;
-    return fp8 ? attend<true>(p, s) : attend<false>(p, s);
+hipError_t cache_attend(const CacheAttend& p, int64_t most, bool fp8, hipStream_t s) {
+    const AttendShape a = shape_of(p.tokens, p.group, p.requests, p.heads, p.width, p.page, p.head_width, most);
+    return fp8 ? attend<true>(p, a, s) : attend<false>(p, a, s);
 }
 
 }  // namespace cozyq
