@@ -59,6 +59,9 @@ __device__ __forceinline__ f16x8 codes8(uint32_t a, uint32_t b) {
 // A finite scale, NaN for an infinite one: whoever sees its page gets NaN, not a score of either sign.
 __device__ __forceinline__ float or_nan(float scale) { return scale + (scale - scale); }
 
+// Keeps a branch a branch: without it the compiler works out both sides and selects.
+__device__ __forceinline__ void rarely() { asm volatile(""); }
+
 // Four elements from d on of a row's result: the sums over its denominator, 0 for a row that sees nothing.
 __device__ __forceinline__ void store_row(const CacheAttend& p, int token, int head, int width, int d, f32x4 v, float total) {
     const float inv = total == 0.0f ? 0.0f : 1.0f / total;
@@ -103,7 +106,8 @@ constexpr int kMinSteps = 16;   // steps a workgroup takes at the least
 // out over `shares` workgroups a head.
 struct Part {
     int over, upto, shares;
-    float* work;  // places of kRows · (width + 4) floats: a row's sums, its reference, its denominator
+    int shift;    // a row tile is 1 << shift rows
+    float* work;  // places of a row tile's rows · (width + 4) floats: a row's sums, reference, denominator
 };
 
 // A request's part of the work: row tiles, and the 64-token steps that any of its rows sees.
@@ -111,13 +115,12 @@ struct Extent {
     int tiles, steps;
 };
 
-template <int kRows>
 __device__ __forceinline__ Extent extent(const CacheAttend& p, const Part& part, int r) {
     const int fresh = row_start(p, r + 1) - row_start(p, r), length = p.lengths[r], rows = fresh * p.group;
     if (rows <= part.over || rows > part.upto) return {0, 0};
     const int low = p.window > 0 ? max(0, length - fresh + 1 - p.window) : 0;
     const int steps = (max(length, 0) + kStep - 1) / kStep - low / kStep;
-    return {(rows + kRows - 1) / kRows, max(steps, 0)};
+    return {(rows + (1 << part.shift) - 1) >> part.shift, max(steps, 0)};
 }
 
 // Tile `tile` of request `request`, its steps split over `splits` workgroups, of which this is number
@@ -130,23 +133,27 @@ struct Share {
 // c = max(kMinSteps, N / shares) of one row tile's, so that there are at most shares + tiles workgroups
 // and at most 2 · shares places (a tile of more than c steps splits into less than 2 · steps / c),
 // whatever the requests' lengths are: the host sizes the launch and the workspace without knowing them.
-// Finds workgroup `id`'s share (kById), or row tile `id`'s first; false past the last. A request's last
+// Finds workgroup `id`'s share (kById), or row tile `id`'s first; false past the last, and for row tiles
+// where none is split. A request's last
 // tile comes first: where causal it has the most to do. Every wave scans all requests, 64 at a time.
-template <int kRows, bool kById>
+template <bool kById>
 __device__ bool find_share(const CacheAttend& p, const Part& part, int id, Share& out) {
     const int lane = threadIdx.x & 63;
     float work = 0.0f;  // in float32, which no number of steps overflows; the margin is over its rounding
+    int longest = 0;
     for (int base = 0; base < p.requests; base += 64) {
         Extent e = {0, 0};
-        if (base + lane < p.requests) e = extent<kRows>(p, part, base + lane);
+        if (base + lane < p.requests) e = extent(p, part, base + lane);
         const float sum = wave_prefix(static_cast<float>(e.tiles) * static_cast<float>(e.steps));
         work += __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, sum), 63));
+        longest = max(longest, e.steps);
     }
     const int c = max(kMinSteps, static_cast<int>(work * 1.001f / static_cast<float>(part.shares)) + 1);
+    if (!kById && !__any(longest > c)) return false;  // nothing is split: nothing to join
     int ids_before = 0, places_before = 0;
     for (int base = 0; base < p.requests; base += 64) {
         Extent e = {0, 0};
-        if (base + lane < p.requests) e = extent<kRows>(p, part, base + lane);
+        if (base + lane < p.requests) e = extent(p, part, base + lane);
         const int splits = max(1, (e.steps + c - 1) / c);
         const int ids = wave_prefix(kById ? e.tiles * splits : e.tiles);
         const int places = wave_prefix(splits > 1 ? e.tiles * splits : 0);
@@ -261,10 +268,11 @@ __global__ __launch_bounds__(256, kWidth == 256 ? 1 : 2) void few_kernel(CacheAt
     __shared__ PageScales entries[kEntries];
     __shared__ float merged[kWaves][16][kWidth + 4];
     __shared__ float tops[kWaves][16], totals[kWaves][16];
-    const int thread = threadIdx.x, lane = thread & 63, wave = thread >> 6, col = lane & 15, g = lane >> 4;
+    const int thread = threadIdx.x, lane = thread & 63, wave = __builtin_amdgcn_readfirstlane(thread >> 6);
+    const int col = lane & 15, g = lane >> 4;
     const int kv = blockIdx.x % p.heads, id = blockIdx.x / p.heads;
     Share share;
-    if (!find_share<kRows, true>(p, part, id, share)) {
+    if (!find_share<true>(p, part, id, share)) {
         if (clears) clear_rest(p, kWidth);
         return;
     }
@@ -388,9 +396,16 @@ __global__ __launch_bounds__(256, kWidth == 256 ? 1 : 2) void few_kernel(CacheAt
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     x[i] = __builtin_fmaf(s[n][i / 4][i % 4], mul, add);
-                    if (!whole && (page.page < 0 || mine + i < low[n] || mine + i >= high[n])) x[i] = -__builtin_inff();
-                    most = fmaxf(most, x[i]);
                 }
+                if (!whole) {
+                    rarely();
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        if (page.page < 0 || mine + i < low[n] || mine + i >= high[n]) x[i] = -__builtin_inff();
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 16; ++i) most = fmaxf(most, x[i]);
                 if (__any(most > bound[n])) {
                     most = fmaxf(most, __shfl_xor(most, 16));
                     most = fmaxf(most, __shfl_xor(most, 32));
@@ -419,6 +434,7 @@ __global__ __launch_bounds__(256, kWidth == 256 ? 1 : 2) void few_kernel(CacheAt
                 total[n] += sum == 0.0f ? 0.0f : sum * page.values_inv;
             }
             if (!whole) {
+                rarely();
                 // Bytes past the request's tokens may hold anything, a NaN of the format too.
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
@@ -508,13 +524,14 @@ __device__ __forceinline__ int exchanged(int m) { return (m & ~12) | ((m & 4) <<
 template <int kWidth, int kWaves, bool kFp8>
 __global__ __launch_bounds__(64 * kWaves, kWidth == 256 ? 1 : 2) void many_kernel(CacheAttend p, Part part, bool clears) {
     constexpr int kRows = 32 * kWaves, kThreads = 64 * kWaves, kOut = kWidth / 32, kDepth = kWidth / 16;
-    constexpr int kKeyBytes = kStep * kWidth * 2, kChunks = kStep * kWidth / 16 / kThreads;
+    constexpr int kBytes = kStep * kWidth * 2, kChunks = kStep * kWidth / 16 / kThreads, kSwizzle = kWidth == 64 ? 7 : 15;
     __shared__ PageScales entries[kEntries];
-    __shared__ __attribute__((aligned(16))) uint8_t tiles[2][2 * kKeyBytes];
-    const int thread = threadIdx.x, lane = thread & 63, wave = thread >> 6, col = lane & 31, h = lane >> 5;
+    __shared__ __attribute__((aligned(16))) uint8_t keys[2][kBytes], values[2][kBytes];
+    const int thread = threadIdx.x, lane = thread & 63, wave = __builtin_amdgcn_readfirstlane(thread >> 6);
+    const int col = lane & 31, h = lane >> 5;
     const int kv = blockIdx.x % p.heads, id = blockIdx.x / p.heads;
     Share share;
-    if (!find_share<kRows, true>(p, part, id, share)) {
+    if (!find_share<true>(p, part, id, share)) {
         if (clears) clear_rest(p, kWidth);
         return;
     }
@@ -563,45 +580,73 @@ __global__ __launch_bounds__(64 * kWaves, kWidth == 256 ? 1 : 2) void many_kerne
     const uint8_t* k_head = p.k_codes + static_cast<int64_t>(kv) * p.page * kWidth;
     const uint8_t* v_head = p.v_codes + static_cast<int64_t>(kv) * p.page * kWidth;
 
+    // Chunk c of a step's codes: 16 channels of token c / (width/16); 16 tokens of channel c / 4.
     i32x4 kc[kChunks], vc[kChunks];
-    int page_first = 0;
-    // Chunk c of the step's codes: 16 channels of token c / (width/16); 16 tokens of channel c / 4.
-    const auto load = [&](int step) {
+    int page_first = 0, kept[kChunks];
+    uint32_t k_to[kChunks][2], v_to[kChunks][2];
+#pragma unroll
+    for (int i = 0; i < kChunks; ++i) {
+        const int c = thread + i * kThreads, t = c / (kWidth / 16), x = c % (kWidth / 16), d = c / 4;
+        const int m = (t & 32) | exchanged(t & 31);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            k_to[i][j] = m * (2 * kWidth) + 16 * ((2 * x + j) ^ (m & kSwizzle));
+            v_to[i][j] = d * (2 * kStep) + 16 * ((2 * (c & 3) + j) ^ (d & 7));
+        }
+    }
+    const auto load_keys = [&](int step) {
 #pragma unroll
         for (int i = 0; i < kChunks; ++i) {
-            const int c = thread + i * kThreads;
-            const int tk = step * kStep + c / (kWidth / 16), tv = step * kStep + 16 * (c & 3);
-            const int pk = max(entries[(tk >> p.shift) - page_first].page, 0);
-            const int pv = max(entries[(tv >> p.shift) - page_first].page, 0);
-            kc[i] = *reinterpret_cast<const i32x4*>(k_head + pk * page_bytes + (tk & within) * kWidth + 16 * (c % (kWidth / 16)));
-            vc[i] = *reinterpret_cast<const i32x4*>(v_head + pv * page_bytes + (c / 4) * p.page + (tv & within));
+            const int c = thread + i * kThreads, t = step * kStep + c / (kWidth / 16);
+            const int page = max(entries[(t >> p.shift) - page_first].page, 0);
+            kc[i] = *reinterpret_cast<const i32x4*>(k_head + page * page_bytes + (t & within) * kWidth + 16 * (c % (kWidth / 16)));
         }
     };
-    const auto put = [&](int step, uint8_t* keys) {
-        uint8_t* values = keys + kKeyBytes;
+    const auto load_values = [&](int step) {
 #pragma unroll
         for (int i = 0; i < kChunks; ++i) {
-            const int c = thread + i * kThreads;
-            const int t = c / (kWidth / 16), part16 = c % (kWidth / 16);
-            const int m = (t & 32) | exchanged(t & 31);
-            uint8_t* k = keys + m * (2 * kWidth);
-            *reinterpret_cast<f16x8*>(k + 16 * ((2 * part16) ^ (m & (kWidth / 8 - 1) & 15))) = codes8<kFp8>(kc[i][0], kc[i][1]);
-            *reinterpret_cast<f16x8*>(k + 16 * ((2 * part16 + 1) ^ (m & (kWidth / 8 - 1) & 15))) = codes8<kFp8>(kc[i][2], kc[i][3]);
-            const int d = c / 4, tv = step * kStep + 16 * (c & 3);
-            i32x4 x = vc[i];
-            if (tv + 16 > length || entries[(tv >> p.shift) - page_first].page < 0) {
-                const bool there = entries[(tv >> p.shift) - page_first].page >= 0;
+            const int c = thread + i * kThreads, t = step * kStep + 16 * (c & 3);
+            const int page = entries[(t >> p.shift) - page_first].page;
+            kept[i] = page < 0 ? 0 : length - t;
+            vc[i] = *reinterpret_cast<const i32x4*>(v_head + max(page, 0) * page_bytes + (c / 4) * p.page + (t & within));
+        }
+    };
+    // Chunk i of a step's codes, as f16, to its places in LDS.
+    const auto put_keys = [&](int step, int i) {
+        *reinterpret_cast<f16x8*>(&keys[step & 1][k_to[i][0]]) = codes8<kFp8>(kc[i][0], kc[i][1]);
+        *reinterpret_cast<f16x8*>(&keys[step & 1][k_to[i][1]]) = codes8<kFp8>(kc[i][2], kc[i][3]);
+    };
+    const auto put_values = [&](int step, int i) {
+        *reinterpret_cast<f16x8*>(&values[step & 1][v_to[i][0]]) = codes8<kFp8>(vc[i][0], vc[i][1]);
+        *reinterpret_cast<f16x8*>(&values[step & 1][v_to[i][1]]) = codes8<kFp8>(vc[i][2], vc[i][3]);
+    };
+    // Where a step's values hold tokens past the request's or of pages that the cache has not, zeros in their
+    // place, over what was put there.
+    const auto cut_values = [&](int step) {
+#pragma unroll
+        for (int i = 0; i < kChunks; ++i) {
+            if (__any(kept[i] < 16)) {
+                rarely();
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const int n = there ? length - tv - 4 * j : 0;
-                    x[j] &= n >= 4 ? -1 : n <= 0 ? 0 : (1 << (8 * n)) - 1;
+                    const int n = kept[i] - 4 * j;
+                    vc[i][j] &= n >= 4 ? -1 : n <= 0 ? 0 : (1 << (8 * n)) - 1;
                 }
+                put_values(step, i);
             }
-            uint8_t* v = values + d * (2 * kStep);
-            *reinterpret_cast<f16x8*>(v + 16 * ((2 * (c & 3)) ^ (d & 7))) = codes8<kFp8>(x[0], x[1]);
-            *reinterpret_cast<f16x8*>(v + 16 * ((2 * (c & 3) + 1) ^ (d & 7))) = codes8<kFp8>(x[2], x[3]);
         }
     };
+    // The matrix unit's operands in LDS: elements 16b + 8h .. of the keys of a half's row, tokens 16a + 8h ..
+    // of the values of 32 channels.
+    const auto key_chunk = [&](int step, int b, int half) {
+        return *reinterpret_cast<const f16x8*>(&keys[step & 1][(32 * half + col) * (2 * kWidth) + 16 * ((2 * b + h) ^ (col & kSwizzle))]);
+    };
+    const auto value_chunk = [&](int step, int a, int o) {
+        return *reinterpret_cast<const f16x8*>(&values[step & 1][(32 * o + col) * (2 * kStep) + 16 * ((2 * a + h) ^ (col & 7))]);
+    };
+    // The scores of a step whose keys are in LDS, as they leave the matrix unit.
+    f32x16 s[2];
+    constexpr int kScores = 2 * kDepth, kSums = 4 * kOut, kAhead = 4;
 
     for (int stage = span.begin; stage < span.end; stage += kStage) {
         const int stage_end = min(span.end, stage + kStage);
@@ -609,46 +654,52 @@ __global__ __launch_bounds__(64 * kWaves, kWidth == 256 ? 1 : 2) void many_kerne
         if (stage != span.begin) __syncthreads();
         stage_pages(p, entries, table, length, kv, page_first, stage_end);
         __syncthreads();
-        load(stage);
-        put(stage, tiles[0]);
+        load_keys(stage);
+        load_values(stage);
+#pragma unroll
+        for (int i = 0; i < kChunks; ++i) {
+            put_keys(stage, i);
+            put_values(stage, i);
+        }
+        cut_values(stage);
+        if (stage + 1 < stage_end) {
+            load_keys(stage + 1);
+#pragma unroll
+            for (int i = 0; i < kChunks; ++i) put_keys(stage + 1, i);
+        }
         __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[0][i] = s[1][i] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < kScores; ++j)
+            s[j % 2] = __builtin_amdgcn_mfma_f32_32x32x16_f16(key_chunk(stage, j / 2, j % 2), q[j / 2], s[j % 2], 0, 0, 0);
         for (int step = stage; step < stage_end; ++step) {
-            const uint8_t* keys = tiles[(step - stage) & 1];
-            const uint8_t* values = keys + kKeyBytes;
-            const bool more = step + 1 < stage_end;
-            if (more) load(step + 1);
-            const int t0 = step * kStep;
-            if (busy && t0 < own.high_most && t0 + kStep > own.low_least) {
+            if (step + 2 < stage_end) load_keys(step + 2);
+            if (step + 1 < stage_end) load_values(step + 1);
+            if (busy) {
+                const int t0 = step * kStep;
                 PageScales page[4];
 #pragma unroll
                 for (int a = 0; a < 4; ++a) page[a] = entries[((t0 + 16 * a) >> p.shift) - page_first];
                 const bool whole = t0 >= own.low_most && t0 + kStep <= own.high_least && page[0].page >= 0 &&
                                    page[1].page >= 0 && page[2].page >= 0 && page[3].page >= 0;
-                f32x16 s[2];
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) s[half][i] = 0.0f;
-                    const uint8_t* k = keys + (32 * half + col) * (2 * kWidth);
-#pragma unroll
-                    for (int b = 0; b < kDepth; ++b) {
-                        const f16x8 x = *reinterpret_cast<const f16x8*>(k + 16 * ((2 * b + h) ^ (col & (kWidth / 8 - 1) & 15)));
-                        s[half] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, q[b], s[half], 0, 0, 0);
-                    }
-                }
                 float most = -__builtin_inff();
 #pragma unroll
                 for (int a = 0; a < 4; ++a) {
                     const float mul = sharp * page[a].keys, add = page[a].values_log - ref;
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        float x = __builtin_fmaf(s[a / 2][8 * (a & 1) + e], mul, add);
-                        const int t = t0 + 16 * a + 8 * h + e;
-                        if (!whole && (page[a].page < 0 || t < low || t >= high)) x = -__builtin_inff();
-                        s[a / 2][8 * (a & 1) + e] = x;
-                        most = fmaxf(most, x);
+                    for (int e = 0; e < 8; ++e) s[a / 2][8 * (a & 1) + e] = __builtin_fmaf(s[a / 2][8 * (a & 1) + e], mul, add);
+                }
+                if (!whole) {
+                    rarely();
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        const int t = t0 + 16 * (i / 8) + 8 * h + i % 8;
+                        if (page[i / 8].page < 0 || t < low || t >= high) s[i / 16][i % 16] = -__builtin_inff();
                     }
                 }
+#pragma unroll
+                for (int i = 0; i < 32; ++i) most = fmaxf(most, s[i / 16][i % 16]);
                 if (__any(most > bound)) {
                     most = fmaxf(most, __shfl_xor(most, 32));
                     const float up = most > bound ? most - kLift : 0.0f;
@@ -664,29 +715,54 @@ __global__ __launch_bounds__(64 * kWaves, kWidth == 256 ? 1 : 2) void many_kerne
                         for (int i = 0; i < 16; ++i) acc[o][i] *= shrink;
                     }
                 }
-                f16x8 w[4];
+                // The next step's scores on the matrix unit over this one's exponentials, then this one's sums
+                // over the next tiles' conversion. Each operand is read from LDS kAhead products before its
+                // own, and the order written here is kept. Past the stage's last step the scores are of
+                // whatever the tile holds, and not used.
+                f16x8 ring[kAhead], w[4];
+                f32x16 next[2];
+                const auto key_operand = [&](int j) { return key_chunk(step + 1, j / 2, j % 2); };
+                const auto value_operand = [&](int j) { return value_chunk(step, j / kOut, j % kOut); };
+                float sum = 0.0f;
 #pragma unroll
-                for (int a = 0; a < 4; ++a) {
-                    float sum = 0.0f;
+                for (int i = 0; i < 16; ++i) next[0][i] = next[1][i] = 0.0f;
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const float x = __builtin_amdgcn_exp2f(s[a / 2][8 * (a & 1) + e]);
-                        sum += x;
-                        w[a][e] = static_cast<_Float16>(x);
+                for (int j = 0; j < kAhead; ++j) ring[j] = key_operand(j);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int j = 0; j < kScores; ++j) {
+                    next[j % 2] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ring[j % kAhead], q[j / 2], next[j % 2], 0, 0, 0);
+                    ring[j % kAhead] = j + kAhead < kScores ? key_operand(j + kAhead) : value_operand(j + kAhead - kScores);
+#pragma unroll
+                    for (int i = 32 / kScores * j; i < 32 / kScores * (j + 1); ++i) {
+                        const float x = __builtin_amdgcn_exp2f(s[i / 16][i % 16]);
+                        sum = i % 8 ? sum + x : x;
+                        w[i / 8][i % 8] = static_cast<_Float16>(x);
+                        // A group whose tokens the row does not see adds nothing, whatever its page's scale is.
+                        if (i % 8 == 7) total += sum == 0.0f ? 0.0f : sum * page[i / 8].values_inv;
                     }
-                    total += sum == 0.0f ? 0.0f : sum * page[a].values_inv;
+                    __builtin_amdgcn_sched_barrier(0);
                 }
 #pragma unroll
-                for (int o = 0; o < kOut; ++o) {
-                    const uint8_t* v = values + (32 * o + col) * (2 * kStep);
-#pragma unroll
-                    for (int a = 0; a < 4; ++a) {
-                        const f16x8 x = *reinterpret_cast<const f16x8*>(v + 16 * ((2 * a + h) ^ (col & 7)));
-                        acc[o] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, w[a], acc[o], 0, 0, 0);
+                for (int j = 0; j < kSums; ++j) {
+                    acc[j % kOut] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ring[(kScores + j) % kAhead], w[j / kOut], acc[j % kOut], 0, 0, 0);
+                    if (j + kAhead < kSums) ring[(kScores + j) % kAhead] = value_operand(j + kAhead);
+                    if (j < kChunks) {
+                        put_keys(step + 2, j);
+                        put_values(step + 1, j);
                     }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                s[0] = next[0];
+                s[1] = next[1];
+            } else {
+#pragma unroll
+                for (int i = 0; i < kChunks; ++i) {
+                    put_keys(step + 2, i);
+                    put_values(step + 1, i);
                 }
             }
-            if (more) put(step + 1, tiles[(step + 1 - stage) & 1]);
+            cut_values(step + 1);
             __syncthreads();
         }
     }
@@ -712,56 +788,88 @@ __global__ __launch_bounds__(64 * kWaves, kWidth == 256 ? 1 : 2) void many_kerne
 
 // ------------------------------------------------------------------------------------- join
 
-// Joins the parts of the row tiles that several workgroups took: a workgroup takes one row (and every
-// kRowGroups-th after it) of a tile and head, its threads kWidth/4 of them a part, all parts brought to the
-// largest reference. Which thread sums which parts is fixed by their number: a call's result does not vary.
-template <int kWidth, int kRows>
-__global__ __launch_bounds__(256) void join_kernel(CacheAttend p, Part part, int row_groups, int items) {
-    constexpr int kQuads = kWidth / 4, kParts = 256 / kQuads;
-    __shared__ float tops[4];
+// A row's parts from slice `slice` on, every `slices`-th, brought to `best` and added up: four elements.
+template <int kWidth>
+__device__ __forceinline__ void add_parts(const float* at, int64_t next, int splits, int slice, int slices, int quad,
+                                          float best, f32x4& v, float& sum) {
+    v = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    sum = 0.0f;
+#pragma unroll 8
+    for (int s = slice; s < splits; s += slices) {
+        const float* one = at + s * next;
+        const f32x4 x = *reinterpret_cast<const f32x4*>(one + 4 * quad);
+        const float factor = __builtin_amdgcn_exp2f(one[kWidth] - best);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = __builtin_fmaf(x[j], factor, v[j]);
+        sum = __builtin_fmaf(one[kWidth + 1], factor, sum);
+    }
+}
+
+// Joins the parts of the row tiles that several workgroups took, all of a row's parts brought to their
+// largest reference; blockIdx.y says of which launch. few_kernel's rows are few and their parts many: a
+// workgroup a row, kWidth/4 threads a part. many_kernel's rows are many and their parts few: a wave takes
+// kJoinRows rows, one after another. Which thread sums which parts is fixed: a call's result does not vary.
+constexpr int kJoinRows = 4;
+
+template <int kWidth>
+__global__ __launch_bounds__(256) void join_kernel(CacheAttend p, Part few, Part many, int few_rows, int few_items, int many_items) {
+    constexpr int kQuads = kWidth / 4, kParts = 256 / kQuads, kSlices = 64 / kQuads;
     __shared__ f32x4 sums[kParts][kQuads];
     __shared__ float totals[kParts];
-    const int thread = threadIdx.x, slice = thread / kQuads, quad = thread % kQuads;
-    for (int item = blockIdx.x; item < items; item += gridDim.x) {
-        const int kv = item % p.heads, group = item / p.heads % row_groups;
+    const int thread = threadIdx.x, lane = thread & 63;
+    const bool wide = blockIdx.y != 0;
+    const Part part = wide ? many : few;
+    const int rows_all = 1 << part.shift, groups = wide ? rows_all / kJoinRows : few_rows;
+    const int items = wide ? many_items : few_items, each = wide ? 4 : 1;
+    const int64_t next = static_cast<int64_t>(p.heads) * rows_all * (kWidth + 4);
+    for (int item = blockIdx.x * each + (wide ? thread >> 6 : 0); item < items; item += gridDim.x * each) {
+        const int kv = item % p.heads, group = item / p.heads % groups;
         Share share;
-        if (!find_share<kRows, false>(p, part, item / (p.heads * row_groups), share)) return;
+        if (!find_share<false>(p, part, item / (p.heads * groups), share)) return;
         if (share.splits == 1) continue;
         const int first = row_start(p, share.request), rows = (row_start(p, share.request + 1) - first) * p.group;
-        const int row0 = kRows * share.tile, count = min(kRows, rows - row0);
-        const int64_t next = static_cast<int64_t>(p.heads) * kRows * (kWidth + 4);
-        for (int r = group; r < count; r += row_groups) {
-            const float* at = part.work + ((static_cast<int64_t>(share.place) * p.heads + kv) * kRows + r) * (kWidth + 4);
-            float best = kNoScore;
-            for (int s = thread; s < share.splits; s += 256) best = nan_max(best, at[s * next + kWidth]);
+        const int row0 = share.tile << part.shift, count = min(rows_all, rows - row0);
+        const float* tile = part.work + (static_cast<int64_t>(share.place) * p.heads + kv) * rows_all * (kWidth + 4);
+        const int from = wide ? group * kJoinRows : group, to = wide ? min(count, from + kJoinRows) : count;
+        for (int r = from; r < to; r += wide ? 1 : groups) {
+            const float* at = tile + static_cast<int64_t>(r) * (kWidth + 4);
+            float best = kNoScore, sum;
+            for (int s = lane; s < share.splits; s += 64) best = nan_max(best, at[s * next + kWidth]);
             best = wave_max_nan(best);
-            if ((thread & 63) == 0) tops[thread >> 6] = best;
-            __syncthreads();
-            best = nan_max(nan_max(tops[0], tops[1]), nan_max(tops[2], tops[3]));
-            float sum = 0.0f;
-            f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
-            for (int s = slice; s < share.splits; s += kParts) {
-                const float* one = at + s * next;
-                const f32x4 x = *reinterpret_cast<const f32x4*>(one + 4 * quad);
-                const float factor = __builtin_amdgcn_exp2f(one[kWidth] - best);
+            f32x4 v;
+            bool mine;
+            int quad;
+            if (wide) {
+                quad = lane % kQuads;
+                add_parts<kWidth>(at, next, share.splits, lane / kQuads, kSlices, quad, best, v, sum);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) v[j] = __builtin_fmaf(x[j], factor, v[j]);
-                sum = __builtin_fmaf(one[kWidth + 1], factor, sum);
-            }
-            sums[slice][quad] = v;
-            if (quad == 0) totals[slice] = sum;
-            __syncthreads();
-            if (thread < kQuads) {
+                for (int step = kQuads; step < 64; step *= 2) {
 #pragma unroll
-                for (int s = 1; s < kParts; ++s) {
-                    v += sums[s][quad];
-                    sum += totals[s];
+                    for (int j = 0; j < 4; ++j) v[j] += __shfl_xor(v[j], step);
+                    sum += __shfl_xor(sum, step);
                 }
+                mine = lane < kQuads;
+            } else {
+                quad = thread % kQuads;
+                const int slice = thread / kQuads;
+                add_parts<kWidth>(at, next, share.splits, slice, kParts, quad, best, v, sum);
+                __syncthreads();
+                sums[slice][quad] = v;
+                if (quad == 0) totals[slice] = sum;
+                __syncthreads();
+                mine = thread < kQuads;
+                if (mine) {
+#pragma unroll
+                    for (int s = 1; s < kParts; ++s) {
+                        v += sums[s][quad];
+                        sum += totals[s];
+                    }
+                }
+            }
+            if (mine) {
                 const int t = (row0 + r) / p.group, h = kv * p.group + (row0 + r) - t * p.group;
                 store_row(p, first + t, h, kWidth, 4 * quad, v, sum);
             }
-            __syncthreads();
         }
     }
 }
@@ -804,9 +912,8 @@ AttendShape shape_of(int64_t tokens, int group, int requests, int heads, int col
     a.many.rows = 32 * many_waves(width);
     a.many.over = a.few.on ? kBesideRows : 0;
     a.many.upto = all;
-    a.many.shares = max(1, 256 / heads);
+    a.many.shares = max(1, (width == 64 ? 512 : 256) / heads);
     a.many.tiles = (tokens * group + a.many.rows - 1) / a.many.rows + requests;
-    a.many.row_groups = 8;
     a.splits = static_cast<int64_t>(columns) * page > kMinSteps * kStep;
     if (a.splits) {
         if (a.few.on) a.floats += 2ll * a.few.shares * heads * a.few.rows * (width + 4);
@@ -816,36 +923,32 @@ AttendShape shape_of(int64_t tokens, int group, int requests, int heads, int col
     return a;
 }
 
-template <int kWidth, int kRows>
-hipError_t join(const CacheAttend& p, const Launch& l, const Part& part, hipStream_t s) {
-    const int64_t items = l.tiles * p.heads * l.row_groups;
-    join_kernel<kWidth, kRows><<<static_cast<unsigned>(items < 8192 ? items : 8192), 256, 0, s>>>(p, part, l.row_groups, static_cast<int>(items));
-    return hipGetLastError();
-}
+int log2_of(int n) { return n > 1 ? 1 + log2_of(n / 2) : 0; }
 
-template <int kWidth, int kTiles, bool kFp8>
-hipError_t few(const CacheAttend& p, const AttendShape& a, hipStream_t s) {
-    const Launch& l = a.few;
-    const Part part = {l.over, l.upto, l.shares, p.work + l.offset};
-    few_kernel<kWidth, kTiles, kFp8><<<static_cast<unsigned>((l.shares + l.tiles + 1) * p.heads), 256, 0, s>>>(p, part, !a.many.on);
-    const hipError_t error = hipGetLastError();
-    if (error != hipSuccess || !a.splits) return error;
-    return join<kWidth, 16 * kTiles>(p, l, part, s);
-}
+Part part_of(const CacheAttend& p, const Launch& l) { return {l.over, l.upto, l.shares, log2_of(l.rows), p.work + l.offset}; }
 
 template <int kWidth, bool kFp8>
 hipError_t attend(const CacheAttend& p, const AttendShape& a, hipStream_t s) {
-    hipError_t error = hipSuccess;
+    const Part few = part_of(p, a.few), many = part_of(p, a.many);
     if (a.many.on) {
         constexpr int kWaves = many_waves(kWidth);
-        const Launch& l = a.many;
-        const Part part = {l.over, l.upto, l.shares, p.work + l.offset};
-        many_kernel<kWidth, kWaves, kFp8><<<static_cast<unsigned>((l.shares + l.tiles + 1) * p.heads), 64 * kWaves, 0, s>>>(p, part, true);
-        error = hipGetLastError();
-        if (error == hipSuccess && a.splits) error = join<kWidth, 32 * kWaves>(p, l, part, s);
+        const unsigned groups = static_cast<unsigned>((a.many.shares + a.many.tiles + 1) * p.heads);
+        many_kernel<kWidth, kWaves, kFp8><<<groups, 64 * kWaves, 0, s>>>(p, many, true);
     }
-    if (error != hipSuccess || !a.few.on) return error;
-    return a.few.rows == 16 ? few<kWidth, 1, kFp8>(p, a, s) : few<kWidth, 2, kFp8>(p, a, s);
+    if (a.few.on) {
+        const unsigned groups = static_cast<unsigned>((a.few.shares + a.few.tiles + 1) * p.heads);
+        if (a.few.rows == 16) few_kernel<kWidth, 1, kFp8><<<groups, 256, 0, s>>>(p, few, !a.many.on);
+        else few_kernel<kWidth, 2, kFp8><<<groups, 256, 0, s>>>(p, few, !a.many.on);
+    }
+    if (a.splits) {
+        const int64_t most = 0x7fffffff;
+        const int64_t few_items = a.few.on ? min(most, a.few.tiles * p.heads * a.few.row_groups) : 0;
+        const int64_t many_items = a.many.on ? min(most, a.many.tiles * p.heads * (a.many.rows / kJoinRows)) : 0;
+        const int64_t groups = max(few_items, (many_items + 3) / 4);
+        join_kernel<kWidth><<<dim3(static_cast<unsigned>(min(groups, static_cast<int64_t>(2048))), a.many.on ? 2 : 1), 256, 0, s>>>(
+            p, few, many, a.few.row_groups, static_cast<int>(few_items), static_cast<int>(many_items));
+    }
+    return hipGetLastError();
 }
 
 template <bool kFp8>
