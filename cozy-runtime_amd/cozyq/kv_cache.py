@@ -37,7 +37,7 @@ PAGES = (16, 32, 64, 128, 256)
 WIDTHS = (64, 128, 256)
 
 
-@dataclass(frozen=True, slots=True)
+@dataclass(slots=True)
 class Plan:
     """A step over a paged cache: `T` rows, the new tokens of `R` requests one request after another.
 
@@ -69,8 +69,13 @@ def plan(torch: Any, table: Tensor, free: Tensor, spare: Tensor, held: Tensor, n
     into `table` (int32 `[R, W]`, in place). A request whose rows would pass `tokens` has its count cut
     there. `out`: a plan of the same shape to write again (its `spare` and `lengths` may not be this
     call's inputs). Up to 4000 requests."""
-    index = _dispatch.card(OP, table)
-    return _dispatch.library(index).cache_plan(table, free, spare, held, new, tokens, page, most, out)
+    if most < 0:
+        raise ValueError(f"plan: a request has no {most} rows")
+    parts = _dispatch.library(_dispatch.card(OP, table)).cache_plan(table, free, spare, held, new, tokens, page, out)
+    if out is None:
+        return Plan(page, most, table, *parts)
+    out.most = most
+    return out
 
 
 def empty(torch: Any, pages: int, heads: int, width: int, *, page: int = 64, dtype: Dtype = None,
@@ -89,7 +94,7 @@ def empty(torch: Any, pages: int, heads: int, width: int, *, page: int = 64, dty
                       scales[0], scales[1])  # fmt: skip
 
 
-@dataclass(frozen=True, slots=True)
+@dataclass(slots=True)
 class PagedCache:
     """One layer's cache: codes `k` `[pages, heads, page, D]` and `v` `[pages, heads, D, page]` (int8 or
     float8_e4m3fn), float32 scales `k_scale` and `v_scale` `[pages, heads]`. `empty` makes one."""

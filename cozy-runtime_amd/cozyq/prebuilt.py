@@ -1063,90 +1063,99 @@ class Prebuilt:
     ) -> tuple[Tensor, Tensor | None]:
         """`heads.norm_rope` on this card (`cozyq_head_norm_rope`)."""
         torch = self.torch
-        half = self._half(q.dtype)
+        dtype = q.dtype
+        half = self._half(dtype)
         tokens, q_heads, width, q_token, q_head = self._heads("norm_rope", "q", q)
         if width > 256 or width % 16:
             raise ValueError(f"norm_rope: a head is a multiple of 16 up to 256 wide, not {width}")
         k_heads = k_token = k_head = 0
+        k_out = k_at = k_to = None
         if k is not None:
             k_tokens, k_heads, k_width, k_token, k_head = self._heads("norm_rope", "k", k)
-            if k.dtype != q.dtype or k_tokens != tokens or k_width != width:
-                raise ValueError(f"norm_rope: k must be {q.dtype} [{tokens}, heads, {width}], not {k.dtype} {list(k.shape)}")
+            if k.dtype is not dtype or k_tokens != tokens or k_width != width:
+                raise ValueError(f"norm_rope: k must be {dtype} [{tokens}, heads, {width}], not {k.dtype} {list(k.shape)}")
+            k_out = q.new_empty((tokens, k_heads, width))
+            k_at, k_to = k.data_ptr(), k_out.data_ptr()
+        else:
+            k_gain = None
         wide = False
-        gains = [g for g in (q_gain, None if k is None else k_gain) if g is not None]
-        if gains:
-            wide = gains[0].dtype is torch.float32
-            for g in gains:
-                if (g.dtype is not (torch.float32 if wide else q.dtype) or tuple(g.shape) != (width,)
-                        or not g.is_contiguous() or g.data_ptr() & 15):  # fmt: skip
-                    raise ValueError(f"norm_rope: gains are dense [{width}], 16-byte aligned, both float32 or {q.dtype}")
-            if eps is None:
-                raise ValueError("norm_rope: gains without a norm (eps None)")
+        q_by = k_by = None
+        if q_gain is not None:
+            wide = q_gain.dtype is torch.float32
+            q_by = self._gain(q_gain, torch.float32 if wide else dtype, width)
+        if k_gain is not None:
+            if q_gain is None:
+                wide = k_gain.dtype is torch.float32
+            k_by = self._gain(k_gain, torch.float32 if wide else dtype, width)
+        if eps is None and (q_by is not None or k_by is not None):
+            raise ValueError("norm_rope: gains without a norm (eps None)")
         rows = rotated = 0
-        if (cos is None) != (sin is None):
-            raise ValueError("norm_rope: cos and sin go together")
-        if cos is not None:
-            rows, rotated = int(cos.shape[0]), 2 * int(cos.shape[-1])
-            for t in (cos, sin):
-                if (t.dtype is not torch.float32 or tuple(t.shape) != (rows, rotated // 2) or not t.is_contiguous()
-                        or t.data_ptr() & 15):  # fmt: skip
-                    raise ValueError("norm_rope: cos and sin are dense float32 [rows, R/2], 16-byte aligned")
+        cos_at = sin_at = rows_at = None
+        if cos is not None and sin is not None:
+            rows, half_turn = cos.shape if cos.dim() == 2 else (0, 0)
+            rotated = 2 * half_turn
+            cos_at, sin_at = cos.data_ptr(), sin.data_ptr()
+            if (cos.dtype is not torch.float32 or sin.dtype is not torch.float32 or cos.shape != sin.shape
+                    or not cos.is_contiguous() or not sin.is_contiguous() or (cos_at | sin_at) & 15):  # fmt: skip
+                raise ValueError("norm_rope: cos and sin are dense float32 [rows, R/2], 16-byte aligned")
             if rotated > width or rotated % 16 or rows < 1 or (positions is None and rows < tokens):
-                raise ValueError(f"norm_rope: a table of [{rows}, {rotated // 2}] does not turn heads of {width} at "
-                                 f"{tokens} tokens (R a multiple of 16)")  # fmt: skip
+                raise ValueError(f"norm_rope: a table of [{rows}, {half_turn}] does not turn heads of {width} at {tokens} "
+                                 "tokens (R a multiple of 16)")  # fmt: skip
+        elif cos is not None or sin is not None:
+            raise ValueError("norm_rope: cos and sin go together")
         if positions is not None:
-            self._ints("norm_rope", "positions", positions, tokens)
-        if off_card(self.index, q, k, *gains, cos, sin, positions):
+            rows_at = self._ints("norm_rope", "positions", positions, tokens)
+        if self._elsewhere(q, k, q_gain, k_gain, cos, sin, positions):
             raise ValueError(f"norm_rope: every tensor must be on cuda:{self.index}")
-        q_out = torch.empty((tokens, q_heads, width), dtype=q.dtype, device=q.device)
-        k_out = None if k is None else torch.empty((tokens, k_heads, width), dtype=q.dtype, device=q.device)
+        q_out = q.new_empty((tokens, q_heads, width))
         code = self._lib.cozyq_head_norm_rope(
-            self.index, q.data_ptr(), _ptr(k), half, tokens, q_heads, k_heads, width, q_token, q_head, k_token,
-            k_head, eps is not None, _ptr(q_gain), None if k is None else _ptr(k_gain), wide, eps or 0.0, _ptr(cos),
-            _ptr(sin), rows, rotated, interleaved, _ptr(positions), q_out.data_ptr(), _ptr(k_out), self._stream(),
+            self.index, q.data_ptr(), k_at, half, tokens, q_heads, k_heads, width, q_token, q_head, k_token, k_head,
+            eps is not None, q_by, k_by, wide, eps or 0.0, cos_at, sin_at, rows, rotated, interleaved, rows_at,
+            q_out.data_ptr(), k_to, self._stream(),
         )  # fmt: skip
-        self._check(code, "the head norm and rotation")
+        if code:
+            self._check(code, "the head norm and rotation")
         return q_out, k_out
 
     def cache_plan(
-        self, table: Tensor, free: Tensor, spare: Tensor, held: Tensor, new: Tensor, tokens: int, page: int, most: int,
+        self, table: Tensor, free: Tensor, spare: Tensor, held: Tensor, new: Tensor, tokens: int, page: int,
         out: Any = None,
-    ) -> Any:
-        """`kv_cache.plan` on this card (`cozyq_cache_plan`)."""
-        from cozyq import kv_cache
-
-        torch = self.torch
-        if table.dtype is not torch.int32 or table.dim() != 2 or not table.is_contiguous():
+    ) -> tuple[Tensor, ...]:
+        """`kv_cache.plan` on this card (`cozyq_cache_plan`): a plan's starts, lengths, positions, requests,
+        slots, runs and spare, new or those of the plan `out`."""
+        int32 = self.torch.int32
+        if table.dtype is not int32 or table.dim() != 2 or not table.is_contiguous():
             raise ValueError("plan: the block table is dense int32 [requests, width]")
         requests, width = table.shape
-        runs = int(self._lib.cozyq_cache_runs(tokens, requests, page))
-        if requests < 1 or width < 1 or most < 0 or runs < 0:
-            raise ValueError(f"plan: {requests} requests of {width} pages, {tokens} tokens (most {most}) in pages of {page}: "
-                             f"1 to {self._lib.cozyq_cache_most_requests()} requests, pages of {kv_cache.PAGES}")  # fmt: skip
-        self._ints("plan", "held", held, requests)
-        self._ints("plan", "new", new, requests)
-        self._ints("plan", "free", free, free.numel())
-        if spare.dtype is not torch.int32 or spare.numel() < 1 or not spare.is_contiguous():
+        runs = self._lib.cozyq_cache_runs(tokens, requests, page) if requests > 0 < width else -1
+        if runs < 0:
+            raise ValueError(f"plan: {requests} requests of {width} pages, {tokens} tokens in pages of {page}: 1 to "
+                             f"{self._lib.cozyq_cache_most_requests()} requests, pages of 16, 32, 64, 128 or 256 tokens")  # fmt: skip
+        held_at = self._ints("plan", "held", held, requests)
+        new_at = self._ints("plan", "new", new, requests)
+        count = free.numel()
+        free_at = self._ints("plan", "free", free, count)
+        if spare.dtype is not int32 or spare.numel() < 1 or not spare.is_contiguous():
             raise ValueError("plan: spare is int32, the number of free pages first")
-        if off_card(self.index, table, free, spare, held, new):
+        if self._elsewhere(table, free, spare, held, new):
             raise ValueError(f"plan: every tensor must be on cuda:{self.index}")
         if out is None:
-            # One allocation; each part begins at a multiple of 16 bytes, the runs' rows first.
-            sizes = [4 * runs, *((n + 3) & ~3 for n in (requests + 1, requests, tokens, tokens, tokens, 2))]
-            parts = torch.empty(sum(sizes), dtype=torch.int32, device=table.device).split(sizes)
-            at, starts, lengths, positions, owners, slots, left = parts
-            out = kv_cache.Plan(page, most, table, starts[: requests + 1], lengths[:requests], positions[:tokens],
-                                owners[:tokens], slots[:tokens], at.view(runs, 4), left[:2])  # fmt: skip
+            # One allocation, the runs' rows of 16 bytes first.
+            sizes = (4 * runs, requests + 1, requests, tokens, tokens, tokens, 2)
+            at, starts, lengths, positions, owners, slots, left = table.new_empty(sum(sizes)).split_with_sizes(sizes)
+            at = at.view(runs, 4)
         else:
             self._same_plan(out, requests, tokens, runs, page, table, spare, held)
+            starts, lengths, positions, owners, slots, at, left = (
+                out.starts, out.lengths, out.positions, out.requests, out.slots, out.runs, out.spare)  # fmt: skip
         code = self._lib.cozyq_cache_plan(
-            self.index, table.data_ptr(), requests, width, free.data_ptr(), free.numel(), spare.data_ptr(),
-            held.data_ptr(), new.data_ptr(), tokens, page, out.starts.data_ptr(), out.lengths.data_ptr(),
-            out.positions.data_ptr(), out.requests.data_ptr(), out.slots.data_ptr(), out.runs.data_ptr(),
-            out.spare.data_ptr(), self._stream(),
+            self.index, table.data_ptr(), requests, width, free_at, count, spare.data_ptr(), held_at, new_at, tokens,
+            page, starts.data_ptr(), lengths.data_ptr(), positions.data_ptr(), owners.data_ptr(), slots.data_ptr(),
+            at.data_ptr(), left.data_ptr(), self._stream(),
         )  # fmt: skip
-        self._check(code, "the plan")
-        return out
+        if code:
+            self._check(code, "the plan")
+        return starts, lengths, positions, owners, slots, at, left
 
     def _same_plan(self, out: Any, requests: int, tokens: int, runs: int, page: int, table: Tensor, spare: Tensor,
                    held: Tensor) -> None:  # fmt: skip
@@ -1158,85 +1167,88 @@ class Prebuilt:
         if (out.page != page or out.table is not table or tuple(out.runs.shape) != (runs, 4)
                 or out.runs.dtype is not self.torch.int32 or not out.runs.is_contiguous()):  # fmt: skip
             raise ValueError("plan: out was made for another table, page size or number of runs")
+        if self._elsewhere(out.starts, out.lengths, out.positions, out.requests, out.slots, out.runs, out.spare):
+            raise ValueError(f"plan: every tensor must be on cuda:{self.index}")
         if out.spare.data_ptr() == spare.data_ptr() or out.lengths.data_ptr() == held.data_ptr():
             raise ValueError("plan: out's spare and lengths may not be this call's inputs")
 
     def cache_append(self, cache: Any, k: Tensor, v: Tensor, plan: Any) -> None:
         """`PagedCache.append` on this card (`cozyq_cache_append`)."""
-        half = self._half(k.dtype)
-        fp8, pages, heads, page, width = self._cache("append", cache)
+        dtype = k.dtype
+        half = self._half(dtype)
+        fp8, pages, heads, page, width, k_codes, v_codes, k_scale, v_scale = self._cache("append", cache)
         tokens, k_heads, k_width, k_token, k_head = self._heads("append", "k", k)
         v_tokens, v_heads, v_width, v_token, v_head = self._heads("append", "v", v)
-        if (k_heads, k_width) != (heads, width) or (v_tokens, v_heads, v_width) != (tokens, heads, width) or v.dtype != k.dtype:
-            raise ValueError(f"append: k and v must be [tokens, {heads}, {width}] of one type, not {k.dtype} {list(k.shape)} "
+        if (k_heads != heads or k_width != width or v_tokens != tokens or v_heads != heads or v_width != width
+                or v.dtype is not dtype):  # fmt: skip
+            raise ValueError(f"append: k and v must be [tokens, {heads}, {width}] of one type, not {dtype} {list(k.shape)} "
                              f"and {v.dtype} {list(v.shape)}")  # fmt: skip
         runs = plan.runs
-        if plan.page != page or int(plan.slots.shape[0]) != tokens:
+        if plan.page != page or plan.slots.shape[0] != tokens:
             raise ValueError(f"append: the plan is of {plan.slots.shape[0]} tokens in pages of {plan.page}, not of {tokens} in "
                              f"pages of {page}")  # fmt: skip
-        if runs.dtype is not self.torch.int32 or runs.dim() != 2 or runs.shape[1] != 4 or not runs.is_contiguous() or runs.data_ptr() & 15:
+        runs_at = runs.data_ptr()
+        if (runs.dtype is not self.torch.int32 or runs.dim() != 2 or runs.shape[1] != 4 or not runs.is_contiguous()
+                or runs_at & 15):  # fmt: skip
             raise ValueError("append: the plan's runs are dense int32 [n, 4], 16-byte aligned")
-        if off_card(self.index, cache.k, cache.v, cache.k_scale, cache.v_scale, k, v, runs):
+        if self._elsewhere(cache.k, cache.v, cache.k_scale, cache.v_scale, k, v, runs):
             raise ValueError(f"append: every tensor must be on cuda:{self.index}")
         code = self._lib.cozyq_cache_append(
-            self.index, fp8, k.data_ptr(), v.data_ptr(), half, tokens, k_token, k_head, v_token, v_head,
-            cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), pages, heads,
-            page, width, runs.data_ptr(), runs.shape[0], self._stream(),
+            self.index, fp8, k.data_ptr(), v.data_ptr(), half, tokens, k_token, k_head, v_token, v_head, k_codes,
+            v_codes, k_scale, v_scale, pages, heads, page, width, runs_at, runs.shape[0], self._stream(),
         )  # fmt: skip
-        self._check(code, "the cache's append")
+        if code:
+            self._check(code, "the cache's append")
 
     def cache_read(self, cache: Any, numbers: Tensor, dtype: Dtype) -> tuple[Tensor, Tensor]:
         """`PagedCache.read` on this card (`cozyq_cache_read`)."""
-        torch = self.torch
         half = self._half(dtype)
-        fp8, pages, heads, page, width = self._cache("read", cache)
-        self._ints("read", "pages", numbers, numbers.numel())
-        if off_card(self.index, cache.k, cache.v, cache.k_scale, cache.v_scale, numbers):
-            raise ValueError(f"read: every tensor must be on cuda:{self.index}")
+        fp8, pages, heads, page, width, k_codes, v_codes, k_scale, v_scale = self._cache("read", cache)
         count = numbers.numel()
-        k = torch.empty((count, heads, page, width), dtype=dtype, device=numbers.device)
-        v = torch.empty((count, heads, page, width), dtype=dtype, device=numbers.device)
+        numbers_at = self._ints("read", "pages", numbers, count)
+        if self._elsewhere(cache.k, cache.v, cache.k_scale, cache.v_scale, numbers):
+            raise ValueError(f"read: every tensor must be on cuda:{self.index}")
+        k, v = numbers.new_empty((2, count, heads, page, width), dtype=dtype).unbind(0)
         code = self._lib.cozyq_cache_read(
-            self.index, fp8, cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(),
-            cache.v_scale.data_ptr(), pages, heads, page, width, numbers.data_ptr(), count, k.data_ptr(),
-            v.data_ptr(), half, self._stream(),
+            self.index, fp8, k_codes, v_codes, k_scale, v_scale, pages, heads, page, width, numbers_at, count,
+            k.data_ptr(), v.data_ptr(), half, self._stream(),
         )  # fmt: skip
-        self._check(code, "the cache's read")
+        if code:
+            self._check(code, "the cache's read")
         return k, v
 
     def cache_attend(
         self, cache: Any, q: Tensor, plan: Any, scale: float | None, causal: bool, window: int
     ) -> Tensor:
         """`PagedCache.attend` on this card (`cozyq_cache_attend`)."""
-        torch = self.torch
         half = self._half(q.dtype)
-        fp8, pages, heads, page, width = self._cache("attend", cache)
+        fp8, pages, heads, page, width, k_codes, v_codes, k_scale, v_scale = self._cache("attend", cache)
         tokens, q_heads, q_width, q_token, q_head = self._heads("attend", "q", q)
         if q_width != width or q_heads % heads or not 0 < q_heads // heads <= 64:
             raise ValueError(f"attend: q must be [tokens, n x {heads}, {width}] with n up to 64, not {list(q.shape)}")
-        table, starts, lengths = plan.table, plan.starts, plan.lengths
-        if table.dtype is not torch.int32 or table.dim() != 2 or not table.is_contiguous():
+        table, starts, lengths, most = plan.table, plan.starts, plan.lengths, plan.most
+        if table.dtype is not self.torch.int32 or table.dim() != 2 or not table.is_contiguous():
             raise ValueError("attend: the block table is dense int32 [requests, width]")
-        requests, table_width = table.shape
-        self._ints("attend", "starts", starts, requests + 1)
-        self._ints("attend", "lengths", lengths, requests)
+        requests, columns = table.shape
+        starts_at = self._ints("attend", "starts", starts, requests + 1)
+        lengths_at = self._ints("attend", "lengths", lengths, requests)
         if plan.page != page:
             raise ValueError(f"attend: the plan has pages of {plan.page} tokens, the cache of {page}")
         if window < 0 or (window and not causal):
             raise ValueError(f"attend: a window of {window} tokens{'' if causal else ' without causal'}")
-        if off_card(self.index, cache.k, cache.v, cache.k_scale, cache.v_scale, q, table, starts, lengths):
+        if self._elsewhere(cache.k, cache.v, cache.k_scale, cache.v_scale, q, table, starts, lengths):
             raise ValueError(f"attend: every tensor must be on cuda:{self.index}")
-        out = torch.empty((tokens, q_heads, width), dtype=q.dtype, device=q.device)
-        size = self._lib.cozyq_cache_attend_workspace_bytes(tokens, q_heads, requests, heads, page, width,
-                                                            table_width, plan.most)
-        work = torch.empty(size, dtype=torch.uint8, device=q.device) if size > 0 else None
+        out = q.new_empty((tokens, q_heads, width))
+        size = self._lib.cozyq_cache_attend_workspace_bytes(tokens, q_heads, requests, heads, page, width, columns, most)
+        work = q.new_empty(size // 2) if size > 0 else None
         code = self._lib.cozyq_cache_attend(
-            self.index, fp8, q.data_ptr(), half, tokens, q_heads, q_token, q_head, cache.k.data_ptr(),
-            cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), pages, heads, page, width,
-            table.data_ptr(), requests, table_width, starts.data_ptr(), lengths.data_ptr(), plan.most,
-            width**-0.5 if scale is None else scale, causal, window, out.data_ptr(), _ptr(work), self._stream(),
+            self.index, fp8, q.data_ptr(), half, tokens, q_heads, q_token, q_head, k_codes, v_codes, k_scale, v_scale,
+            pages, heads, page, width, table.data_ptr(), requests, columns, starts_at, lengths_at, most,
+            width**-0.5 if scale is None else scale, causal, window, out.data_ptr(),
+            None if work is None else work.data_ptr(), self._stream(),
         )  # fmt: skip
-        self._check(code, "attention over the cache")
+        if code:
+            self._check(code, "attention over the cache")
         return out
 
     def _heads(self, op: str, name: str, x: Tensor) -> tuple[int, int, int, int, int]:
@@ -1246,30 +1258,53 @@ class Prebuilt:
             raise ValueError(f"{op}: {name} must be [tokens, heads, width], not {list(x.shape)}")
         tokens, heads, width = x.shape
         by_token, by_head, dense = x.stride()
-        if (dense != 1 and width > 1) or (by_token % 8 and tokens > 1) or (by_head % 8 and heads > 1) or x.data_ptr() & 15:
-            raise ValueError(f"{op}: {name}'s last axis must be dense, its other strides and address multiples of 16 bytes")
-        return tokens, heads, width, by_token & ~7, by_head & ~7
+        if (by_token | by_head) & 7 or dense != 1 or x.data_ptr() & 15:
+            # The stride of an extent of one is never taken.
+            if (dense != 1 and width > 1) or (by_token & 7 and tokens > 1) or (by_head & 7 and heads > 1) or x.data_ptr() & 15:
+                raise ValueError(f"{op}: {name}'s last axis must be dense, its other strides and address multiples of 16 bytes")
+            by_token, by_head = by_token & ~7, by_head & ~7
+        return tokens, heads, width, by_token, by_head
 
-    def _ints(self, op: str, name: str, x: Tensor, count: int) -> None:
-        """ValueError unless `x` is `count` dense int32 numbers."""
+    def _gain(self, gain: Tensor, dtype: Dtype, width: int) -> int:
+        """The address of a head gain; ValueError unless it is dense `[width]` of `dtype`."""
+        at = gain.data_ptr()
+        if gain.dtype is not dtype or gain.dim() != 1 or gain.shape[0] != width or not gain.is_contiguous() or at & 15:
+            raise ValueError(f"norm_rope: gains are dense [{width}], 16-byte aligned, both float32 or of q's type")
+        return at
+
+    def _ints(self, op: str, name: str, x: Tensor, count: int) -> int:
+        """The address of `count` dense int32 numbers; ValueError for other tensors."""
         if x.dtype is not self.torch.int32 or x.dim() != 1 or x.shape[0] != count or not x.is_contiguous():
             raise ValueError(f"{op}: {name} must be dense int32 [{count}], not {x.dtype} {list(x.shape)}")
+        return x.data_ptr()
 
-    def _cache(self, op: str, cache: Any) -> tuple[bool, int, int, int, int]:
-        """Whether a cache is E4M3, its pages, heads, page size and width; ValueError for tensors that
-        are no cache."""
+    def _elsewhere(self, *tensors: Tensor | None) -> bool:
+        """Whether any of the given tensors is not on this card (a CPU tensor's device number is -1)."""
+        index = self.index
+        for t in tensors:
+            if t is not None and t.get_device() != index:
+                return True
+        return False
+
+    def _cache(self, op: str, cache: Any) -> tuple[bool, int, int, int, int, int, int, int, int]:
+        """Whether a cache is E4M3, its pages, heads, page size and width, and its tensors' addresses;
+        ValueError for tensors that are no cache."""
         torch = self.torch
-        k, v = cache.k, cache.v
-        if k.dim() != 4 or k.dtype is not v.dtype or (k.dtype is not torch.int8 and k.dtype is not torch.float8_e4m3fn):
+        k, v, k_scale, v_scale = cache.k, cache.v, cache.k_scale, cache.v_scale
+        dtype = k.dtype
+        fp8 = dtype is not torch.int8
+        if k.dim() != 4 or v.dtype is not dtype or (fp8 and dtype is not torch.float8_e4m3fn):
             raise ValueError(f"{op}: the cache's codes are int8 or float8_e4m3fn [pages, heads, page, width]")
         pages, heads, page, width = k.shape
+        k_at, v_at = k.data_ptr(), v.data_ptr()
         if (v.shape != (pages, heads, width, page) or page not in (16, 32, 64, 128, 256) or width not in (64, 128, 256)
-                or not k.is_contiguous() or not v.is_contiguous() or (k.data_ptr() | v.data_ptr()) & 15):  # fmt: skip
+                or not k.is_contiguous() or not v.is_contiguous() or (k_at | v_at) & 15):  # fmt: skip
             raise ValueError(f"{op}: no cache of dense, 16-byte aligned keys {list(k.shape)} and values {list(v.shape)}")
-        for s in (cache.k_scale, cache.v_scale):
-            if s.dtype is not torch.float32 or s.shape != (pages, heads) or not s.is_contiguous():
-                raise ValueError(f"{op}: the cache's scales are dense float32 [{pages}, {heads}]")
-        return k.dtype is not torch.int8, pages, heads, page, width
+        shape, f32 = (pages, heads), torch.float32
+        if (k_scale.dtype is not f32 or v_scale.dtype is not f32 or k_scale.shape != shape or v_scale.shape != shape
+                or not k_scale.is_contiguous() or not v_scale.is_contiguous()):  # fmt: skip
+            raise ValueError(f"{op}: the cache's scales are dense float32 [{pages}, {heads}]")
+        return fp8, pages, heads, page, width, k_at, v_at, k_scale.data_ptr(), v_scale.data_ptr()
 
     def _half(self, dtype: Dtype) -> bool:
         """Contract V4: the kernels' flag for a 16-bit activation or output dtype (fp16 True,

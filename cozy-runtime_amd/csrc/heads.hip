@@ -10,31 +10,12 @@
 
 #include "common.h"
 #include "kernels.h"
+#include "sixteen.h"
 
 namespace cozyq {
 namespace {
 
 constexpr int kThreads = 256;
-
-__device__ __forceinline__ void load8(const uint16_t* p, bool half, float* v) {
-    const i32x4 raw = *reinterpret_cast<const i32x4*>(p);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const uint16_t h = static_cast<uint16_t>(static_cast<uint32_t>(raw[i / 2]) >> (16 * (i & 1)));
-        v[i] = half ? widen<true>(h) : widen<false>(h);
-    }
-}
-
-__device__ __forceinline__ void store8(uint16_t* p, bool half, const float* v) {
-    i32x4 raw;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const uint32_t lo = half ? narrow<true>(v[2 * i]) : narrow<false>(v[2 * i]);
-        const uint32_t hi = half ? narrow<true>(v[2 * i + 1]) : narrow<false>(v[2 * i + 1]);
-        raw[i] = static_cast<int32_t>(lo | (hi << 16));
-    }
-    *reinterpret_cast<i32x4*>(p) = raw;
-}
 
 __device__ __forceinline__ void load8f(const float* p, float* v) {
 #pragma unroll

@@ -18,6 +18,7 @@
 
 #include "common.h"
 #include "kernels.h"
+#include "sixteen.h"
 
 namespace cozyq {
 namespace {
@@ -65,14 +66,8 @@ __device__ __forceinline__ void rarely() { asm volatile(""); }
 // Four elements from d on of a row's result: the sums over its denominator, 0 for a row that sees nothing.
 __device__ __forceinline__ void store_row(const CacheAttend& p, int token, int head, int width, int d, f32x4 v, float total) {
     const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-    uint16_t h[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float f = v[i] * inv;
-        h[i] = p.half ? narrow<true>(f) : narrow<false>(f);
-    }
-    const i32x2 two = {static_cast<int32_t>(h[0] | (static_cast<uint32_t>(h[1]) << 16)),
-                       static_cast<int32_t>(h[2] | (static_cast<uint32_t>(h[3]) << 16))};
+    const i32x2 two = {static_cast<int32_t>(narrow2(v[0] * inv, v[1] * inv, p.half)),
+                       static_cast<int32_t>(narrow2(v[2] * inv, v[3] * inv, p.half))};
     *reinterpret_cast<i32x2*>(p.out + (static_cast<int64_t>(token) * p.q_heads + head) * width + d) = two;
 }
 
@@ -241,14 +236,11 @@ __device__ __forceinline__ void row_unit(uint32_t most, float& unit, float& down
     down = float_of(static_cast<uint32_t>(254 - e) << 23);
 }
 
-__device__ __forceinline__ void widen8(const CacheAttend& p, const uint16_t* x, float* v, uint32_t& most) {
-    const i32x4 raw = *reinterpret_cast<const i32x4*>(x);
+// Eight elements of a query row as float32, and their largest magnitude's bits.
+__device__ __forceinline__ void query8(const CacheAttend& p, const uint16_t* x, float* v, uint32_t& most) {
+    load8(x, p.half, v);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const uint16_t h = static_cast<uint16_t>(static_cast<uint32_t>(raw[i / 2]) >> (16 * (i & 1)));
-        v[i] = p.half ? widen<true>(h) : widen<false>(h);
-        most = max(most, bits_of(v[i]) & 0x7fffffffu);
-    }
+    for (int i = 0; i < 8; ++i) most = max(most, bits_of(v[i]) & 0x7fffffffu);
 }
 
 // ------------------------------------------------------------------------ few rows a request
@@ -305,8 +297,8 @@ __global__ __launch_bounds__(256, kWidth == 256 ? 1 : 2) void few_kernel(CacheAt
         uint32_t most = 0;
 #pragma unroll
         for (int b = 0; b < kBlocks; ++b) {
-            widen8(p, x + 64 * b + 16 * g, v[b], most);
-            widen8(p, x + 64 * b + 16 * g + 8, v[b] + 8, most);
+            query8(p, x + 64 * b + 16 * g, v[b], most);
+            query8(p, x + 64 * b + 16 * g + 8, v[b] + 8, most);
         }
         most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), 16)));
         most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), 32)));
@@ -556,7 +548,7 @@ __global__ __launch_bounds__(64 * kWaves, kWidth == 256 ? 1 : 2) void many_kerne
         uint32_t most = 0;
         float v[kDepth][8];
 #pragma unroll
-        for (int b = 0; b < kDepth; ++b) widen8(p, x + 16 * b, v[b], most);
+        for (int b = 0; b < kDepth; ++b) query8(p, x + 16 * b, v[b], most);
         most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), 32)));
         row_unit(most, unit, down);
         sharp = unit * p.scale * kLog2e;

@@ -9,6 +9,7 @@
 
 #include "common.h"
 #include "kernels.h"
+#include "sixteen.h"
 
 namespace cozyq {
 namespace {
@@ -163,60 +164,79 @@ __global__ __launch_bounds__(kThreads) void plan_kernel(CachePlan p) {
 
 // ---------------------------------------------------------------------------------- append
 
-// Magnitudes compare as their bits do, and an infinity or NaN is above every number: a page's
-// largest magnitude carries what is not finite into the page's scale.
-__device__ __forceinline__ uint32_t magnitude(uint16_t h, bool half) {
-    return bits_of(half ? widen<true>(h) : widen<false>(h)) & 0x7fffffffu;
-}
-
-__device__ __forceinline__ float value16(uint16_t h, bool half) { return half ? widen<true>(h) : widen<false>(h); }
-
-// The code of v (already over the scale): int8 by rint, E4M3 by the conversion, clamped to the
-// format's largest. A NaN (only where the scale is not finite) becomes code 0, so that codes are
-// always finite.
+// The codes of four values (already over the scale): int8 by rint, E4M3 by the conversion, clamped to the
+// format's largest. A NaN (only where the scale is not finite) becomes code 0: codes are always finite.
 template <bool kFp8>
-__device__ __forceinline__ uint32_t code_of(float v) {
+__device__ __forceinline__ uint32_t codes_of(const float* x) {
     constexpr float kMost = kFp8 ? kE4m3Max : 127.0f;
-    v = v != v ? 0.0f : fminf(fmaxf(v, -kMost), kMost);
-    if constexpr (kFp8) return static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(v, v, 0, false)) & 0xffu;
-    else return static_cast<uint32_t>(static_cast<int>(__builtin_rintf(v))) & 0xffu;
+    float v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = x[i] != x[i] ? 0.0f : fminf(fmaxf(x[i], -kMost), kMost);
+    if constexpr (kFp8) {
+        return e4m3x4(v[0], v[1], v[2], v[3]);
+    } else {
+        uint32_t c = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c |= (static_cast<uint32_t>(static_cast<int>(__builtin_rintf(v[i]))) & 0xffu) << (8 * i);
+        return c;
+    }
 }
 
+// A dword of codes at a new scale: code · ratio, rounded again.
 template <bool kFp8>
-__device__ __forceinline__ float code_value(uint32_t c) {
-    if constexpr (kFp8) return e4m3_value(c);
-    else return static_cast<float>(static_cast<int8_t>(c));
+__device__ __forceinline__ uint32_t rescaled(uint32_t c, float ratio) {
+    float v[4];
+    codes4f<kFp8>(c, v);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] *= ratio;
+    return codes_of<kFp8>(v);
 }
+
+// Bytes [from, to) of the dword whose first byte is number `at`.
+__device__ __forceinline__ uint32_t byte_mask(int at, int from, int to) {
+    const int a = max(from - at, 0), b = min(to - at, 4);
+    if (a >= b) return 0;
+    return (b == 4 ? 0xffffffffu : (1u << (8 * b)) - 1u) & ~((1u << (8 * a)) - 1u);
+}
+
+// Up to this many tokens of a page whose scale stands have their values stored byte by byte: a read of what
+// the page holds would be another trip to memory for 16 bytes of which one to a few change.
+constexpr int kFewTokens = 4;
 
 // One workgroup a (run, head, keys or values): the run's new tokens of one page. The scale is
 // max(the page's, largest new magnitude / largest code, 1e-12), the page's own only where it was
 // begun before. Where it grows, the codes that the page holds are rounded again at the new scale
-// (code · old/new); a page that the run begins is cleared past its tokens.
+// (code · old/new); a page that the run begins is cleared past its tokens. Magnitudes compare as their bits
+// do, and an infinity or NaN is above every number: what is not finite goes into the page's scale.
+// Elements are read eight at a time, twice (the second time out of L1 or L2). New values are transposed in
+// LDS, four tokens of a channel a dword, rows of page/4 + 1 dwords; both kinds leave 16 bytes a thread.
 template <bool kFp8>
-__global__ __launch_bounds__(kThreads) void append_kernel(CacheAppend p) {
+__global__ __launch_bounds__(kThreads) void append_kernel(CacheAppend p, int width_shift, int page_shift) {
+    extern __shared__ uint32_t turned[];
     __shared__ uint32_t wave_most[kWaves];
     const i32x4 run = *reinterpret_cast<const i32x4*>(p.runs + 4 * static_cast<int64_t>(blockIdx.x));
     const int row = run[0], count = run[1], page = run[2], offset = run[3];
     if (count <= 0 || page < 0 || page >= p.pages || row < 0 || row + count > p.tokens || offset < 0 ||
         offset + count > p.page)
         return;
-    const int head = blockIdx.y;
+    const int head = blockIdx.y, end = offset + count, eights = width_shift - 3;
     const bool values = blockIdx.z != 0;
     const uint16_t* x = values ? p.v + row * p.v_token + head * p.v_head : p.k + row * p.k_token + head * p.k_head;
     const int64_t token_step = values ? p.v_token : p.k_token;
     const int64_t tile = static_cast<int64_t>(page) * p.heads + head;
     uint8_t* codes = (values ? p.v_codes : p.k_codes) + tile * p.page * p.width;
     float* scale_at = (values ? p.v_scale : p.k_scale) + tile;
+    const float before = offset > 0 ? *scale_at : 0.0f;
 
     uint32_t most = 0;
-    for (int i = threadIdx.x; i < count * (p.width / 2); i += kThreads) {
-        const int t = i / (p.width / 2), d = 2 * (i - t * (p.width / 2));
-        const uint32_t two = *reinterpret_cast<const uint32_t*>(x + t * token_step + d);
-        most = max(most, max(magnitude(static_cast<uint16_t>(two), p.half), magnitude(static_cast<uint16_t>(two >> 16), p.half)));
+    for (int i = threadIdx.x; i < count << eights; i += kThreads) {
+        float v[8];
+        load8(x + (i >> eights) * token_step + 8 * (i & ((1 << eights) - 1)), p.half, v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) most = max(most, bits_of(v[j]) & 0x7fffffffu);
     }
     for (int step = 1; step < 64; step *= 2) most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), step)));
     if ((threadIdx.x & 63) == 0) wave_most[threadIdx.x >> 6] = most;
-    const float before = offset > 0 ? *scale_at : 0.0f;
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) most = max(most, wave_most[w]);
@@ -227,27 +247,81 @@ __global__ __launch_bounds__(kThreads) void append_kernel(CacheAppend p) {
     const bool keep = offset > 0 && bits_of(scale) == bits_of(before);
     if (threadIdx.x == 0 && !keep) *scale_at = scale;
 
-    // 16 codes a thread and step: of one token's keys, or of one channel's values.
-    const int chunks = p.page * p.width / 16;
-    for (int i = threadIdx.x; i < chunks; i += kThreads) {
-        // Values: neighbouring threads take neighbouring channels, whose new values are neighbours.
-        const int t0 = values ? 16 * (i / p.width) : i / (p.width / 16);
-        const int d0 = values ? i % p.width : 16 * (i % (p.width / 16));
-        const int last = values ? t0 + 15 : t0;
-        const bool any_new = last >= offset && t0 < offset + count;
-        if (keep && !any_new) continue;
-        i32x4* at = reinterpret_cast<i32x4*>(codes + (values ? static_cast<int64_t>(d0) * p.page + t0 : static_cast<int64_t>(t0) * p.width + d0));
-        i32x4 old = {0, 0, 0, 0}, got;
-        if (offset > 0) old = *at;
+    if (!values) {
+        // A thread: 16 channels of a token; where the scale stands, of the new tokens alone.
+        const int sixteens = width_shift - 4, first = keep ? offset : 0, last = keep ? end : p.page;
+        for (int i = threadIdx.x; i < (last - first) << sixteens; i += kThreads) {
+            const int t = first + (i >> sixteens), d = 16 * (i & ((1 << sixteens) - 1));
+            i32x4* at = reinterpret_cast<i32x4*>(codes + (static_cast<int64_t>(t) << width_shift) + d);
+            i32x4 got = {0, 0, 0, 0};
+            if (t >= offset && t < end) {
+                float v[16];
+                load8(x + (t - offset) * token_step + d, p.half, v);
+                load8(x + (t - offset) * token_step + d + 8, p.half, v + 8);
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-            const int t = values ? t0 + j : t0, d = values ? d0 : d0 + j;
-            uint32_t c = (static_cast<uint32_t>(old[j / 4]) >> (8 * (j & 3))) & 0xffu;
-            if (t >= offset && t < offset + count)
-                c = code_of<kFp8>(div_rn(value16(x[(t - offset) * token_step + d], p.half), scale, inv));
-            else if (!keep && offset > 0)
-                c = code_of<kFp8>(code_value<kFp8>(c) * ratio);
-            got[j / 4] = j % 4 ? static_cast<int32_t>(static_cast<uint32_t>(got[j / 4]) | (c << (8 * (j & 3)))) : static_cast<int32_t>(c);
+                for (int j = 0; j < 16; ++j) v[j] = div_rn(v[j], scale, inv);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) got[j] = static_cast<int32_t>(codes_of<kFp8>(v + 4 * j));
+            } else if (offset > 0) {
+                got = *at;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) got[j] = static_cast<int32_t>(rescaled<kFp8>(static_cast<uint32_t>(got[j]), ratio));
+            }
+            *at = got;
+        }
+        return;
+    }
+    if (keep && count <= kFewTokens) {
+        for (int i = threadIdx.x; i < count << eights; i += kThreads) {
+            const int t = i >> eights, d = 8 * (i & ((1 << eights) - 1));
+            float v[8];
+            load8(x + t * token_step + d, p.half, v);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = div_rn(v[j], scale, inv);
+            const uint32_t c[2] = {codes_of<kFp8>(v), codes_of<kFp8>(v + 4)};
+#pragma unroll
+            for (int j = 0; j < 8; ++j) codes[((d + j) << page_shift) + offset + t] = static_cast<uint8_t>(c[j / 4] >> (8 * (j & 3)));
+        }
+        return;
+    }
+    // A thread: four tokens of the page, eight channels.
+    const int pitch = (p.page >> 2) + 1, t_first = offset & ~3;
+    const int fours = (end - t_first + 3) >> 2;
+    for (int i = threadIdx.x; i < fours << eights; i += kThreads) {
+        const int t = t_first + 4 * (i >> eights), d = 8 * (i & ((1 << eights) - 1));
+        float v[4][8];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (t + j >= offset && t + j < end) {
+                load8(x + (t + j - offset) * token_step + d, p.half, v[j]);
+            } else {
+#pragma unroll
+                for (int k = 0; k < 8; ++k) v[j][k] = 0.0f;
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const float four[4] = {div_rn(v[0][k], scale, inv), div_rn(v[1][k], scale, inv), div_rn(v[2][k], scale, inv),
+                                   div_rn(v[3][k], scale, inv)};
+            turned[(d + k) * pitch + (t >> 2)] = codes_of<kFp8>(four);
+        }
+    }
+    __syncthreads();
+    // A thread: 16 tokens of a channel; where the scale stands, of those with new tokens alone.
+    const int first = keep ? offset >> 4 : 0, last = keep ? (end + 15) >> 4 : p.page >> 4;
+    const int chunks = last - first;
+    for (int i = threadIdx.x; i < chunks << width_shift; i += kThreads) {
+        const int d = i / chunks, t = 16 * (first + i - d * chunks);
+        i32x4* at = reinterpret_cast<i32x4*>(codes + (static_cast<int64_t>(d) << page_shift) + t);
+        i32x4 got = {0, 0, 0, 0};
+        if (offset > 0 && (t < offset || t + 16 > end)) got = *at;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            uint32_t c = static_cast<uint32_t>(got[j]);
+            if (!keep && offset > 0) c = rescaled<kFp8>(c, ratio);
+            const uint32_t mine = byte_mask(t + 4 * j, offset, end);
+            if (mine) c = (c & ~mine) | (turned[d * pitch + (t >> 2) + j] & mine);
+            got[j] = static_cast<int32_t>(c);
         }
         *at = got;
     }
@@ -255,21 +329,53 @@ __global__ __launch_bounds__(kThreads) void append_kernel(CacheAppend p) {
 
 // ------------------------------------------------------------------------------------ read
 
-// One workgroup a (listed page, head): its keys and values as 16-bit numbers, tokens by width.
+// One workgroup a (listed page, head): its keys and values as 16-bit numbers, tokens by width. A thread
+// takes 16 channels of a token's keys, and 16 tokens of four channels' values, which it turns in registers:
+// a wave's stores of a token's values are of neighbouring channels.
 template <bool kFp8>
-__global__ __launch_bounds__(kThreads) void read_kernel(CacheRead p) {
+__global__ __launch_bounds__(kThreads) void read_kernel(CacheRead p, int width_shift, int page_shift) {
     const int page = p.numbers[blockIdx.x], head = blockIdx.y;
     const int64_t to = (static_cast<int64_t>(blockIdx.x) * p.heads + head) * p.page * p.width;
-    const bool held = page >= 0 && page < p.pages;
-    const int64_t tile = static_cast<int64_t>(held ? page : 0) * p.heads + head;
-    const float ks = held ? p.k_scale[tile] : 0.0f, vs = held ? p.v_scale[tile] : 0.0f;
-    const uint8_t *k = p.k_codes + tile * p.page * p.width, *v = p.v_codes + tile * p.page * p.width;
-    for (int i = threadIdx.x; i < p.page * p.width; i += kThreads) {
-        const int t = i / p.width, d = i - t * p.width;
-        const float a = held ? code_value<kFp8>(k[i]) * ks : 0.0f;
-        const float b = held ? code_value<kFp8>(v[static_cast<int64_t>(d) * p.page + t]) * vs : 0.0f;
-        p.k_out[to + i] = p.half ? narrow<true>(a) : narrow<false>(a);
-        p.v_out[to + i] = p.half ? narrow<true>(b) : narrow<false>(b);
+    uint16_t *k_out = p.k_out + to, *v_out = p.v_out + to;
+    const int elements = p.page << width_shift;
+    if (page < 0 || page >= p.pages) {
+        for (int i = threadIdx.x; i < elements / 8; i += kThreads) {
+            reinterpret_cast<i32x4*>(k_out)[i] = i32x4{0, 0, 0, 0};
+            reinterpret_cast<i32x4*>(v_out)[i] = i32x4{0, 0, 0, 0};
+        }
+        return;
+    }
+    const int64_t tile = static_cast<int64_t>(page) * p.heads + head;
+    const float ks = p.k_scale[tile], vs = p.v_scale[tile];
+    const uint8_t *k = p.k_codes + tile * elements, *v = p.v_codes + tile * elements;
+    for (int i = threadIdx.x; i < elements / 16; i += kThreads) {
+        const i32x4 c = reinterpret_cast<const i32x4*>(k)[i];
+        float x[16];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) codes4f<kFp8>(static_cast<uint32_t>(c[j]), x + 4 * j);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) x[j] *= ks;
+        store8(k_out + 16 * i, p.half, x);
+        store8(k_out + 16 * i + 8, p.half, x + 8);
+    }
+    const int fours = width_shift - 2;
+    for (int i = threadIdx.x; i < elements / 64; i += kThreads) {
+        const int d = 4 * (i & ((1 << fours) - 1)), t = 16 * (i >> fours);
+        i32x4 c[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) c[j] = *reinterpret_cast<const i32x4*>(v + ((d + j) << page_shift) + t);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            float x[4][4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) codes4f<kFp8>(static_cast<uint32_t>(c[j][q]), x[j]);
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+                const i32x2 two = {static_cast<int32_t>(narrow2(x[0][s] * vs, x[1][s] * vs, p.half)),
+                                   static_cast<int32_t>(narrow2(x[2][s] * vs, x[3][s] * vs, p.half))};
+                *reinterpret_cast<i32x2*>(v_out + ((t + 4 * q + s) << width_shift) + d) = two;
+            }
+        }
     }
 }
 
@@ -283,17 +389,22 @@ hipError_t cache_plan(const CachePlan& p, hipStream_t s) {
     return hipGetLastError();
 }
 
+static int log2_of(int n) { return n > 1 ? 1 + log2_of(n / 2) : 0; }
+
 hipError_t cache_append(const CacheAppend& p, bool fp8, hipStream_t s) {
     const dim3 grid(static_cast<unsigned>(p.runs_most), static_cast<unsigned>(p.heads), 2);
-    if (fp8) append_kernel<true><<<grid, kThreads, 0, s>>>(p);
-    else append_kernel<false><<<grid, kThreads, 0, s>>>(p);
+    const size_t turned = static_cast<size_t>(p.width) * (p.page / 4 + 1) * 4;
+    const int w = log2_of(p.width), t = log2_of(p.page);
+    if (fp8) append_kernel<true><<<grid, kThreads, turned, s>>>(p, w, t);
+    else append_kernel<false><<<grid, kThreads, turned, s>>>(p, w, t);
     return hipGetLastError();
 }
 
 hipError_t cache_read(const CacheRead& p, bool fp8, hipStream_t s) {
     const dim3 grid(static_cast<unsigned>(p.count), static_cast<unsigned>(p.heads));
-    if (fp8) read_kernel<true><<<grid, kThreads, 0, s>>>(p);
-    else read_kernel<false><<<grid, kThreads, 0, s>>>(p);
+    const int w = log2_of(p.width), t = log2_of(p.page);
+    if (fp8) read_kernel<true><<<grid, kThreads, 0, s>>>(p, w, t);
+    else read_kernel<false><<<grid, kThreads, 0, s>>>(p, w, t);
     return hipGetLastError();
 }
 
