@@ -95,12 +95,12 @@ __device__ __forceinline__ T wave_prefix(T x) {
 // --------------------------------------------------------------------- sharing the work out
 
 constexpr int kStep = 64;       // tokens taken at a time
-constexpr int kMinSteps = 16;   // steps a workgroup takes at the least
 
 // Which requests a launch takes: those of more than `over` and up to `upto` rows, in row tiles shared
 // out over `shares` workgroups a head.
 struct Part {
     int over, upto, shares;
+    int least;    // steps a workgroup takes at the least
     int shift;    // a row tile is 1 << shift rows
     float* work;  // places of a row tile's rows · (width + 4) floats: a row's sums, reference, denominator
 };
@@ -114,7 +114,8 @@ __device__ __forceinline__ Extent extent(const CacheAttend& p, const Part& part,
     const int fresh = row_start(p, r + 1) - row_start(p, r), length = p.lengths[r], rows = fresh * p.group;
     if (rows <= part.over || rows > part.upto) return {0, 0};
     const int low = p.window > 0 ? max(0, length - fresh + 1 - p.window) : 0;
-    const int steps = (max(length, 0) + kStep - 1) / kStep - low / kStep;
+    const int held = min(max(length, 0), p.width << p.shift);  // what the table's row has pages for
+    const int steps = (held + kStep - 1) / kStep - low / kStep;
     return {(rows + (1 << part.shift) - 1) >> part.shift, max(steps, 0)};
 }
 
@@ -125,7 +126,7 @@ struct Share {
 };
 
 // All the row tiles' steps are shared out evenly: with N steps in all (a head), a workgroup takes
-// c = max(kMinSteps, N / shares) of one row tile's, so that there are at most shares + tiles workgroups
+// c = max(least, N / shares) of one row tile's, so that there are at most shares + tiles workgroups
 // and at most 2 · shares places (a tile of more than c steps splits into less than 2 · steps / c),
 // whatever the requests' lengths are: the host sizes the launch and the workspace without knowing them.
 // Finds workgroup `id`'s share (kById), or row tile `id`'s first; false past the last, and for row tiles
@@ -136,19 +137,21 @@ __device__ bool find_share(const CacheAttend& p, const Part& part, int id, Share
     const int lane = threadIdx.x & 63;
     float work = 0.0f;  // in float32, which no number of steps overflows; the margin is over its rounding
     int longest = 0;
+    Extent e0 = {0, 0};
     for (int base = 0; base < p.requests; base += 64) {
         Extent e = {0, 0};
         if (base + lane < p.requests) e = extent(p, part, base + lane);
         const float sum = wave_prefix(static_cast<float>(e.tiles) * static_cast<float>(e.steps));
         work += __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, sum), 63));
         longest = max(longest, e.steps);
+        if (base == 0) e0 = e;
     }
-    const int c = max(kMinSteps, static_cast<int>(work * 1.001f / static_cast<float>(part.shares)) + 1);
+    const int c = max(part.least, static_cast<int>(work * 1.001f / static_cast<float>(part.shares)) + 1);
     if (!kById && !__any(longest > c)) return false;  // nothing is split: nothing to join
     int ids_before = 0, places_before = 0;
     for (int base = 0; base < p.requests; base += 64) {
-        Extent e = {0, 0};
-        if (base + lane < p.requests) e = extent(p, part, base + lane);
+        Extent e = e0;
+        if (base) e = base + lane < p.requests ? extent(p, part, base + lane) : Extent{0, 0};
         const int splits = max(1, (e.steps + c - 1) / c);
         const int ids = wave_prefix(kById ? e.tiles * splits : e.tiles);
         const int places = wave_prefix(splits > 1 ? e.tiles * splits : 0);
@@ -164,6 +167,84 @@ __device__ bool find_share(const CacheAttend& p, const Part& part, int id, Share
         }
         ids_before += __builtin_amdgcn_readlane(ids, 63);
         places_before += __builtin_amdgcn_readlane(places, 63);
+    }
+    return false;
+}
+
+// The few rows' work, shared out to the step: the steps of all row tiles, one tile after another, are cut
+// into equal runs of c = max(least, N / shares), one a workgroup, wherever the cuts fall. A workgroup
+// then takes the end of one tile, whole tiles and the beginning of another, and leaves sums to be joined for
+// the first and the last alone: two places each. Where runs of `least` steps are enough workgroups even if
+// none of them holds two tiles' steps (`aligned`), none does: the second tile would only wait for the first.
+// Positions count units of 1 << shift steps, one but for N past 2^29.
+struct Survey {
+    Extent first;  // of the lane's request among the first 64
+    int c, shift, total;
+    bool aligned;
+};
+
+__device__ __forceinline__ Extent extent_at(const CacheAttend& p, const Part& part, const Survey& sv, int base) {
+    if (base == 0) return sv.first;
+    const int r = base + (threadIdx.x & 63);
+    return r < p.requests ? extent(p, part, r) : Extent{0, 0};
+}
+
+// A row tile's units: at the least one, so that a tile that sees nothing is written too; whole runs where
+// they are aligned.
+__device__ __forceinline__ int units_of(const Extent& e, const Survey& sv) {
+    const int units = max(1, (e.steps + (1 << sv.shift) - 1) >> sv.shift);
+    return sv.aligned ? (units + sv.c - 1) / sv.c * sv.c : units;
+}
+
+__device__ Survey survey(const CacheAttend& p, const Part& part) {
+    const int lane = threadIdx.x & 63;
+    Survey sv = {lane < p.requests ? extent(p, part, lane) : Extent{0, 0}, 0, 0, 0, false};
+    float work = 0.0f;
+    for (int base = 0; base < p.requests; base += 64) {
+        const Extent e = extent_at(p, part, sv, base);
+        const float sum = wave_prefix(static_cast<float>(e.tiles) * static_cast<float>(max(e.steps, 1)));
+        work += __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, sum), 63));
+    }
+    sv.shift = max(0, static_cast<int>(bits_of(work) >> 23) - 127 - 28);
+    sv.c = max(part.least >> sv.shift, 1);
+    int runs = 0;
+    for (int base = 0; base < p.requests; base += 64) {
+        const Extent e = extent_at(p, part, sv, base);
+        const int units = units_of(e, sv);
+        sv.total += __builtin_amdgcn_readlane(wave_prefix(e.tiles * units), 63);
+        runs += __builtin_amdgcn_readlane(wave_prefix(e.tiles * ((units + sv.c - 1) / sv.c)), 63);
+    }
+    sv.aligned = runs <= part.shares;
+    if (sv.aligned) sv.total = runs * sv.c;
+    else sv.c = max(sv.c, (sv.total + part.shares - 1) / part.shares);
+    return sv;
+}
+
+// A row tile, its units [start, start + units) of all.
+struct Item {
+    int request, tile, start, units;
+};
+
+// The tile that unit `id` is of (kByUnit), or tile number `id`; false past the last.
+template <bool kByUnit>
+__device__ bool find_item(const CacheAttend& p, const Part& part, const Survey& sv, int id, Item& out) {
+    int ids_before = 0, units_before = 0;
+    for (int base = 0; base < p.requests; base += 64) {
+        const Extent e = extent_at(p, part, sv, base);
+        const int one = units_of(e, sv);
+        const int units = wave_prefix(e.tiles * one), tiles = wave_prefix(e.tiles);
+        const int ids = kByUnit ? units : tiles;
+        const uint64_t past = __ballot(ids_before + ids > id);
+        if (past) {
+            const int at = __ffsll(static_cast<unsigned long long>(past)) - 1;
+            const int u = __builtin_amdgcn_readlane(one, at), t = __builtin_amdgcn_readlane(e.tiles, at);
+            const int from = id - ids_before - __builtin_amdgcn_readlane(ids, at) + (kByUnit ? t * u : t);
+            const int tile = kByUnit ? from / u : from;
+            out = {base + at, tile, units_before + __builtin_amdgcn_readlane(units, at) - (t - tile) * u, u};
+            return true;
+        }
+        ids_before += __builtin_amdgcn_readlane(ids, 63);
+        units_before += __builtin_amdgcn_readlane(units, 63);
     }
     return false;
 }
@@ -188,7 +269,7 @@ struct Span {
     int begin, end, low_least, low_most, high_least, high_most;
 };
 
-__device__ __forceinline__ Span span_of(const CacheAttend& p, int row0, int rows, int fresh, int length, int split, int splits) {
+__device__ __forceinline__ Span span_of(const CacheAttend& p, int row0, int rows, int fresh, int length, int split = 0, int splits = 1) {
     const int before = length - fresh, t0 = row0 / p.group, t1 = (rows - 1) / p.group;
     Span s;
     s.low_least = p.window > 0 ? max(0, before + t0 + 1 - p.window) : 0;
@@ -245,14 +326,14 @@ __device__ __forceinline__ void query8(const CacheAttend& p, const uint16_t* x, 
 
 // ------------------------------------------------------------------------ few rows a request
 
-// Four waves take a row tile of 16 rows (kTiles of them) of one key head, the heads that share it token
-// by token, over the workgroup's share of its tokens: each wave every fourth step of 64. Both products
+// Four waves take row tiles of 16 rows (kTiles of them) of one key head, the heads that share it token
+// by token, over the workgroup's run of their tokens: each wave every fourth step of 64. Both products
 // are taken transposed, Sᵀ = K·Qᵀ and Oᵀ = Vᵀ·Pᵀ, on v_mfma_f32_16x16x32_f16, so that a query row is a
 // column of both results: lane l holds column l%16. Score tile j's row m is token 16·(m/4) + 4j + m%4
 // of the step, which leaves lane group g = l/16 with the scores of tokens 16g .. 16g+15 in order: all
 // of one page (pages are multiples of 16 tokens), one scale each, and exactly the 16 bytes of a channel's
 // values that the group loads for the second product. Codes go from memory to registers to the matrix
-// unit; nothing of the cache passes through LDS but its pages' numbers and scales, read once a share.
+// unit; nothing of the cache passes through LDS but its pages' numbers and scales, read once a tile.
 // A step's keys are loaded over the previous step's second product and its values over its first.
 template <int kWidth, int kTiles, bool kFp8>
 __global__ __launch_bounds__(256, kWidth == 256 ? 1 : 2) void few_kernel(CacheAttend p, Part part, bool clears) {
@@ -263,240 +344,271 @@ __global__ __launch_bounds__(256, kWidth == 256 ? 1 : 2) void few_kernel(CacheAt
     const int thread = threadIdx.x, lane = thread & 63, wave = __builtin_amdgcn_readfirstlane(thread >> 6);
     const int col = lane & 15, g = lane >> 4;
     const int kv = blockIdx.x % p.heads, id = blockIdx.x / p.heads;
-    Share share;
-    if (!find_share<true>(p, part, id, share)) {
+    const Survey sv = survey(p, part);
+    const int64_t run_begin = static_cast<int64_t>(id) * sv.c;
+    if (run_begin >= sv.total) {
         if (clears) clear_rest(p, kWidth);
         return;
     }
-    const int first = row_start(p, share.request), fresh = row_start(p, share.request + 1) - first;
-    const int length = p.lengths[share.request], rows = fresh * p.group;
-
-    // Tokens [low, high) of each of the lane's rows, of which the tile's steps span [begin, end).
-    int low[kTiles], high[kTiles], token[kTiles], head[kTiles];
-    bool live[kTiles];
-#pragma unroll
-    for (int n = 0; n < kTiles; ++n) {
-        const int row = kRows * share.tile + 16 * n + col;
-        live[n] = row < rows;
-        token[n] = live[n] ? row / p.group : 0;
-        head[n] = kv * p.group + (live[n] ? row - token[n] * p.group : 0);
-        const int position = length - fresh + token[n];
-        high[n] = live[n] ? (p.causal ? position + 1 : length) : 0;
-        low[n] = live[n] ? (p.window > 0 ? max(0, position + 1 - p.window) : 0) : 0x7fffffff;
-    }
-    const Span span = span_of(p, kRows * share.tile, min(rows, kRows * (share.tile + 1)), fresh, length, share.split, share.splits);
-
-    // Each row brought to a largest magnitude of about 2^12; a lane holds elements 64b + 16g .. + 15 of
-    // each block of 64, as two operands.
-    f16x8 q[kTiles][kBlocks][2];
-    float sharp[kTiles];
-#pragma unroll
-    for (int n = 0; n < kTiles; ++n) {
-        const uint16_t* x = p.q + (first + token[n]) * p.q_token + head[n] * p.q_head;
-        float v[kBlocks][16], unit, down;
-        uint32_t most = 0;
-#pragma unroll
-        for (int b = 0; b < kBlocks; ++b) {
-            query8(p, x + 64 * b + 16 * g, v[b], most);
-            query8(p, x + 64 * b + 16 * g + 8, v[b] + 8, most);
-        }
-        most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), 16)));
-        most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), 32)));
-        row_unit(most, unit, down);
-        sharp[n] = unit * p.scale * kLog2e;
-#pragma unroll
-        for (int b = 0; b < kBlocks; ++b) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) q[n][b][i / 8][i % 8] = static_cast<_Float16>(v[b][i] * down);
-        }
-    }
-
-    // `ref` is subtracted from every exponent. It follows the row's largest, set 2^kLift below it when a
-    // row sees its first token and moved up only when a weight would pass 2^15: most steps need neither
-    // the maximum over the lane groups nor the accumulators' scaling. `bound` is −inf until it is set.
-    f32x4 acc[kTiles][kOut];
-    float ref[kTiles], bound[kTiles], total[kTiles];
-#pragma unroll
-    for (int n = 0; n < kTiles; ++n) {
-#pragma unroll
-        for (int i = 0; i < kOut; ++i) acc[n][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        ref[n] = total[n] = 0.0f;
-        bound[n] = -__builtin_inff();
-    }
-    const int* table = p.table + static_cast<int64_t>(share.request) * p.width;
+    const int run_from = static_cast<int>(run_begin), run_to = static_cast<int>(min(run_begin + sv.c, static_cast<int64_t>(sv.total)));
     const int within = p.page - 1;
     const uint8_t* k_lane = p.k_codes + static_cast<int64_t>(kv) * p.page * kWidth + (col & 3) * kWidth + 16 * g;
     const uint8_t* v_lane = p.v_codes + static_cast<int64_t>(kv) * p.page * kWidth + col * p.page;
     const int64_t page_bytes = static_cast<int64_t>(p.heads) * p.page * kWidth;
 
-    i32x4 kc[4][kBlocks], vc[kOut];
-    for (int stage = span.begin; stage < span.end; stage += kStage) {
-        const int stage_end = min(span.end, stage + kStage);
-        const int page_first = stage * kStep >> p.shift;
-        if (stage != span.begin) __syncthreads();
-        stage_pages(p, entries, table, length, kv, page_first, stage_end);
-        __syncthreads();
+    Item item;
+    for (int at = run_from; at < run_to && find_item<true>(p, part, sv, at, item);) {
+        const int first = row_start(p, item.request), fresh = row_start(p, item.request + 1) - first;
+        const int length = p.lengths[item.request], rows = fresh * p.group;
+        const int stop = min(item.start + item.units, run_to);
+        const bool split = item.start < run_from || item.start + item.units > run_to;
+        const int place = 2 * id + (at != run_from);
 
-        const auto load_keys = [&](int step) {
-            const int t = step * kStep + 16 * (col >> 2);
-            const int page = max(entries[(t >> p.shift) - page_first].page, 0);
-            const uint8_t* k = k_lane + page * page_bytes + static_cast<int64_t>(t & within) * kWidth;
+        // Tokens [low, high) of each of the lane's rows, of which the segment's steps span [begin, end).
+        int low[kTiles], high[kTiles], token[kTiles], head[kTiles];
+        i32x4 raw[kTiles][kBlocks][2];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-#pragma unroll
-                for (int b = 0; b < kBlocks; ++b) kc[j][b] = *reinterpret_cast<const i32x4*>(k + 4 * j * kWidth + 64 * b);
-            }
-        };
-        const auto load_values = [&](int step) {
-            const int t = step * kStep + 16 * g;
-            const int page = max(entries[(t >> p.shift) - page_first].page, 0);
-            const uint8_t* v = v_lane + page * page_bytes + (t & within);
-#pragma unroll
-            for (int o = 0; o < kOut; ++o) vc[o] = *reinterpret_cast<const i32x4*>(v + 16 * o * p.page);
-        };
-        int step = stage + wave;
-        if (step < stage_end) {
-            load_keys(step);
-            load_values(step);
+        for (int n = 0; n < kTiles; ++n) {
+            const int row = kRows * item.tile + 16 * n + col;
+            const bool live = row < rows;
+            token[n] = live ? row / p.group : 0;
+            head[n] = kv * p.group + (live ? row - token[n] * p.group : 0);
+            const int position = length - fresh + token[n];
+            high[n] = live ? (p.causal ? position + 1 : length) : 0;
+            low[n] = live ? (p.window > 0 ? max(0, position + 1 - p.window) : 0) : 0x7fffffff;
         }
-        for (; step < stage_end; step += kWaves) {
-            const int t0 = step * kStep, mine = t0 + 16 * g;
-            const PageScales page = entries[(mine >> p.shift) - page_first];
-            const bool whole = t0 >= span.low_most && t0 + kStep <= span.high_least && __all(page.page >= 0);
-            f32x4 s[kTiles][4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-#pragma unroll
-                for (int n = 0; n < kTiles; ++n) s[n][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int b = 0; b < kBlocks; ++b) {
-                    const f16x8 k0 = codes8<kFp8>(kc[j][b][0], kc[j][b][1]), k1 = codes8<kFp8>(kc[j][b][2], kc[j][b][3]);
-#pragma unroll
-                    for (int n = 0; n < kTiles; ++n) {
-                        s[n][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, q[n][b][0], s[n][j], 0, 0, 0);
-                        s[n][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, q[n][b][1], s[n][j], 0, 0, 0);
-                    }
-                }
-            }
-            if (step + kWaves < stage_end) load_keys(step + kWaves);
-
-            f16x8 w[kTiles][2];
+        // The rows, read before the pages are looked up where there is one tile of them.
+        const auto read_rows = [&]() {
 #pragma unroll
             for (int n = 0; n < kTiles; ++n) {
-                const float mul = sharp[n] * page.keys, add = page.values_log - ref[n];
-                float x[16], most = -__builtin_inff();
+                const uint16_t* x = p.q + (first + token[n]) * p.q_token + head[n] * p.q_head + 16 * g;
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    x[i] = __builtin_fmaf(s[n][i / 4][i % 4], mul, add);
+                for (int b = 0; b < kBlocks; ++b) {
+                    raw[n][b][0] = *reinterpret_cast<const i32x4*>(x + 64 * b);
+                    raw[n][b][1] = *reinterpret_cast<const i32x4*>(x + 64 * b + 8);
+                }
+            }
+        };
+        if constexpr (kTiles == 1) read_rows();
+        const Span span = span_of(p, kRows * item.tile, min(rows, kRows * (item.tile + 1)), fresh, length);
+        const int base = (p.window > 0 ? max(0, length - fresh + 1 - p.window) : 0) / kStep;
+        const int begin = max(span.begin, base + ((at - item.start) << sv.shift));
+        const int end = stop == item.start + item.units ? span.end : min(span.end, base + ((stop - item.start) << sv.shift));
+        const int* table = p.table + static_cast<int64_t>(item.request) * p.width;
+        at = stop;
+
+        // Each row brought to a largest magnitude of about 2^12; a lane holds elements 64b + 16g .. + 15 of
+        // each block of 64, as two operands.
+        f16x8 q[kTiles][kBlocks][2];
+        float sharp[kTiles];
+        const auto bring_rows = [&]() {
+            if constexpr (kTiles > 1) read_rows();
+#pragma unroll
+            for (int n = 0; n < kTiles; ++n) {
+                float v[kBlocks][16], unit, down;
+                uint32_t most = 0;
+#pragma unroll
+                for (int b = 0; b < kBlocks; ++b) {
+                    widen8(raw[n][b][0], p.half, v[b]);
+                    widen8(raw[n][b][1], p.half, v[b] + 8);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) most = max(most, bits_of(v[b][i]) & 0x7fffffffu);
+                }
+                most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), 16)));
+                most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), 32)));
+                row_unit(most, unit, down);
+                sharp[n] = unit * p.scale * kLog2e;
+#pragma unroll
+                for (int b = 0; b < kBlocks; ++b) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) q[n][b][i / 8][i % 8] = static_cast<_Float16>(v[b][i] * down);
+                }
+            }
+        };
+
+        // `ref` is subtracted from every exponent. It follows the row's largest, set 2^kLift below it when a
+        // row sees its first token and moved up only when a weight would pass 2^15: most steps need neither
+        // the maximum over the lane groups nor the accumulators' scaling. `bound` is −inf until it is set.
+        f32x4 acc[kTiles][kOut];
+        float ref[kTiles], bound[kTiles], total[kTiles];
+#pragma unroll
+        for (int n = 0; n < kTiles; ++n) {
+#pragma unroll
+            for (int i = 0; i < kOut; ++i) acc[n][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            ref[n] = total[n] = 0.0f;
+            bound[n] = -__builtin_inff();
+        }
+
+        i32x4 kc[4][kBlocks], vc[kOut];
+        for (int stage = begin; stage < end; stage += kStage) {
+            const int stage_end = min(end, stage + kStage);
+            const int page_first = stage * kStep >> p.shift;
+            if (stage != begin) __syncthreads();
+            stage_pages(p, entries, table, length, kv, page_first, stage_end);
+            if (stage == begin) bring_rows();
+            __syncthreads();
+            const auto load_keys = [&](int step) {
+                const int t = step * kStep + 16 * (col >> 2);
+                const int page = max(entries[(t >> p.shift) - page_first].page, 0);
+                const uint8_t* k = k_lane + page * page_bytes + static_cast<int64_t>(t & within) * kWidth;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+#pragma unroll
+                    for (int b = 0; b < kBlocks; ++b) kc[j][b] = *reinterpret_cast<const i32x4*>(k + 4 * j * kWidth + 64 * b);
+                }
+            };
+            const auto load_values = [&](int step) {
+                const int t = step * kStep + 16 * g;
+                const int page = max(entries[(t >> p.shift) - page_first].page, 0);
+                const uint8_t* v = v_lane + page * page_bytes + (t & within);
+#pragma unroll
+                for (int o = 0; o < kOut; ++o) vc[o] = *reinterpret_cast<const i32x4*>(v + 16 * o * p.page);
+            };
+            int step = stage + wave;
+            if (step < stage_end) {
+                load_keys(step);
+                load_values(step);
+            }
+            for (; step < stage_end; step += kWaves) {
+                const int t0 = step * kStep, mine = t0 + 16 * g;
+                const PageScales page = entries[(mine >> p.shift) - page_first];
+                const bool whole = t0 >= span.low_most && t0 + kStep <= span.high_least && __all(page.page >= 0);
+                f32x4 s[kTiles][4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+#pragma unroll
+                    for (int n = 0; n < kTiles; ++n) s[n][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int b = 0; b < kBlocks; ++b) {
+                        const f16x8 k0 = codes8<kFp8>(kc[j][b][0], kc[j][b][1]), k1 = codes8<kFp8>(kc[j][b][2], kc[j][b][3]);
+#pragma unroll
+                        for (int n = 0; n < kTiles; ++n) {
+                            s[n][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, q[n][b][0], s[n][j], 0, 0, 0);
+                            s[n][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, q[n][b][1], s[n][j], 0, 0, 0);
+                        }
+                    }
+                }
+                if (step + kWaves < stage_end) load_keys(step + kWaves);
+
+                f16x8 w[kTiles][2];
+#pragma unroll
+                for (int n = 0; n < kTiles; ++n) {
+                    const float mul = sharp[n] * page.keys, add = page.values_log - ref[n];
+                    float x[16], most = -__builtin_inff();
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        x[i] = __builtin_fmaf(s[n][i / 4][i % 4], mul, add);
+                    }
+                    if (!whole) {
+                        rarely();
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            if (page.page < 0 || mine + i < low[n] || mine + i >= high[n]) x[i] = -__builtin_inff();
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) most = fmaxf(most, x[i]);
+                    if (__any(most > bound[n])) {
+                        most = fmaxf(most, __shfl_xor(most, 16));
+                        most = fmaxf(most, __shfl_xor(most, 32));
+                        const float up = most > bound[n] ? most - kLift : 0.0f;
+                        // Nothing is there to scale before the row's first token, and 0 · 2^-up may be 0 · inf.
+                        const float shrink = bound[n] > 0.0f ? __builtin_amdgcn_exp2f(-up) : 0.0f;
+                        if (most > bound[n]) bound[n] = 15.0f;
+                        ref[n] += up;
+                        total[n] *= shrink;
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) x[i] -= up;
+#pragma unroll
+                        for (int o = 0; o < kOut; ++o) {
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) acc[n][o][i] *= shrink;
+                        }
+                    }
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const float e = __builtin_amdgcn_exp2f(x[i]);
+                        sum += e;
+                        w[n][i / 8][i % 8] = static_cast<_Float16>(e);
+                    }
+                    // A group whose tokens the row does not see adds nothing, whatever its page's scale is.
+                    total[n] += sum == 0.0f ? 0.0f : sum * page.values_inv;
                 }
                 if (!whole) {
                     rarely();
+                    // Bytes past the request's tokens may hold anything, a NaN of the format too.
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        if (page.page < 0 || mine + i < low[n] || mine + i >= high[n]) x[i] = -__builtin_inff();
+                    for (int i = 0; i < 4; ++i) {
+                        const int n = page.page >= 0 ? length - mine - 4 * i : 0;
+                        const int kept = n >= 4 ? -1 : n <= 0 ? 0 : (1 << (8 * n)) - 1;
+#pragma unroll
+                        for (int o = 0; o < kOut; ++o) vc[o][i] &= kept;
                     }
                 }
 #pragma unroll
-                for (int i = 0; i < 16; ++i) most = fmaxf(most, x[i]);
-                if (__any(most > bound[n])) {
-                    most = fmaxf(most, __shfl_xor(most, 16));
-                    most = fmaxf(most, __shfl_xor(most, 32));
-                    const float up = most > bound[n] ? most - kLift : 0.0f;
-                    // Nothing is there to scale before the row's first token, and 0 · 2^-up may be 0 · inf.
-                    const float shrink = bound[n] > 0.0f ? __builtin_amdgcn_exp2f(-up) : 0.0f;
-                    if (most > bound[n]) bound[n] = 15.0f;
-                    ref[n] += up;
-                    total[n] *= shrink;
+                for (int o = 0; o < kOut; ++o) {
+                    const f16x8 v0 = codes8<kFp8>(vc[o][0], vc[o][1]), v1 = codes8<kFp8>(vc[o][2], vc[o][3]);
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) x[i] -= up;
-#pragma unroll
-                    for (int o = 0; o < kOut; ++o) {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) acc[n][o][i] *= shrink;
+                    for (int n = 0; n < kTiles; ++n) {
+                        acc[n][o] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, w[n][0], acc[n][o], 0, 0, 0);
+                        acc[n][o] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, w[n][1], acc[n][o], 0, 0, 0);
                     }
                 }
-                float sum = 0.0f;
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const float e = __builtin_amdgcn_exp2f(x[i]);
-                    sum += e;
-                    w[n][i / 8][i % 8] = static_cast<_Float16>(e);
-                }
-                // A group whose tokens the row does not see adds nothing, whatever its page's scale is.
-                total[n] += sum == 0.0f ? 0.0f : sum * page.values_inv;
+                if (step + kWaves < stage_end) load_values(step + kWaves);
             }
-            if (!whole) {
-                rarely();
-                // Bytes past the request's tokens may hold anything, a NaN of the format too.
+        }
+
+        // The four waves' sums, brought to one reference; then the rows, or their part of them.
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int n = page.page >= 0 ? length - mine - 4 * i : 0;
-                    const int kept = n >= 4 ? -1 : n <= 0 ? 0 : (1 << (8 * n)) - 1;
-#pragma unroll
-                    for (int o = 0; o < kOut; ++o) vc[o][i] &= kept;
-                }
+        for (int n = 0; n < kTiles; ++n) {
+            total[n] += __shfl_xor(total[n], 16);
+            total[n] += __shfl_xor(total[n], 32);
+            const float top = bound[n] > 0.0f ? ref[n] : kNoScore;
+            if (n) __syncthreads();
+            if (g == 0) {
+                tops[wave][col] = top;
+                totals[wave][col] = total[n];
             }
+            __syncthreads();
+            float most = kNoScore;
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) most = nan_max(most, tops[w][col]);
+            const float factor = __builtin_amdgcn_exp2f(top - most);
 #pragma unroll
             for (int o = 0; o < kOut; ++o) {
-                const f16x8 v0 = codes8<kFp8>(vc[o][0], vc[o][1]), v1 = codes8<kFp8>(vc[o][2], vc[o][3]);
+                f32x4 v = acc[n][o];
 #pragma unroll
-                for (int n = 0; n < kTiles; ++n) {
-                    acc[n][o] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, w[n][0], acc[n][o], 0, 0, 0);
-                    acc[n][o] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, w[n][1], acc[n][o], 0, 0, 0);
+                for (int i = 0; i < 4; ++i) v[i] *= factor;
+                *reinterpret_cast<f32x4*>(&merged[wave][col][16 * o + 4 * g]) = v;
+            }
+            __syncthreads();
+            const int row0 = kRows * item.tile + 16 * n, count = min(16, rows - row0);
+            for (int i = thread; i < count * (kWidth / 4); i += 256) {
+                const int r = i / (kWidth / 4), d = 4 * (i - r * (kWidth / 4));
+                float best = kNoScore, sum = 0.0f;
+#pragma unroll
+                for (int w = 0; w < kWaves; ++w) best = nan_max(best, tops[w][r]);
+                f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int w = 0; w < kWaves; ++w) {
+                    v += *reinterpret_cast<const f32x4*>(&merged[w][r][d]);
+                    sum += totals[w][r] * __builtin_amdgcn_exp2f(tops[w][r] - best);
                 }
-            }
-            if (step + kWaves < stage_end) load_values(step + kWaves);
-        }
-    }
-
-    // The four waves' sums, brought to one reference; then the rows, or their part of them.
-#pragma unroll
-    for (int n = 0; n < kTiles; ++n) {
-        total[n] += __shfl_xor(total[n], 16);
-        total[n] += __shfl_xor(total[n], 32);
-        const float top = bound[n] > 0.0f ? ref[n] : kNoScore;
-        if (n) __syncthreads();
-        if (g == 0) {
-            tops[wave][col] = top;
-            totals[wave][col] = total[n];
-        }
-        __syncthreads();
-        float most = kNoScore;
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w) most = nan_max(most, tops[w][col]);
-        const float factor = __builtin_amdgcn_exp2f(top - most);
-#pragma unroll
-        for (int o = 0; o < kOut; ++o) {
-            f32x4 v = acc[n][o];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] *= factor;
-            *reinterpret_cast<f32x4*>(&merged[wave][col][16 * o + 4 * g]) = v;
-        }
-        __syncthreads();
-        const int row0 = kRows * share.tile + 16 * n, count = min(16, rows - row0);
-        for (int i = thread; i < count * (kWidth / 4); i += 256) {
-            const int r = i / (kWidth / 4), d = 4 * (i - r * (kWidth / 4));
-            float best = kNoScore, sum = 0.0f;
-#pragma unroll
-            for (int w = 0; w < kWaves; ++w) best = nan_max(best, tops[w][r]);
-            f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int w = 0; w < kWaves; ++w) {
-                v += *reinterpret_cast<const f32x4*>(&merged[w][r][d]);
-                sum += totals[w][r] * __builtin_amdgcn_exp2f(tops[w][r] - best);
-            }
-            if (share.splits == 1) {
-                const int t = (row0 + r) / p.group, h = kv * p.group + (row0 + r) - t * p.group;
-                store_row(p, first + t, h, kWidth, d, v, sum);
-            } else {
-                float* to = part.work + ((static_cast<int64_t>(share.place + share.split) * p.heads + kv) * kRows + 16 * n + r) * (kWidth + 4);
-                *reinterpret_cast<f32x4*>(to + d) = v;
-                if (d == 0) {
-                    to[kWidth] = best;
-                    to[kWidth + 1] = sum;
+                if (!split) {
+                    const int t = (row0 + r) / p.group, h = kv * p.group + (row0 + r) - t * p.group;
+                    store_row(p, first + t, h, kWidth, d, v, sum);
+                } else {
+                    float* to = part.work + ((static_cast<int64_t>(place) * p.heads + kv) * kRows + 16 * n + r) * (kWidth + 4);
+                    *reinterpret_cast<f32x4*>(to + d) = v;
+                    if (d == 0) {
+                        to[kWidth] = best;
+                        to[kWidth + 1] = sum;
+                    }
                 }
             }
         }
+        if (at < run_to) __syncthreads();
     }
 }
 
@@ -533,7 +645,7 @@ __global__ __launch_bounds__(64 * kWaves, kWidth == 256 ? 1 : 2) void many_kerne
     const Span span = span_of(p, row0, min(rows, row0 + kRows), fresh, length, share.split, share.splits);
     // The wave's own rows; one without rows only helps to load.
     const bool busy = mine0 < rows;
-    const Span own = span_of(p, busy ? mine0 : 0, min(rows, mine0 + 32), fresh, length, 0, 1);
+    const Span own = span_of(p, busy ? mine0 : 0, min(rows, mine0 + 32), fresh, length);
     const bool live = row < rows;
     const int token = live ? row / p.group : 0, head = kv * p.group + (live ? row - token * p.group : 0);
     const int position = length - fresh + token;
@@ -780,77 +892,89 @@ __global__ __launch_bounds__(64 * kWaves, kWidth == 256 ? 1 : 2) void many_kerne
 
 // ------------------------------------------------------------------------------------- join
 
-// A row's parts from slice `slice` on, every `slices`-th, brought to `best` and added up: four elements.
-template <int kWidth>
-__device__ __forceinline__ void add_parts(const float* at, int64_t next, int splits, int slice, int slices, int quad,
-                                          float best, f32x4& v, float& sum) {
+// Where a row's parts stand: the first, and the others `next` apart.
+struct Parts {
+    const float *first, *others;
+    int64_t next;
+    int count;
+    __device__ const float* operator[](int s) const { return s == 0 ? first : others + s * next; }
+};
+
+// A row's parts from `slice` on, every `slices`-th, brought to `best` and added up: four elements.
+__device__ __forceinline__ void add_parts(const Parts& parts, int slice, int slices, int width, int quad, float best, f32x4& v, float& sum) {
     v = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     sum = 0.0f;
 #pragma unroll 8
-    for (int s = slice; s < splits; s += slices) {
-        const float* one = at + s * next;
+    for (int s = slice; s < parts.count; s += slices) {
+        const float* one = parts[s];
         const f32x4 x = *reinterpret_cast<const f32x4*>(one + 4 * quad);
-        const float factor = __builtin_amdgcn_exp2f(one[kWidth] - best);
+        const float factor = __builtin_amdgcn_exp2f(one[width] - best);
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[j] = __builtin_fmaf(x[j], factor, v[j]);
-        sum = __builtin_fmaf(one[kWidth + 1], factor, sum);
+        sum = __builtin_fmaf(one[width + 1], factor, sum);
     }
 }
 
 // Joins the parts of the row tiles that several workgroups took, all of a row's parts brought to their
 // largest reference; blockIdx.y says of which launch. few_kernel's rows are few and their parts many: a
-// workgroup a row, kWidth/4 threads a part. many_kernel's rows are many and their parts few: a wave takes
-// kJoinRows rows, one after another. Which thread sums which parts is fixed: a call's result does not vary.
-constexpr int kJoinRows = 4;
-
+// workgroup a row, kWidth/4 threads a part. many_kernel's rows are many and their parts few: kWidth/4
+// threads a row, its parts one after another. Which thread sums which parts is fixed: a call's result does
+// not vary.
 template <int kWidth>
 __global__ __launch_bounds__(256) void join_kernel(CacheAttend p, Part few, Part many, int few_rows, int few_items, int many_items) {
-    constexpr int kQuads = kWidth / 4, kParts = 256 / kQuads, kSlices = 64 / kQuads;
+    constexpr int kQuads = kWidth / 4, kParts = 256 / kQuads;
     __shared__ f32x4 sums[kParts][kQuads];
     __shared__ float totals[kParts];
-    const int thread = threadIdx.x, lane = thread & 63;
+    const int thread = threadIdx.x, slice = thread / kQuads, quad = thread % kQuads;
     const bool wide = blockIdx.y != 0;
     const Part part = wide ? many : few;
-    const int rows_all = 1 << part.shift, groups = wide ? rows_all / kJoinRows : few_rows;
-    const int items = wide ? many_items : few_items, each = wide ? 4 : 1;
-    const int64_t next = static_cast<int64_t>(p.heads) * rows_all * (kWidth + 4);
-    for (int item = blockIdx.x * each + (wide ? thread >> 6 : 0); item < items; item += gridDim.x * each) {
-        const int kv = item % p.heads, group = item / p.heads % groups;
-        Share share;
-        if (!find_share<false>(p, part, item / (p.heads * groups), share)) return;
-        if (share.splits == 1) continue;
-        const int first = row_start(p, share.request), rows = (row_start(p, share.request + 1) - first) * p.group;
-        const int row0 = share.tile << part.shift, count = min(rows_all, rows - row0);
-        const float* tile = part.work + (static_cast<int64_t>(share.place) * p.heads + kv) * rows_all * (kWidth + 4);
-        const int from = wide ? group * kJoinRows : group, to = wide ? min(count, from + kJoinRows) : count;
-        for (int r = from; r < to; r += wide ? 1 : groups) {
-            const float* at = tile + static_cast<int64_t>(r) * (kWidth + 4);
+    const int rows_all = 1 << part.shift, groups = wide ? rows_all / kParts : few_rows;
+    const int items = wide ? many_items : few_items;
+    const int64_t row_floats = kWidth + 4, place_floats = static_cast<int64_t>(p.heads) * rows_all * row_floats;
+    Survey sv;
+    if (!wide) {
+        sv = survey(p, part);
+        if (sv.total <= sv.c) return;  // one run takes it all
+    }
+    for (int number = blockIdx.x; number < items; number += gridDim.x) {
+        const int kv = number % p.heads, group = number / p.heads % groups, id = number / (p.heads * groups);
+        int request, tile;
+        Parts parts;
+        if (wide) {
+            Share share;
+            if (!find_share<false>(p, part, id, share)) return;
+            request = share.request;
+            tile = share.tile;
+            parts = {part.work + share.place * place_floats, part.work + share.place * place_floats, place_floats, share.splits};
+        } else {
+            Item item;
+            if (!find_item<false>(p, part, sv, id, item)) return;
+            request = item.request;
+            tile = item.tile;
+            const int run = item.start / sv.c, last = (item.start + item.units - 1) / sv.c;
+            parts = {part.work + (2 * run + (item.start != run * sv.c)) * place_floats, part.work + 2 * run * place_floats,
+                     2 * place_floats, last - run + 1};
+        }
+        if (parts.count == 1) continue;
+        const int first = row_start(p, request), rows = (row_start(p, request + 1) - first) * p.group;
+        const int row0 = tile << part.shift, count = min(rows_all, rows - row0);
+        for (int r = wide ? group * kParts + slice : group; r < count; r += wide ? rows_all : groups) {
+            const int64_t at = (static_cast<int64_t>(kv) * rows_all + r) * row_floats;
+            const Parts row = {parts.first + at, parts.others + at, parts.next, parts.count};
             float best = kNoScore, sum;
-            for (int s = lane; s < share.splits; s += 64) best = nan_max(best, at[s * next + kWidth]);
-            best = wave_max_nan(best);
             f32x4 v;
-            bool mine;
-            int quad;
             if (wide) {
-                quad = lane % kQuads;
-                add_parts<kWidth>(at, next, share.splits, lane / kQuads, kSlices, quad, best, v, sum);
-#pragma unroll
-                for (int step = kQuads; step < 64; step *= 2) {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) v[j] += __shfl_xor(v[j], step);
-                    sum += __shfl_xor(sum, step);
-                }
-                mine = lane < kQuads;
+                for (int s = 0; s < row.count; ++s) best = nan_max(best, row[s][kWidth]);
+                add_parts(row, 0, 1, kWidth, quad, best, v, sum);
             } else {
-                quad = thread % kQuads;
-                const int slice = thread / kQuads;
-                add_parts<kWidth>(at, next, share.splits, slice, kParts, quad, best, v, sum);
+                for (int s = thread & 63; s < row.count; s += 64) best = nan_max(best, row[s][kWidth]);
+                best = wave_max_nan(best);
+                add_parts(row, slice, kParts, kWidth, quad, best, v, sum);
                 __syncthreads();
                 sums[slice][quad] = v;
                 if (quad == 0) totals[slice] = sum;
                 __syncthreads();
-                mine = thread < kQuads;
-                if (mine) {
+                if (slice == 0) {
 #pragma unroll
                     for (int s = 1; s < kParts; ++s) {
                         v += sums[s][quad];
@@ -858,7 +982,7 @@ __global__ __launch_bounds__(256) void join_kernel(CacheAttend p, Part few, Part
                     }
                 }
             }
-            if (mine) {
+            if (wide || slice == 0) {
                 const int t = (row0 + r) / p.group, h = kv * p.group + (row0 + r) - t * p.group;
                 store_row(p, first + t, h, kWidth, 4 * quad, v, sum);
             }
@@ -871,7 +995,7 @@ __global__ __launch_bounds__(256) void join_kernel(CacheAttend p, Part few, Part
 // One of a call's launches: its row tiles' rows, their number at the most, and where its places begin.
 struct Launch {
     bool on;
-    int rows, over, upto, shares, row_groups;
+    int rows, over, upto, shares, least, row_groups;
     int64_t tiles, offset;
 };
 
@@ -885,6 +1009,10 @@ struct AttendShape {
     int64_t floats;
 };
 
+constexpr int kFewShares = 512;   // few_kernel's workgroups over all heads: two a CU
+constexpr int kFewSteps = 8;      // of which each takes so many steps at the least,
+constexpr int kWholeSteps = 16;   // but a whole tile where none can have more than these: no join then
+constexpr int kManySteps = 16;    // many_kernel's, whose parts are larger
 constexpr int kFewRows = 64;      // up to here a request's rows are taken by few_kernel alone
 constexpr int kBesideRows = 16;   // and up to here beside requests of more
 
@@ -898,15 +1026,24 @@ AttendShape shape_of(int64_t tokens, int group, int requests, int heads, int col
     a.many.on = rows > kFewRows;
     a.few.rows = rows > 16 && !a.many.on ? 32 : 16;
     a.few.upto = a.many.on ? kBesideRows : all;
-    a.few.shares = max(1, 2 * 512 / heads);
-    a.few.tiles = a.many.on ? requests : (tokens * group + a.few.rows - 1) / a.few.rows + requests;
+    const int64_t steps = (static_cast<int64_t>(columns) * page + kStep - 1) / kStep;  // of a tile, at the most
+    a.few.tiles = a.many.on ? requests : (tokens * group + a.few.rows - 1) / a.few.rows + requests - 1;
+    if (steps <= kWholeSteps) {
+        a.few.least = kWholeSteps;
+        a.few.shares = static_cast<int>(a.few.tiles);
+    } else {  // no more workgroups than the runs that there can be
+        const int64_t runs = min(a.few.tiles, requests * ((rows + a.few.rows - 1) / a.few.rows)) * ((steps + kFewSteps - 1) / kFewSteps);
+        a.few.least = kFewSteps;
+        a.few.shares = static_cast<int>(min(runs, static_cast<int64_t>(max(1, kFewShares / heads))));
+    }
     a.few.row_groups = static_cast<int>(rows < a.few.rows ? rows : a.few.rows);
     a.many.rows = 32 * many_waves(width);
     a.many.over = a.few.on ? kBesideRows : 0;
     a.many.upto = all;
+    a.many.least = kManySteps;
     a.many.shares = max(1, (width == 64 ? 512 : 256) / heads);
-    a.many.tiles = (tokens * group + a.many.rows - 1) / a.many.rows + requests;
-    a.splits = static_cast<int64_t>(columns) * page > kMinSteps * kStep;
+    a.many.tiles = (tokens * group + a.many.rows - 1) / a.many.rows + requests - 1;
+    a.splits = steps > kWholeSteps;
     if (a.splits) {
         if (a.few.on) a.floats += 2ll * a.few.shares * heads * a.few.rows * (width + 4);
         a.many.offset = a.floats;
@@ -917,7 +1054,7 @@ AttendShape shape_of(int64_t tokens, int group, int requests, int heads, int col
 
 int log2_of(int n) { return n > 1 ? 1 + log2_of(n / 2) : 0; }
 
-Part part_of(const CacheAttend& p, const Launch& l) { return {l.over, l.upto, l.shares, log2_of(l.rows), p.work + l.offset}; }
+Part part_of(const CacheAttend& p, const Launch& l) { return {l.over, l.upto, l.shares, l.least, log2_of(l.rows), p.work + l.offset}; }
 
 template <int kWidth, bool kFp8>
 hipError_t attend(const CacheAttend& p, const AttendShape& a, hipStream_t s) {
@@ -928,17 +1065,17 @@ hipError_t attend(const CacheAttend& p, const AttendShape& a, hipStream_t s) {
         many_kernel<kWidth, kWaves, kFp8><<<groups, 64 * kWaves, 0, s>>>(p, many, true);
     }
     if (a.few.on) {
-        const unsigned groups = static_cast<unsigned>((a.few.shares + a.few.tiles + 1) * p.heads);
+        const unsigned groups = static_cast<unsigned>((a.few.shares + 1) * p.heads);
         if (a.few.rows == 16) few_kernel<kWidth, 1, kFp8><<<groups, 256, 0, s>>>(p, few, !a.many.on);
         else few_kernel<kWidth, 2, kFp8><<<groups, 256, 0, s>>>(p, few, !a.many.on);
     }
     if (a.splits) {
         const int64_t most = 0x7fffffff;
         const int64_t few_items = a.few.on ? min(most, a.few.tiles * p.heads * a.few.row_groups) : 0;
-        const int64_t many_items = a.many.on ? min(most, a.many.tiles * p.heads * (a.many.rows / kJoinRows)) : 0;
-        const int64_t groups = max(few_items, (many_items + 3) / 4);
-        join_kernel<kWidth><<<dim3(static_cast<unsigned>(min(groups, static_cast<int64_t>(2048))), a.many.on ? 2 : 1), 256, 0, s>>>(
-            p, few, many, a.few.row_groups, static_cast<int>(few_items), static_cast<int>(many_items));
+        const int64_t many_items = a.many.on ? min(most, a.many.tiles * p.heads * (a.many.rows * kWidth / 1024)) : 0;
+        const unsigned groups = static_cast<unsigned>(min(max(few_items, many_items), static_cast<int64_t>(4096)));
+        join_kernel<kWidth><<<dim3(groups, a.many.on ? 2 : 1), 256, 0, s>>>(p, few, many, a.few.row_groups, static_cast<int>(few_items),
+                                                                           static_cast<int>(many_items));
     }
     return hipGetLastError();
 }
