@@ -364,7 +364,7 @@ __global__ __launch_bounds__(256, kWidth == 256 ? 1 : 2) void few_kernel(CacheAt
         const bool split = item.start < run_from || item.start + item.units > run_to;
         const int place = 2 * id + (at != run_from);
 
-        // Tokens [low, high) of each of the lane's rows, of which the segment's steps span [begin, end).
+        // Tokens [low, high) of each of the lane's rows, none of a row that is not there.
         int low[kTiles], high[kTiles], token[kTiles], head[kTiles];
         i32x4 raw[kTiles][kBlocks][2];
 #pragma unroll
@@ -374,8 +374,8 @@ __global__ __launch_bounds__(256, kWidth == 256 ? 1 : 2) void few_kernel(CacheAt
             token[n] = live ? row / p.group : 0;
             head[n] = kv * p.group + (live ? row - token[n] * p.group : 0);
             const int position = length - fresh + token[n];
-            high[n] = live ? (p.causal ? position + 1 : length) : 0;
-            low[n] = live ? (p.window > 0 ? max(0, position + 1 - p.window) : 0) : 0x7fffffff;
+            high[n] = live ? max(p.causal ? position + 1 : length, 0) : 0;
+            low[n] = live && p.window > 0 ? max(0, position + 1 - p.window) : 0;
         }
         // The rows, read before the pages are looked up where there is one tile of them.
         const auto read_rows = [&]() {
@@ -501,9 +501,10 @@ __global__ __launch_bounds__(256, kWidth == 256 ? 1 : 2) void few_kernel(CacheAt
                     }
                     if (!whole) {
                         rarely();
+                        const uint32_t seen = page.page < 0 ? 0 : high[n] - low[n];
 #pragma unroll
                         for (int i = 0; i < 16; ++i) {
-                            if (page.page < 0 || mine + i < low[n] || mine + i >= high[n]) x[i] = -__builtin_inff();
+                            if (static_cast<uint32_t>(mine + i - low[n]) >= seen) x[i] = -__builtin_inff();
                         }
                     }
 #pragma unroll
@@ -629,8 +630,9 @@ template <int kWidth, int kWaves, bool kFp8>
 __global__ __launch_bounds__(64 * kWaves, kWidth == 256 ? 1 : 2) void many_kernel(CacheAttend p, Part part, bool clears) {
     constexpr int kRows = 32 * kWaves, kThreads = 64 * kWaves, kOut = kWidth / 32, kDepth = kWidth / 16;
     constexpr int kBytes = kStep * kWidth * 2, kChunks = kStep * kWidth / 16 / kThreads, kSwizzle = kWidth == 64 ? 7 : 15;
+    constexpr bool kLate = kWaves == 8;
     __shared__ PageScales entries[kEntries];
-    __shared__ __attribute__((aligned(16))) uint8_t keys[2][kBytes], values[2][kBytes];
+    __shared__ __attribute__((aligned(16))) uint8_t keys[2][kBytes], values[kLate ? 3 : 2][kBytes];
     const int thread = threadIdx.x, lane = thread & 63, wave = __builtin_amdgcn_readfirstlane(thread >> 6);
     const int col = lane & 31, h = lane >> 5;
     const int kv = blockIdx.x % p.heads, id = blockIdx.x / p.heads;
@@ -649,8 +651,8 @@ __global__ __launch_bounds__(64 * kWaves, kWidth == 256 ? 1 : 2) void many_kerne
     const bool live = row < rows;
     const int token = live ? row / p.group : 0, head = kv * p.group + (live ? row - token * p.group : 0);
     const int position = length - fresh + token;
-    const int high = live ? (p.causal ? position + 1 : length) : 0;
-    const int low = live ? (p.window > 0 ? max(0, position + 1 - p.window) : 0) : 0x7fffffff;
+    const int high = live ? max(p.causal ? position + 1 : length, 0) : 0;
+    const int low = live && p.window > 0 ? max(0, position + 1 - p.window) : 0;
 
     f16x8 q[kDepth];
     float sharp;
@@ -715,18 +717,21 @@ __global__ __launch_bounds__(64 * kWaves, kWidth == 256 ? 1 : 2) void many_kerne
             vc[i] = *reinterpret_cast<const i32x4*>(v_head + max(page, 0) * page_bytes + (c / 4) * p.page + (t & within));
         }
     };
+    // The tiles of values that the step before, this one and the next have.
+    int v_before = kLate ? 2 * kBytes : kBytes, v_now = 0, v_next = kBytes;
+    uint8_t* const values_at = &values[0][0];
     // Chunk i of a step's codes, as f16, to its places in LDS.
     const auto put_keys = [&](int step, int i) {
         *reinterpret_cast<f16x8*>(&keys[step & 1][k_to[i][0]]) = codes8<kFp8>(kc[i][0], kc[i][1]);
         *reinterpret_cast<f16x8*>(&keys[step & 1][k_to[i][1]]) = codes8<kFp8>(kc[i][2], kc[i][3]);
     };
-    const auto put_values = [&](int step, int i) {
-        *reinterpret_cast<f16x8*>(&values[step & 1][v_to[i][0]]) = codes8<kFp8>(vc[i][0], vc[i][1]);
-        *reinterpret_cast<f16x8*>(&values[step & 1][v_to[i][1]]) = codes8<kFp8>(vc[i][2], vc[i][3]);
+    const auto put_values = [&](int tile, int i) {
+        *reinterpret_cast<f16x8*>(values_at + tile + v_to[i][0]) = codes8<kFp8>(vc[i][0], vc[i][1]);
+        *reinterpret_cast<f16x8*>(values_at + tile + v_to[i][1]) = codes8<kFp8>(vc[i][2], vc[i][3]);
     };
     // Where a step's values hold tokens past the request's or of pages that the cache has not, zeros in their
     // place, over what was put there.
-    const auto cut_values = [&](int step) {
+    const auto cut_values = [&](int tile) {
 #pragma unroll
         for (int i = 0; i < kChunks; ++i) {
             if (__any(kept[i] < 16)) {
@@ -736,7 +741,7 @@ __global__ __launch_bounds__(64 * kWaves, kWidth == 256 ? 1 : 2) void many_kerne
                     const int n = kept[i] - 4 * j;
                     vc[i][j] &= n >= 4 ? -1 : n <= 0 ? 0 : (1 << (8 * n)) - 1;
                 }
-                put_values(step, i);
+                put_values(tile, i);
             }
         }
     };
@@ -745,12 +750,32 @@ __global__ __launch_bounds__(64 * kWaves, kWidth == 256 ? 1 : 2) void many_kerne
     const auto key_chunk = [&](int step, int b, int half) {
         return *reinterpret_cast<const f16x8*>(&keys[step & 1][(32 * half + col) * (2 * kWidth) + 16 * ((2 * b + h) ^ (col & kSwizzle))]);
     };
-    const auto value_chunk = [&](int step, int a, int o) {
-        return *reinterpret_cast<const f16x8*>(&values[step & 1][(32 * o + col) * (2 * kStep) + 16 * ((2 * a + h) ^ (col & 7))]);
+    const auto value_chunk = [&](int tile, int a, int o) {
+        return *reinterpret_cast<const f16x8*>(values_at + tile + ((32 * o + col) * (2 * kStep) + 16 * ((2 * a + h) ^ (col & 7))));
     };
     // The scores of a step whose keys are in LDS, as they leave the matrix unit.
     f32x16 s[2];
     constexpr int kScores = 2 * kDepth, kSums = 4 * kOut, kAhead = 4;
+
+    f16x8 w[4];
+    // A step's weights times its values, `beside` done with the last products, a chunk each.
+    const auto add_values = [&](int tile, auto beside) {
+        f16x8 ring[kAhead];
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) ring[j] = value_chunk(tile, j / kOut, j % kOut);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int j = 0; j < kSums; ++j) {
+            acc[j % kOut] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ring[j % kAhead], w[j / kOut], acc[j % kOut], 0, 0, 0);
+            if (j + kAhead < kSums) ring[j % kAhead] = value_chunk(tile, (j + kAhead) / kOut, (j + kAhead) % kOut);
+            if (j >= kSums - kChunks) beside(j - (kSums - kChunks));
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    // Half of the waves, one on each SIMD, are half a step behind: they multiply a step's values after the
+    // barrier, while the others are at the exponentials, so that the two waves of a SIMD want the matrix
+    // unit and the vector unit in turn.
+    const bool late = kLate && wave >= kWaves / 2;
 
     for (int stage = span.begin; stage < span.end; stage += kStage) {
         const int stage_end = min(span.end, stage + kStage);
@@ -763,9 +788,9 @@ __global__ __launch_bounds__(64 * kWaves, kWidth == 256 ? 1 : 2) void many_kerne
 #pragma unroll
         for (int i = 0; i < kChunks; ++i) {
             put_keys(stage, i);
-            put_values(stage, i);
+            put_values(v_now, i);
         }
-        cut_values(stage);
+        cut_values(v_now);
         if (stage + 1 < stage_end) {
             load_keys(stage + 1);
 #pragma unroll
@@ -781,6 +806,7 @@ __global__ __launch_bounds__(64 * kWaves, kWidth == 256 ? 1 : 2) void many_kerne
             if (step + 2 < stage_end) load_keys(step + 2);
             if (step + 1 < stage_end) load_values(step + 1);
             if (busy) {
+                if (late && step > stage) add_values(v_before, [](int) {});
                 const int t0 = step * kStep;
                 PageScales page[4];
 #pragma unroll
@@ -798,8 +824,8 @@ __global__ __launch_bounds__(64 * kWaves, kWidth == 256 ? 1 : 2) void many_kerne
                     rarely();
 #pragma unroll
                     for (int i = 0; i < 32; ++i) {
-                        const int t = t0 + 16 * (i / 8) + 8 * h + i % 8;
-                        if (page[i / 8].page < 0 || t < low || t >= high) s[i / 16][i % 16] = -__builtin_inff();
+                        const uint32_t seen = page[i / 8].page < 0 ? 0 : high - low;
+                        if (static_cast<uint32_t>(t0 + 16 * (i / 8) + 8 * h + i % 8 - low) >= seen) s[i / 16][i % 16] = -__builtin_inff();
                     }
                 }
 #pragma unroll
@@ -819,14 +845,12 @@ __global__ __launch_bounds__(64 * kWaves, kWidth == 256 ? 1 : 2) void many_kerne
                         for (int i = 0; i < 16; ++i) acc[o][i] *= shrink;
                     }
                 }
-                // The next step's scores on the matrix unit over this one's exponentials, then this one's sums
-                // over the next tiles' conversion. Each operand is read from LDS kAhead products before its
-                // own, and the order written here is kept. Past the stage's last step the scores are of
-                // whatever the tile holds, and not used.
-                f16x8 ring[kAhead], w[4];
+                // The next step's scores on the matrix unit over this one's exponentials. Each operand is read
+                // from LDS kAhead products before its own, and the order written here is kept. Past the stage's
+                // last step the scores are of whatever the tile holds, and not used.
+                f16x8 ring[kAhead];
                 f32x16 next[2];
                 const auto key_operand = [&](int j) { return key_chunk(step + 1, j / 2, j % 2); };
-                const auto value_operand = [&](int j) { return value_chunk(step, j / kOut, j % kOut); };
                 float sum = 0.0f;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) next[0][i] = next[1][i] = 0.0f;
@@ -836,7 +860,7 @@ __global__ __launch_bounds__(64 * kWaves, kWidth == 256 ? 1 : 2) void many_kerne
 #pragma unroll
                 for (int j = 0; j < kScores; ++j) {
                     next[j % 2] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ring[j % kAhead], q[j / 2], next[j % 2], 0, 0, 0);
-                    ring[j % kAhead] = j + kAhead < kScores ? key_operand(j + kAhead) : value_operand(j + kAhead - kScores);
+                    if (j + kAhead < kScores) ring[j % kAhead] = key_operand(j + kAhead);
 #pragma unroll
                     for (int i = 32 / kScores * j; i < 32 / kScores * (j + 1); ++i) {
                         const float x = __builtin_amdgcn_exp2f(s[i / 16][i % 16]);
@@ -847,28 +871,30 @@ __global__ __launch_bounds__(64 * kWaves, kWidth == 256 ? 1 : 2) void many_kerne
                     }
                     __builtin_amdgcn_sched_barrier(0);
                 }
-#pragma unroll
-                for (int j = 0; j < kSums; ++j) {
-                    acc[j % kOut] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ring[(kScores + j) % kAhead], w[j / kOut], acc[j % kOut], 0, 0, 0);
-                    if (j + kAhead < kSums) ring[(kScores + j) % kAhead] = value_operand(j + kAhead);
-                    if (j < kChunks) {
-                        put_keys(step + 2, j);
-                        put_values(step + 1, j);
-                    }
-                    __builtin_amdgcn_sched_barrier(0);
+                if (!late) {
+                    add_values(v_now, [&](int i) {
+                        put_keys(step + 2, i);
+                        put_values(v_next, i);
+                    });
                 }
                 s[0] = next[0];
                 s[1] = next[1];
-            } else {
+            }
+            if (!busy || late) {
 #pragma unroll
                 for (int i = 0; i < kChunks; ++i) {
                     put_keys(step + 2, i);
-                    put_values(step + 1, i);
+                    put_values(v_next, i);
                 }
             }
-            cut_values(step + 1);
+            cut_values(v_next);
             __syncthreads();
+            const int freed = kLate ? v_before : v_now;
+            v_before = v_now;
+            v_now = v_next;
+            v_next = freed;
         }
+        if (busy && late) add_values(v_before, [](int) {});
     }
 
     if (!live) return;
@@ -1073,7 +1099,7 @@ hipError_t attend(const CacheAttend& p, const AttendShape& a, hipStream_t s) {
         const int64_t most = 0x7fffffff;
         const int64_t few_items = a.few.on ? min(most, a.few.tiles * p.heads * a.few.row_groups) : 0;
         const int64_t many_items = a.many.on ? min(most, a.many.tiles * p.heads * (a.many.rows * kWidth / 1024)) : 0;
-        const unsigned groups = static_cast<unsigned>(min(max(few_items, many_items), static_cast<int64_t>(4096)));
+        const unsigned groups = static_cast<unsigned>(min(max(few_items, many_items), static_cast<int64_t>(1024)));
         join_kernel<kWidth><<<dim3(groups, a.many.on ? 2 : 1), 256, 0, s>>>(p, few, many, a.few.row_groups, static_cast<int>(few_items),
                                                                            static_cast<int>(many_items));
     }
