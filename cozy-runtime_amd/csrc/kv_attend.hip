@@ -941,6 +941,38 @@ __device__ __forceinline__ void add_parts(const Parts& parts, int slice, int sli
     }
 }
 
+// The same of all of a row's parts, four of them read at a time, their references with them.
+__device__ __forceinline__ void add_all(const Parts& parts, int width, int quad, f32x4& v, float& sum) {
+    v = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    sum = 0.0f;
+    float best = kNoScore;
+    for (int from = 0; from < parts.count; from += 4) {
+        f32x4 x[4];
+        float top[4], one[4], most = best;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float* part = parts[min(from + i, parts.count - 1)];
+            x[i] = *reinterpret_cast<const f32x4*>(part + 4 * quad);
+            top[i] = part[width];
+            one[i] = part[width + 1];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) most = nan_max(most, top[i]);
+        const float shrink = __builtin_amdgcn_exp2f(best - most);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] *= shrink;
+        sum *= shrink;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float factor = from + i < parts.count ? __builtin_amdgcn_exp2f(top[i] - most) : 0.0f;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = __builtin_fmaf(x[i][j], factor, v[j]);
+            sum = __builtin_fmaf(one[i], factor, sum);
+        }
+        best = most;
+    }
+}
+
 // Joins the parts of the row tiles that several workgroups took, all of a row's parts brought to their
 // largest reference; blockIdx.y says of which launch. few_kernel's rows are few and their parts many: a
 // workgroup a row, kWidth/4 threads a part. many_kernel's rows are many and their parts few: kWidth/4
@@ -990,8 +1022,7 @@ __global__ __launch_bounds__(256) void join_kernel(CacheAttend p, Part few, Part
             float best = kNoScore, sum;
             f32x4 v;
             if (wide) {
-                for (int s = 0; s < row.count; ++s) best = nan_max(best, row[s][kWidth]);
-                add_parts(row, 0, 1, kWidth, quad, best, v, sum);
+                add_all(row, kWidth, quad, v, sum);
             } else {
                 for (int s = thread & 63; s < row.count; s += 64) best = nan_max(best, row[s][kWidth]);
                 best = wave_max_nan(best);
