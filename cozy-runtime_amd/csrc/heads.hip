@@ -29,6 +29,7 @@ __device__ __forceinline__ void load8f(const float* p, float* v) {
 // A head is width/16 units of 16 elements, one a lane, on `lanes` lanes (a power of two). A unit of
 // the rotated part holds both elements of eight pairs, so that a rotation needs no other lane: for
 // halves the chunks u and u + rotated/16 of eight elements, otherwise the neighbours 2u and 2u + 1.
+template <bool kHalf>
 __global__ __launch_bounds__(kThreads) void norm_rope_kernel(HeadRows r) {
     const int64_t head_slot = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) / r.lanes;
     const int u = threadIdx.x & (r.lanes - 1);
@@ -53,8 +54,8 @@ __global__ __launch_bounds__(kThreads) void norm_rope_kernel(HeadRows r) {
             at_a = 8 * u;
             at_b = 8 * u + r.rotated / 2;
         }
-        load8(x + at_a, r.half, a);
-        load8(x + at_b, r.half, b);
+        load8<kHalf>(x + at_a, a);
+        load8<kHalf>(x + at_b, b);
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i) a[i] = b[i] = 0.0f;
@@ -76,8 +77,8 @@ __global__ __launch_bounds__(kThreads) void norm_rope_kernel(HeadRows r) {
                 load8f(static_cast<const float*>(gain) + at_a, ga);
                 load8f(static_cast<const float*>(gain) + at_b, gb);
             } else {
-                load8(static_cast<const uint16_t*>(gain) + at_a, r.half, ga);
-                load8(static_cast<const uint16_t*>(gain) + at_b, r.half, gb);
+                load8<kHalf>(static_cast<const uint16_t*>(gain) + at_a, ga);
+                load8<kHalf>(static_cast<const uint16_t*>(gain) + at_b, gb);
             }
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
@@ -112,8 +113,8 @@ __global__ __launch_bounds__(kThreads) void norm_rope_kernel(HeadRows r) {
             }
         }
     }
-    store8(out + at_a, r.half, a);
-    store8(out + at_b, r.half, b);
+    store8<kHalf>(out + at_a, a);
+    store8<kHalf>(out + at_b, b);
 }
 
 }  // namespace
@@ -123,7 +124,9 @@ hipError_t head_norm_rope(HeadRows rows, hipStream_t s) {
     while (rows.lanes * 16 < rows.width) rows.lanes *= 2;
     const int64_t threads = static_cast<int64_t>(rows.tokens) * (rows.q_heads + rows.k_heads) * rows.lanes;
     if (threads == 0) return hipSuccess;
-    norm_rope_kernel<<<static_cast<unsigned>((threads + kThreads - 1) / kThreads), kThreads, 0, s>>>(rows);
+    const unsigned groups = static_cast<unsigned>((threads + kThreads - 1) / kThreads);
+    if (rows.half) norm_rope_kernel<true><<<groups, kThreads, 0, s>>>(rows);
+    else norm_rope_kernel<false><<<groups, kThreads, 0, s>>>(rows);
     return hipGetLastError();
 }
 

@@ -319,7 +319,7 @@ __device__ __forceinline__ void row_unit(uint32_t most, float& unit, float& down
 
 // Eight elements of a query row as float32, and their largest magnitude's bits.
 __device__ __forceinline__ void query8(const CacheAttend& p, const uint16_t* x, float* v, uint32_t& most) {
-    load8(x, p.half, v);
+    widen8(*reinterpret_cast<const i32x4*>(x), p.half, v);
 #pragma unroll
     for (int i = 0; i < 8; ++i) most = max(most, bits_of(v[i]) & 0x7fffffffu);
 }

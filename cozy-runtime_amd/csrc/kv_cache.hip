@@ -164,32 +164,44 @@ __global__ __launch_bounds__(kThreads) void plan_kernel(CachePlan p) {
 
 // ---------------------------------------------------------------------------------- append
 
-// The codes of four values (already over the scale): int8 by rint, E4M3 by the conversion, clamped to the
-// format's largest. A NaN (only where the scale is not finite) becomes code 0: codes are always finite.
+// The codes of four values already over the scale, so within the format's largest but for a rounding that
+// the code's own takes back: int8 by adding 1.5·2^23, whose sum's low byte is the value rounded to nearest
+// even, E4M3 by the conversion.
 template <bool kFp8>
 __device__ __forceinline__ uint32_t codes_of(const float* x) {
-    constexpr float kMost = kFp8 ? kE4m3Max : 127.0f;
-    float v[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = x[i] != x[i] ? 0.0f : fminf(fmaxf(x[i], -kMost), kMost);
     if constexpr (kFp8) {
-        return e4m3x4(v[0], v[1], v[2], v[3]);
+        return e4m3x4(x[0], x[1], x[2], x[3]);
     } else {
-        uint32_t c = 0;
+        uint32_t c[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) c |= (static_cast<uint32_t>(static_cast<int>(__builtin_rintf(v[i]))) & 0xffu) << (8 * i);
-        return c;
+        for (int i = 0; i < 4; ++i) c[i] = bits_of(x[i] + 12582912.0f);
+        const uint32_t lo = __builtin_amdgcn_perm(c[1], c[0], 0x0c0c0400u), hi = __builtin_amdgcn_perm(c[3], c[2], 0x04000c0cu);
+        return lo | hi;
     }
 }
 
-// A dword of codes at a new scale: code · ratio, rounded again.
+// A dword of codes at a new scale: code · ratio, rounded again; 0 where the scale is not finite.
 template <bool kFp8>
 __device__ __forceinline__ uint32_t rescaled(uint32_t c, float ratio) {
     float v[4];
     codes4f<kFp8>(c, v);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] *= ratio;
+    for (int i = 0; i < 4; ++i) v[i] = v[i] * ratio == v[i] * ratio ? v[i] * ratio : 0.0f;
     return codes_of<kFp8>(v);
+}
+
+// x / s rounded to nearest even for s > 0, given r = RN(1/s), as div_rn but for the sign of a zero, which
+// no code keeps apart.
+__device__ __forceinline__ float over_scale(float x, float s, float r) {
+    const float q = x * r;
+    return __builtin_fmaf(__builtin_fmaf(-q, s, x), r, q);
+}
+
+// The larger magnitude of each half's 16-bit numbers, as their bits without the sign.
+__device__ __forceinline__ uint32_t magnitudes(uint32_t most, uint32_t two) {
+    typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, most),
+                                                                  __builtin_bit_cast(u16x2, two & 0x7fff7fffu)));
 }
 
 // Bytes [from, to) of the dword whose first byte is number `at`.
@@ -208,123 +220,165 @@ constexpr int kFewTokens = 4;
 // begun before. Where it grows, the codes that the page holds are rounded again at the new scale
 // (code · old/new); a page that the run begins is cleared past its tokens. Magnitudes compare as their bits
 // do, and an infinity or NaN is above every number: what is not finite goes into the page's scale.
-// Elements are read eight at a time, twice (the second time out of L1 or L2). New values are transposed in
-// LDS, four tokens of a channel a dword, rows of page/4 + 1 dwords; both kinds leave 16 bytes a thread.
-template <bool kFp8>
-__global__ __launch_bounds__(kThreads) void append_kernel(CacheAppend p, int width_shift, int page_shift) {
-    extern __shared__ uint32_t turned[];
-    __shared__ uint32_t wave_most[kWaves];
-    const i32x4 run = *reinterpret_cast<const i32x4*>(p.runs + 4 * static_cast<int64_t>(blockIdx.x));
+// A thread reads eight elements at a time, kHeld times before it looks at any: a page of up to 16384 elements
+// is in the workgroup's registers after one trip to memory and is coded from there; a larger one is read
+// twice. New values are turned in LDS, four tokens of a channel a dword, rows of page/4 + 1 dwords.
+template <bool kFp8, bool kHalf, bool kValues>
+__device__ void append(const CacheAppend& p, int width_shift, int page_shift, const i32x4& run, uint32_t* turned, uint32_t* wave_most) {
+    constexpr int kHeld = 8;
     const int row = run[0], count = run[1], page = run[2], offset = run[3];
-    if (count <= 0 || page < 0 || page >= p.pages || row < 0 || row + count > p.tokens || offset < 0 ||
-        offset + count > p.page)
-        return;
-    const int head = blockIdx.y, end = offset + count, eights = width_shift - 3;
-    const bool values = blockIdx.z != 0;
-    const uint16_t* x = values ? p.v + row * p.v_token + head * p.v_head : p.k + row * p.k_token + head * p.k_head;
-    const int64_t token_step = values ? p.v_token : p.k_token;
+    const int head = blockIdx.y, end = offset + count, eights = width_shift - 3, thread = threadIdx.x;
+    const uint16_t* x = kValues ? p.v + row * p.v_token + head * p.v_head : p.k + row * p.k_token + head * p.k_head;
+    const int64_t token_step = kValues ? p.v_token : p.k_token;
     const int64_t tile = static_cast<int64_t>(page) * p.heads + head;
-    uint8_t* codes = (values ? p.v_codes : p.k_codes) + tile * p.page * p.width;
-    float* scale_at = (values ? p.v_scale : p.k_scale) + tile;
+    uint8_t* codes = (kValues ? p.v_codes : p.k_codes) + tile * p.page * p.width;
+    float* scale_at = (kValues ? p.v_scale : p.k_scale) + tile;
     const float before = offset > 0 ? *scale_at : 0.0f;
 
-    uint32_t most = 0;
-    for (int i = threadIdx.x; i < count << eights; i += kThreads) {
-        float v[8];
-        load8(x + (i >> eights) * token_step + 8 * (i & ((1 << eights) - 1)), p.half, v);
+    // A round is kHeld chunks of eight channels of a token a thread. The tokens of keys' chunks follow one
+    // another; of values', four tokens from a multiple of four on are four chunks of one thread.
+    const int t_first = kValues ? offset & ~3 : offset, d = 8 * (thread & ((1 << eights) - 1));
+    const int each = kValues ? 4 : 1;  // tokens of a thread's chunks that stand together
+    const int units = ((end - t_first + each - 1) / each) << eights, round_units = kHeld / each * kThreads;
+    const int rounds = (units + round_units - 1) / round_units;
+    const auto unit_of = [&](int round, int j) { return round * round_units + j / each * kThreads; };  // of thread 0
+    const auto token_of = [&](int round, int j) { return t_first + each * ((unit_of(round, j) + thread) >> eights) + j % each; };
+    i32x4 held[kHeld];
+    const auto load = [&](int round) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) most = max(most, bits_of(v[j]) & 0x7fffffffu);
+        for (int j = 0; j < kHeld; ++j) {
+            held[j] = i32x4{0, 0, 0, 0};
+            const int t = token_of(round, j);
+            if (unit_of(round, j) < units && t >= offset && t < end)
+                held[j] = *reinterpret_cast<const i32x4*>(x + (t - offset) * token_step + d);
+        }
+    };
+    uint32_t pair = 0;
+    for (int round = 0; round < rounds; ++round) {
+        load(round);
+#pragma unroll
+        for (int j = 0; j < kHeld; ++j) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) pair = magnitudes(pair, static_cast<uint32_t>(held[j][i]));
+        }
     }
-    for (int step = 1; step < 64; step *= 2) most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), step)));
-    if ((threadIdx.x & 63) == 0) wave_most[threadIdx.x >> 6] = most;
+    uint32_t largest = max(pair & 0xffffu, pair >> 16);
+    for (int step = 1; step < 64; step *= 2) largest = max(largest, static_cast<uint32_t>(__shfl_xor(static_cast<int>(largest), step)));
+    if ((thread & 63) == 0) wave_most[thread >> 6] = largest;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) most = max(most, wave_most[w]);
-    const float reach = nan_max(float_of(most) / (kFp8 ? kE4m3Max : 127.0f), kScaleFloor);
+    for (int w = 0; w < kWaves; ++w) largest = max(largest, wave_most[w]);
+    const float reach = nan_max(widen<kHalf>(static_cast<uint16_t>(largest)) / (kFp8 ? kE4m3Max : 127.0f), kScaleFloor);
     const float scale = nan_max(before, reach);
+    const bool finite = scale - scale == 0.0f;
     const float inv = 1.0f / scale;
     const float ratio = before / scale;
     const bool keep = offset > 0 && bits_of(scale) == bits_of(before);
-    if (threadIdx.x == 0 && !keep) *scale_at = scale;
+    if (thread == 0 && !keep) *scale_at = scale;
+    // Chunk j over the scale: eight values, zeros where that is not finite.
+    const auto over = [&](int j, float* v) {
+        widen8<kHalf>(held[j], v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = over_scale(v[i], scale, inv);
+        if (!finite) {
+            asm volatile("");
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+        }
+    };
 
-    if (!values) {
-        // A thread: 16 channels of a token; where the scale stands, of the new tokens alone.
-        const int sixteens = width_shift - 4, first = keep ? offset : 0, last = keep ? end : p.page;
-        for (int i = threadIdx.x; i < (last - first) << sixteens; i += kThreads) {
-            const int t = first + (i >> sixteens), d = 16 * (i & ((1 << sixteens) - 1));
-            i32x4* at = reinterpret_cast<i32x4*>(codes + (static_cast<int64_t>(t) << width_shift) + d);
+    if constexpr (!kValues) {
+        for (int round = 0; round < rounds; ++round) {
+            if (rounds > 1) load(round);
+#pragma unroll
+            for (int j = 0; j < kHeld; ++j) {
+                if (unit_of(round, j) >= units) break;
+                const int t = token_of(round, j);
+                if (t < end) {
+                    float v[8];
+                    over(j, v);
+                    const i32x2 got = {static_cast<int32_t>(codes_of<kFp8>(v)), static_cast<int32_t>(codes_of<kFp8>(v + 4))};
+                    *reinterpret_cast<i32x2*>(codes + (t << width_shift) + d) = got;
+                }
+            }
+        }
+        if (keep) return;
+        // The page's other tokens, 16 channels a thread: rounded again, or cleared.
+        const int sixteens = width_shift - 4;
+        for (int i = thread; i < (p.page - count) << sixteens; i += kThreads) {
+            const int other = i >> sixteens, t = other < offset ? other : other + count;
+            i32x4* at = reinterpret_cast<i32x4*>(codes + (t << width_shift) + 16 * (i & ((1 << sixteens) - 1)));
             i32x4 got = {0, 0, 0, 0};
-            if (t >= offset && t < end) {
-                float v[16];
-                load8(x + (t - offset) * token_step + d, p.half, v);
-                load8(x + (t - offset) * token_step + d + 8, p.half, v + 8);
-#pragma unroll
-                for (int j = 0; j < 16; ++j) v[j] = div_rn(v[j], scale, inv);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) got[j] = static_cast<int32_t>(codes_of<kFp8>(v + 4 * j));
-            } else if (offset > 0) {
+            if (offset > 0) {
                 got = *at;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) got[j] = static_cast<int32_t>(rescaled<kFp8>(static_cast<uint32_t>(got[j]), ratio));
             }
             *at = got;
         }
-        return;
-    }
-    if (keep && count <= kFewTokens) {
-        for (int i = threadIdx.x; i < count << eights; i += kThreads) {
-            const int t = i >> eights, d = 8 * (i & ((1 << eights) - 1));
-            float v[8];
-            load8(x + t * token_step + d, p.half, v);
+    } else {
+        const bool bytes = keep && count <= kFewTokens;
+        const int pitch = (p.page >> 2) + 1;
+        for (int round = 0; round < rounds; ++round) {
+            if (rounds > 1) load(round);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = div_rn(v[j], scale, inv);
-            const uint32_t c[2] = {codes_of<kFp8>(v), codes_of<kFp8>(v + 4)};
+            for (int q = 0; q < kHeld; q += 4) {
+                if (unit_of(round, q) >= units) break;
+                const int t = token_of(round, q);
+                if (t >= end) continue;
+                uint32_t c[8];
+                float v[4][8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) codes[((d + j) << page_shift) + offset + t] = static_cast<uint8_t>(c[j / 4] >> (8 * (j & 3)));
-        }
-        return;
-    }
-    // A thread: four tokens of the page, eight channels.
-    const int pitch = (p.page >> 2) + 1, t_first = offset & ~3;
-    const int fours = (end - t_first + 3) >> 2;
-    for (int i = threadIdx.x; i < fours << eights; i += kThreads) {
-        const int t = t_first + 4 * (i >> eights), d = 8 * (i & ((1 << eights) - 1));
-        float v[4][8];
+                for (int j = 0; j < 4; ++j) over(q + j, v[j]);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if (t + j >= offset && t + j < end) {
-                load8(x + (t + j - offset) * token_step + d, p.half, v[j]);
-            } else {
+                for (int i = 0; i < 8; ++i) {
+                    const float four[4] = {v[0][i], v[1][i], v[2][i], v[3][i]};
+                    c[i] = codes_of<kFp8>(four);
+                }
+                if (!bytes) {
 #pragma unroll
-                for (int k = 0; k < 8; ++k) v[j][k] = 0.0f;
+                    for (int i = 0; i < 8; ++i) turned[(d + i) * pitch + (t >> 2)] = c[i];
+                } else {
+                    for (int j = max(offset - t, 0); j < min(end - t, 4); ++j) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) codes[((d + i) << page_shift) + t + j] = static_cast<uint8_t>(c[i] >> (8 * j));
+                    }
+                }
             }
         }
+        if (bytes) return;
+        __syncthreads();
+        // A thread: 16 tokens of a channel; where the scale stands, of those with new tokens alone.
+        const int first = keep ? offset >> 4 : 0, last = keep ? (end + 15) >> 4 : p.page >> 4;
+        const int wide = last - first;
+        for (int i = thread; i < wide << width_shift; i += kThreads) {
+            const int channel = i / wide, t = 16 * (first + i - channel * wide);
+            i32x4* at = reinterpret_cast<i32x4*>(codes + (channel << page_shift) + t);
+            i32x4 got = {0, 0, 0, 0};
+            if (offset > 0 && (t < offset || t + 16 > end)) got = *at;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            const float four[4] = {div_rn(v[0][k], scale, inv), div_rn(v[1][k], scale, inv), div_rn(v[2][k], scale, inv),
-                                   div_rn(v[3][k], scale, inv)};
-            turned[(d + k) * pitch + (t >> 2)] = codes_of<kFp8>(four);
+            for (int j = 0; j < 4; ++j) {
+                uint32_t kept = static_cast<uint32_t>(got[j]);
+                if (!keep && offset > 0) kept = rescaled<kFp8>(kept, ratio);
+                const uint32_t mine = byte_mask(t + 4 * j, offset, end);
+                if (mine) kept = (kept & ~mine) | (turned[channel * pitch + (t >> 2) + j] & mine);
+                got[j] = static_cast<int32_t>(kept);
+            }
+            *at = got;
         }
     }
-    __syncthreads();
-    // A thread: 16 tokens of a channel; where the scale stands, of those with new tokens alone.
-    const int first = keep ? offset >> 4 : 0, last = keep ? (end + 15) >> 4 : p.page >> 4;
-    const int chunks = last - first;
-    for (int i = threadIdx.x; i < chunks << width_shift; i += kThreads) {
-        const int d = i / chunks, t = 16 * (first + i - d * chunks);
-        i32x4* at = reinterpret_cast<i32x4*>(codes + (static_cast<int64_t>(d) << page_shift) + t);
-        i32x4 got = {0, 0, 0, 0};
-        if (offset > 0 && (t < offset || t + 16 > end)) got = *at;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            uint32_t c = static_cast<uint32_t>(got[j]);
-            if (!keep && offset > 0) c = rescaled<kFp8>(c, ratio);
-            const uint32_t mine = byte_mask(t + 4 * j, offset, end);
-            if (mine) c = (c & ~mine) | (turned[d * pitch + (t >> 2) + j] & mine);
-            got[j] = static_cast<int32_t>(c);
-        }
-        *at = got;
-    }
+}
+
+template <bool kFp8, bool kHalf>
+__global__ __launch_bounds__(kThreads) void append_kernel(CacheAppend p, int width_shift, int page_shift) {
+    extern __shared__ uint32_t turned[];
+    __shared__ uint32_t wave_most[kWaves];
+    const i32x4 run = *reinterpret_cast<const i32x4*>(p.runs + 4 * static_cast<int64_t>(blockIdx.x));
+    if (run[1] <= 0 || run[2] < 0 || run[2] >= p.pages || run[0] < 0 || run[0] + run[1] > p.tokens || run[3] < 0 ||
+        run[3] + run[1] > p.page)
+        return;
+    if (blockIdx.z) append<kFp8, kHalf, true>(p, width_shift, page_shift, run, turned, wave_most);
+    else append<kFp8, kHalf, false>(p, width_shift, page_shift, run, turned, wave_most);
 }
 
 // ------------------------------------------------------------------------------------ read
@@ -332,7 +386,7 @@ __global__ __launch_bounds__(kThreads) void append_kernel(CacheAppend p, int wid
 // One workgroup a (listed page, head): its keys and values as 16-bit numbers, tokens by width. A thread
 // takes 16 channels of a token's keys, and 16 tokens of four channels' values, which it turns in registers:
 // a wave's stores of a token's values are of neighbouring channels.
-template <bool kFp8>
+template <bool kFp8, bool kHalf>
 __global__ __launch_bounds__(kThreads) void read_kernel(CacheRead p, int width_shift, int page_shift) {
     const int page = p.numbers[blockIdx.x], head = blockIdx.y;
     const int64_t to = (static_cast<int64_t>(blockIdx.x) * p.heads + head) * p.page * p.width;
@@ -348,15 +402,23 @@ __global__ __launch_bounds__(kThreads) void read_kernel(CacheRead p, int width_s
     const int64_t tile = static_cast<int64_t>(page) * p.heads + head;
     const float ks = p.k_scale[tile], vs = p.v_scale[tile];
     const uint8_t *k = p.k_codes + tile * elements, *v = p.v_codes + tile * elements;
-    for (int i = threadIdx.x; i < elements / 16; i += kThreads) {
-        const i32x4 c = reinterpret_cast<const i32x4*>(k)[i];
-        float x[16];
+    constexpr int kHeld = 4;  // read before any of them is written
+    for (int from = threadIdx.x; from < elements / 16; from += kHeld * kThreads) {
+        i32x4 c[kHeld];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) codes4f<kFp8>(static_cast<uint32_t>(c[j]), x + 4 * j);
+        for (int h = 0; h < kHeld; ++h) c[h] = reinterpret_cast<const i32x4*>(k)[min(from + h * kThreads, elements / 16 - 1)];
 #pragma unroll
-        for (int j = 0; j < 16; ++j) x[j] *= ks;
-        store8(k_out + 16 * i, p.half, x);
-        store8(k_out + 16 * i + 8, p.half, x + 8);
+        for (int h = 0; h < kHeld; ++h) {
+            const int i = from + h * kThreads;
+            if (i >= elements / 16) break;
+            float x[16];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) codes4f<kFp8>(static_cast<uint32_t>(c[h][j]), x + 4 * j);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) x[j] *= ks;
+            store8<kHalf>(k_out + 16 * i, x);
+            store8<kHalf>(k_out + 16 * i + 8, x + 8);
+        }
     }
     const int fours = width_shift - 2;
     for (int i = threadIdx.x; i < elements / 64; i += kThreads) {
@@ -371,8 +433,8 @@ __global__ __launch_bounds__(kThreads) void read_kernel(CacheRead p, int width_s
             for (int j = 0; j < 4; ++j) codes4f<kFp8>(static_cast<uint32_t>(c[j][q]), x[j]);
 #pragma unroll
             for (int s = 0; s < 4; ++s) {
-                const i32x2 two = {static_cast<int32_t>(narrow2(x[0][s] * vs, x[1][s] * vs, p.half)),
-                                   static_cast<int32_t>(narrow2(x[2][s] * vs, x[3][s] * vs, p.half))};
+                const i32x2 two = {static_cast<int32_t>(narrow2<kHalf>(x[0][s] * vs, x[1][s] * vs)),
+                                   static_cast<int32_t>(narrow2<kHalf>(x[2][s] * vs, x[3][s] * vs))};
                 *reinterpret_cast<i32x2*>(v_out + ((t + 4 * q + s) << width_shift) + d) = two;
             }
         }
@@ -391,21 +453,29 @@ hipError_t cache_plan(const CachePlan& p, hipStream_t s) {
 
 static int log2_of(int n) { return n > 1 ? 1 + log2_of(n / 2) : 0; }
 
-hipError_t cache_append(const CacheAppend& p, bool fp8, hipStream_t s) {
+template <bool kFp8, bool kHalf>
+static hipError_t append(const CacheAppend& p, hipStream_t s) {
     const dim3 grid(static_cast<unsigned>(p.runs_most), static_cast<unsigned>(p.heads), 2);
     const size_t turned = static_cast<size_t>(p.width) * (p.page / 4 + 1) * 4;
-    const int w = log2_of(p.width), t = log2_of(p.page);
-    if (fp8) append_kernel<true><<<grid, kThreads, turned, s>>>(p, w, t);
-    else append_kernel<false><<<grid, kThreads, turned, s>>>(p, w, t);
+    append_kernel<kFp8, kHalf><<<grid, kThreads, turned, s>>>(p, log2_of(p.width), log2_of(p.page));
+    return hipGetLastError();
+}
+
+hipError_t cache_append(const CacheAppend& p, bool fp8, hipStream_t s) {
+    if (fp8) return p.half ? append<true, true>(p, s) : append<true, false>(p, s);
+    return p.half ? append<false, true>(p, s) : append<false, false>(p, s);
+}
+
+template <bool kFp8, bool kHalf>
+static hipError_t read(const CacheRead& p, hipStream_t s) {
+    const dim3 grid(static_cast<unsigned>(p.count), static_cast<unsigned>(p.heads));
+    read_kernel<kFp8, kHalf><<<grid, kThreads, 0, s>>>(p, log2_of(p.width), log2_of(p.page));
     return hipGetLastError();
 }
 
 hipError_t cache_read(const CacheRead& p, bool fp8, hipStream_t s) {
-    const dim3 grid(static_cast<unsigned>(p.count), static_cast<unsigned>(p.heads));
-    const int w = log2_of(p.width), t = log2_of(p.page);
-    if (fp8) read_kernel<true><<<grid, kThreads, 0, s>>>(p, w, t);
-    else read_kernel<false><<<grid, kThreads, 0, s>>>(p, w, t);
-    return hipGetLastError();
+    if (fp8) return p.half ? read<true, true>(p, s) : read<true, false>(p, s);
+    return p.half ? read<false, true>(p, s) : read<false, false>(p, s);
 }
 
 }  // namespace cozyq

@@ -5,32 +5,52 @@
 
 namespace cozyq {
 
-// Eight 16-bit elements at a 16-byte address, as float32.
-__device__ __forceinline__ void widen8(const i32x4& raw, bool half, float* v) {
+// Eight 16-bit elements as float32.
+template <bool kHalf>
+__device__ __forceinline__ void widen8(const i32x4& raw, float* v) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const uint16_t h = static_cast<uint16_t>(static_cast<uint32_t>(raw[i / 2]) >> (16 * (i & 1)));
-        v[i] = half ? widen<true>(h) : widen<false>(h);
+    for (int i = 0; i < 8; ++i) v[i] = widen<kHalf>(static_cast<uint16_t>(static_cast<uint32_t>(raw[i / 2]) >> (16 * (i & 1))));
+}
+
+// The same where the type is known at run time alone: a branch, as a select would work out both.
+__device__ __forceinline__ void widen8(const i32x4& raw, bool half, float* v) {
+    if (half) {
+        asm volatile("");
+        widen8<true>(raw, v);
+    } else {
+        widen8<false>(raw, v);
     }
 }
 
-__device__ __forceinline__ void load8(const uint16_t* p, bool half, float* v) {
-    widen8(*reinterpret_cast<const i32x4*>(p), half, v);
+// Eight 16-bit elements at a 16-byte address, as float32.
+template <bool kHalf>
+__device__ __forceinline__ void load8(const uint16_t* p, float* v) {
+    widen8<kHalf>(*reinterpret_cast<const i32x4*>(p), v);
 }
 
 // Two float32 values rounded to nearest even, the first in the low half: v_cvt_pk_bf16_f32 for bf16; for
 // fp16 each float32 value stands on its own first (see narrow).
-__device__ __forceinline__ uint32_t narrow2(float a, float b, bool half) {
-    if (half) return narrow<true>(a) | (static_cast<uint32_t>(narrow<true>(b)) << 16);
+template <bool kHalf>
+__device__ __forceinline__ uint32_t narrow2(float a, float b) {
+    if constexpr (kHalf) return narrow<true>(a) | (static_cast<uint32_t>(narrow<true>(b)) << 16);
     typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
     const bf16x2 two = {static_cast<__bf16>(a), static_cast<__bf16>(b)};
     return __builtin_bit_cast(uint32_t, two);
 }
 
-__device__ __forceinline__ void store8(uint16_t* p, bool half, const float* v) {
+__device__ __forceinline__ uint32_t narrow2(float a, float b, bool half) {
+    if (half) {
+        asm volatile("");
+        return narrow2<true>(a, b);
+    }
+    return narrow2<false>(a, b);
+}
+
+template <bool kHalf>
+__device__ __forceinline__ void store8(uint16_t* p, const float* v) {
     i32x4 raw;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) raw[i] = static_cast<int32_t>(narrow2(v[2 * i], v[2 * i + 1], half));
+    for (int i = 0; i < 4; ++i) raw[i] = static_cast<int32_t>(narrow2<kHalf>(v[2 * i], v[2 * i + 1]));
     *reinterpret_cast<i32x4*>(p) = raw;
 }
 
