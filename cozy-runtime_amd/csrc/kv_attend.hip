@@ -57,6 +57,14 @@ __device__ __forceinline__ f16x8 codes8(uint32_t a, uint32_t b) {
     return __builtin_bit_cast(f16x8, v);
 }
 
+// 16 bytes of codes, marked as read once or not.
+template <bool kOnce>
+__device__ __forceinline__ i32x4 codes16(const uint8_t* at) {
+    const i32x4* p = reinterpret_cast<const i32x4*>(at);
+    if constexpr (kOnce) return __builtin_nontemporal_load(p);
+    else return *p;
+}
+
 // A finite scale, NaN for an infinite one: whoever sees its page gets NaN, not a score of either sign.
 __device__ __forceinline__ float or_nan(float scale) { return scale + (scale - scale); }
 
@@ -335,7 +343,10 @@ __device__ __forceinline__ void query8(const CacheAttend& p, const uint16_t* x, 
 // values that the group loads for the second product. Codes go from memory to registers to the matrix
 // unit; nothing of the cache passes through LDS but its pages' numbers and scales, read once a tile.
 // A step's keys are loaded over the previous step's second product and its values over its first.
-template <int kWidth, int kTiles, bool kFp8>
+// kOnce (pages of up to 64 tokens): every line of codes is read by one load alone and marked so, which leaves
+// the caches to what is read again: one token for each of 40 requests 86 -> 76 us. The values of a larger
+// page's channel fill a line that two steps share: with the mark 53 us became 57 at 131071 tokens.
+template <int kWidth, int kTiles, bool kFp8, bool kOnce>
 __global__ __launch_bounds__(256, kWidth == 256 ? 1 : 2) void few_kernel(CacheAttend p, Part part, bool clears) {
     constexpr int kWaves = 4, kBlocks = kWidth / 64, kOut = kWidth / 16, kRows = 16 * kTiles;
     __shared__ PageScales entries[kEntries];
@@ -454,7 +465,7 @@ __global__ __launch_bounds__(256, kWidth == 256 ? 1 : 2) void few_kernel(CacheAt
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
 #pragma unroll
-                    for (int b = 0; b < kBlocks; ++b) kc[j][b] = *reinterpret_cast<const i32x4*>(k + 4 * j * kWidth + 64 * b);
+                    for (int b = 0; b < kBlocks; ++b) kc[j][b] = codes16<kOnce>(k + 4 * j * kWidth + 64 * b);
                 }
             };
             const auto load_values = [&](int step) {
@@ -462,7 +473,7 @@ __global__ __launch_bounds__(256, kWidth == 256 ? 1 : 2) void few_kernel(CacheAt
                 const int page = max(entries[(t >> p.shift) - page_first].page, 0);
                 const uint8_t* v = v_lane + page * page_bytes + (t & within);
 #pragma unroll
-                for (int o = 0; o < kOut; ++o) vc[o] = *reinterpret_cast<const i32x4*>(v + 16 * o * p.page);
+                for (int o = 0; o < kOut; ++o) vc[o] = codes16<kOnce>(v + 16 * o * p.page);
             };
             int step = stage + wave;
             if (step < stage_end) {
@@ -1123,8 +1134,10 @@ hipError_t attend(const CacheAttend& p, const AttendShape& a, hipStream_t s) {
     }
     if (a.few.on) {
         const unsigned groups = static_cast<unsigned>((a.few.shares + 1) * p.heads);
-        if (a.few.rows == 16) few_kernel<kWidth, 1, kFp8><<<groups, 256, 0, s>>>(p, few, !a.many.on);
-        else few_kernel<kWidth, 2, kFp8><<<groups, 256, 0, s>>>(p, few, !a.many.on);
+        const bool once = p.page <= 64;
+        const auto kernel = a.few.rows == 16 ? (once ? few_kernel<kWidth, 1, kFp8, true> : few_kernel<kWidth, 1, kFp8, false>)
+                                             : (once ? few_kernel<kWidth, 2, kFp8, true> : few_kernel<kWidth, 2, kFp8, false>);
+        kernel<<<groups, 256, 0, s>>>(p, few, !a.many.on);
     }
     if (a.splits) {
         const int64_t most = 0x7fffffff;
