@@ -592,3 +592,41 @@ def test_a_layer_decodes_as_it_prefills(kv, codes):
     # Keys and values hold 7 (int8, of the page's largest) or 4 bits: a few hundredths of the output.
     rel = (outs[0] - outs[1]).norm() / outs[0].norm()
     assert rel < (0.02 if codes is torch.int8 else 0.08), float(rel)
+
+
+def test_the_decoding_example_replays_what_it_does_eagerly():
+    """`examples/decode.py`: prompts, then tokens from a recorded step, against the same steps run eagerly in
+    a second server: the same kernels on the same numbers, so the same bits, over page boundaries."""
+    import importlib.util
+    from pathlib import Path
+
+    path = Path(__file__).resolve().parents[1] / "examples" / "decode.py"
+    spec = importlib.util.spec_from_file_location("decode_example", path)
+    example = importlib.util.module_from_spec(spec)
+    import sys
+
+    sys.modules["decode_example"] = example
+    spec.loader.exec_module(example)
+    shape = dict(layers=2, requests=3, q_heads=8, kv_heads=2, width=64, page=16, pages=24, longest=96)
+    lengths, steps = [30, 16, 1], 20
+    gen = torch.Generator("cuda").manual_seed(71)
+    prompt = torch.randn(sum(lengths), 512, generator=gen, device=DEV).bfloat16()
+    tokens = torch.randn(steps, 3, 512, generator=gen, device=DEV).bfloat16()
+    a, b = example.Server(**shape), example.Server(**shape)
+    assert torch.equal(a.prompt(prompt, lengths), b.prompt(prompt, lengths))
+    x, y, graph = a.recorded_step()
+    one = torch.ones(3, dtype=torch.int32, device=DEV)
+    # The recorded server has run its step once before it was recorded: the second one does so too.
+    b.forward(torch.zeros_like(x), b.plan(one, 3, 1))
+    for t in range(steps):
+        x.copy_(tokens[t])
+        graph.replay()
+        junk = [torch.full((n,), 7, dtype=torch.int32, device=DEV) for n in (3, 3, 200)]  # takes what is free
+        plan = b.plan(one, 3, 1)
+        want = b.forward(tokens[t], plan)
+        b.commit(plan)
+        torch.cuda.synchronize()
+        assert torch.equal(y, want), t
+        del junk
+    assert a.held.tolist() == [n + steps for n in lengths] == b.held.tolist()
+    assert a.spare.tolist() == b.spare.tolist() and torch.equal(a.table, b.table)
