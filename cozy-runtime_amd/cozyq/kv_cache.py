@@ -114,7 +114,7 @@ class PagedCache:
         over 127 (int8) or 448 (E4M3), at least 1e-12: a run that begins its page sets it, a later one
         raises it where it must, and what the page holds is then rounded again. An infinity or NaN makes
         its page's scale so, for that head: every query that sees the page is NaN there."""
-        index = _dispatch.activation_card(OP, torch, k, v.dtype)
+        index = _dispatch.card(OP, k)
         _dispatch.library(index).cache_append(self, k, v, plan)
 
     def read(self, torch: Any, pages: Tensor, dtype: Dtype) -> tuple[Tensor, Tensor]:
@@ -131,5 +131,5 @@ class PagedCache:
         head h reads key head h // (q_heads / heads). Row t sees its request's tokens up to its own
         position, with a `window` the last `window` of them; without `causal`, all of them. `scale`
         multiplies the scores (None: D^-1/2). A row that sees nothing, or belongs to no request, is 0."""
-        index = _dispatch.activation_card(OP, torch, q)
+        index = _dispatch.card(OP, q)
         return _dispatch.library(index).cache_attend(self, q, plan, scale, causal, window)

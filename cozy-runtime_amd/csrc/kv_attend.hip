@@ -1081,17 +1081,22 @@ constexpr int kFewShares = 512;   // few_kernel's workgroups over all heads: two
 constexpr int kFewSteps = 8;      // of which each takes so many steps at the least,
 constexpr int kWholeSteps = 16;   // but a whole tile where none can have more than these: no join then
 constexpr int kManySteps = 16;    // many_kernel's, whose parts are larger
-constexpr int kFewRows = 64;      // up to here a request's rows are taken by few_kernel alone
-constexpr int kBesideRows = 16;   // and up to here beside requests of more
+constexpr int kFewRows = 64;      // up to here a request's rows are few_kernel's alone,
+constexpr int kFewAllRows = 1024; // and so are all, up to here: one launch less (60 tokens of 8 requests 48 -> 31 us)
+constexpr int kBesideRows = 16;   // up to here they are few_kernel's beside requests of more,
+constexpr int kManyRows = 1024;   // unless so many a request on average leave few such requests
 
 // The shape of a call, which its workspace goes by too. Where a request may have more than kFewRows
 // rows, those of more than kBesideRows go to many_kernel and the others, if there are others, to few_kernel.
+// (With kFewAllRows at 2048 chunks of 300 tokens among 8 requests took 70 us for 57; with kManyRows at 256
+// the chunks of 2311 tokens among 12 took 99 for 87, as their single tokens then run a wave a workgroup.)
 AttendShape shape_of(int64_t tokens, int group, int requests, int heads, int columns, int page, int width, int64_t most) {
     const int64_t rows = (most > 0 && most < tokens ? most : tokens) * group;
     const int all = 0x7fffffff;
     AttendShape a = {};
-    a.few.on = rows <= kFewRows || requests > 1;
-    a.many.on = rows > kFewRows;
+    const int64_t all_rows = tokens * group;
+    a.many.on = rows > kFewRows && all_rows > kFewAllRows;
+    a.few.on = !a.many.on || (requests > 1 && all_rows < kManyRows * requests);
     a.few.rows = rows > 16 && !a.many.on ? 32 : 16;
     a.few.upto = a.many.on ? kBesideRows : all;
     const int64_t steps = (static_cast<int64_t>(columns) * page + kStep - 1) / kStep;  // of a tile, at the most
