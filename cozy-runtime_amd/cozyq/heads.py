@@ -26,5 +26,4 @@ def norm_rope(torch: Any, q: Tensor, k: Tensor | None, q_gain: Tensor | None, k_
     None: row t; a position outside the table reads its nearest row). D and R are multiples of 16, D up
     to 256. q and k may be views (of one QKV buffer, say) whose last axis is dense and whose other
     strides and address are multiples of 16 bytes; the results are new and contiguous."""
-    index = _dispatch.activation_card(OP, torch, q)
-    return _dispatch.library(index).head_norm_rope(q, k, q_gain, k_gain, cos, sin, positions, eps, interleaved)
+    return _dispatch.library(_dispatch.card(OP, q)).head_norm_rope(q, k, q_gain, k_gain, cos, sin, positions, eps, interleaved)

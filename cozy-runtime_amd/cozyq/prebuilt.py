@@ -140,6 +140,8 @@ class Prebuilt:
     _gemv_rows: int = field(init=False)
     _widest: int = field(init=False)
     _current_stream: Any = field(init=False)
+    _int32: Any = field(init=False)
+    _float32: Any = field(init=False)
     #: The fused linear's counters, one zeroed int32 buffer per stream (each call leaves its
     #: buffer zero; calls on one stream run in order, so they share it).
     _workspaces: dict[int, Tensor] = field(init=False, default_factory=dict)
@@ -154,6 +156,7 @@ class Prebuilt:
         self._gemv_rows = int(self._lib.cozyq_gemv_rows())
         self._widest = int(self._lib.cozyq_max_k())
         self._current_stream = self.torch._C._cuda_getCurrentRawStream
+        self._int32, self._float32 = self.torch.int32, self.torch.float32
 
     # ------------------------------------------------------------------ reference surface
 
@@ -1062,7 +1065,7 @@ class Prebuilt:
         sin: Tensor | None, positions: Tensor | None, eps: float | None, interleaved: bool,
     ) -> tuple[Tensor, Tensor | None]:
         """`heads.norm_rope` on this card (`cozyq_head_norm_rope`)."""
-        torch = self.torch
+        f32 = self._float32
         dtype = q.dtype
         half = self._half(dtype)
         tokens, q_heads, width, q_token, q_head = self._heads("norm_rope", "q", q)
@@ -1081,12 +1084,12 @@ class Prebuilt:
         wide = False
         q_by = k_by = None
         if q_gain is not None:
-            wide = q_gain.dtype is torch.float32
-            q_by = self._gain(q_gain, torch.float32 if wide else dtype, width)
+            wide = q_gain.dtype is f32
+            q_by = self._gain(q_gain, f32 if wide else dtype, width)
         if k_gain is not None:
             if q_gain is None:
-                wide = k_gain.dtype is torch.float32
-            k_by = self._gain(k_gain, torch.float32 if wide else dtype, width)
+                wide = k_gain.dtype is f32
+            k_by = self._gain(k_gain, f32 if wide else dtype, width)
         if eps is None and (q_by is not None or k_by is not None):
             raise ValueError("norm_rope: gains without a norm (eps None)")
         rows = rotated = 0
@@ -1095,7 +1098,7 @@ class Prebuilt:
             rows, half_turn = cos.shape if cos.dim() == 2 else (0, 0)
             rotated = 2 * half_turn
             cos_at, sin_at = cos.data_ptr(), sin.data_ptr()
-            if (cos.dtype is not torch.float32 or sin.dtype is not torch.float32 or cos.shape != sin.shape
+            if (cos.dtype is not f32 or sin.dtype is not f32 or cos.shape != sin.shape
                     or not cos.is_contiguous() or not sin.is_contiguous() or (cos_at | sin_at) & 15):  # fmt: skip
                 raise ValueError("norm_rope: cos and sin are dense float32 [rows, R/2], 16-byte aligned")
             if rotated > width or rotated % 16 or rows < 1 or (positions is None and rows < tokens):
@@ -1105,7 +1108,7 @@ class Prebuilt:
             raise ValueError("norm_rope: cos and sin go together")
         if positions is not None:
             rows_at = self._ints("norm_rope", "positions", positions, tokens)
-        if self._elsewhere(q, k, q_gain, k_gain, cos, sin, positions):
+        if self._elsewhere((q, k, q_gain, k_gain, cos, sin, positions)):
             raise ValueError(f"norm_rope: every tensor must be on cuda:{self.index}")
         q_out = q.new_empty((tokens, q_heads, width))
         code = self._lib.cozyq_head_norm_rope(
@@ -1123,7 +1126,7 @@ class Prebuilt:
     ) -> tuple[Tensor, ...]:
         """`kv_cache.plan` on this card (`cozyq_cache_plan`): a plan's starts, lengths, positions, requests,
         slots, runs and spare, new or those of the plan `out`."""
-        int32 = self.torch.int32
+        int32 = self._int32
         if table.dtype is not int32 or table.dim() != 2 or not table.is_contiguous():
             raise ValueError("plan: the block table is dense int32 [requests, width]")
         requests, width = table.shape
@@ -1137,7 +1140,7 @@ class Prebuilt:
         free_at = self._ints("plan", "free", free, count)
         if spare.dtype is not int32 or spare.numel() < 1 or not spare.is_contiguous():
             raise ValueError("plan: spare is int32, the number of free pages first")
-        if self._elsewhere(table, free, spare, held, new):
+        if self._elsewhere((table, free, spare, held, new)):
             raise ValueError(f"plan: every tensor must be on cuda:{self.index}")
         if out is None:
             # One allocation, the runs' rows of 16 bytes first.
@@ -1165,9 +1168,9 @@ class Prebuilt:
         for name, n in parts:
             self._ints("plan", f"out.{name}", getattr(out, name), n)
         if (out.page != page or out.table is not table or tuple(out.runs.shape) != (runs, 4)
-                or out.runs.dtype is not self.torch.int32 or not out.runs.is_contiguous()):  # fmt: skip
+                or out.runs.dtype is not self._int32 or not out.runs.is_contiguous()):  # fmt: skip
             raise ValueError("plan: out was made for another table, page size or number of runs")
-        if self._elsewhere(out.starts, out.lengths, out.positions, out.requests, out.slots, out.runs, out.spare):
+        if self._elsewhere((out.starts, out.lengths, out.positions, out.requests, out.slots, out.runs, out.spare)):
             raise ValueError(f"plan: every tensor must be on cuda:{self.index}")
         if out.spare.data_ptr() == spare.data_ptr() or out.lengths.data_ptr() == held.data_ptr():
             raise ValueError("plan: out's spare and lengths may not be this call's inputs")
@@ -1188,10 +1191,10 @@ class Prebuilt:
             raise ValueError(f"append: the plan is of {plan.slots.shape[0]} tokens in pages of {plan.page}, not of {tokens} in "
                              f"pages of {page}")  # fmt: skip
         runs_at = runs.data_ptr()
-        if (runs.dtype is not self.torch.int32 or runs.dim() != 2 or runs.shape[1] != 4 or not runs.is_contiguous()
+        if (runs.dtype is not self._int32 or runs.dim() != 2 or runs.shape[1] != 4 or not runs.is_contiguous()
                 or runs_at & 15):  # fmt: skip
             raise ValueError("append: the plan's runs are dense int32 [n, 4], 16-byte aligned")
-        if self._elsewhere(cache.k, cache.v, cache.k_scale, cache.v_scale, k, v, runs):
+        if self._elsewhere((cache.k, cache.v, cache.k_scale, cache.v_scale, k, v, runs)):
             raise ValueError(f"append: every tensor must be on cuda:{self.index}")
         code = self._lib.cozyq_cache_append(
             self.index, fp8, k.data_ptr(), v.data_ptr(), half, tokens, k_token, k_head, v_token, v_head, k_codes,
@@ -1206,7 +1209,7 @@ class Prebuilt:
         fp8, pages, heads, page, width, k_codes, v_codes, k_scale, v_scale = self._cache("read", cache)
         count = numbers.numel()
         numbers_at = self._ints("read", "pages", numbers, count)
-        if self._elsewhere(cache.k, cache.v, cache.k_scale, cache.v_scale, numbers):
+        if self._elsewhere((cache.k, cache.v, cache.k_scale, cache.v_scale, numbers)):
             raise ValueError(f"read: every tensor must be on cuda:{self.index}")
         k, v = numbers.new_empty((2, count, heads, page, width), dtype=dtype).unbind(0)
         code = self._lib.cozyq_cache_read(
@@ -1227,7 +1230,7 @@ class Prebuilt:
         if q_width != width or q_heads % heads or not 0 < q_heads // heads <= 64:
             raise ValueError(f"attend: q must be [tokens, n x {heads}, {width}] with n up to 64, not {list(q.shape)}")
         table, starts, lengths, most = plan.table, plan.starts, plan.lengths, plan.most
-        if table.dtype is not self.torch.int32 or table.dim() != 2 or not table.is_contiguous():
+        if table.dtype is not self._int32 or table.dim() != 2 or not table.is_contiguous():
             raise ValueError("attend: the block table is dense int32 [requests, width]")
         requests, columns = table.shape
         starts_at = self._ints("attend", "starts", starts, requests + 1)
@@ -1236,7 +1239,7 @@ class Prebuilt:
             raise ValueError(f"attend: the plan has pages of {plan.page} tokens, the cache of {page}")
         if window < 0 or (window and not causal):
             raise ValueError(f"attend: a window of {window} tokens{'' if causal else ' without causal'}")
-        if self._elsewhere(cache.k, cache.v, cache.k_scale, cache.v_scale, q, table, starts, lengths):
+        if self._elsewhere((cache.k, cache.v, cache.k_scale, cache.v_scale, q, table, starts, lengths)):
             raise ValueError(f"attend: every tensor must be on cuda:{self.index}")
         out = q.new_empty((tokens, q_heads, width))
         size = self._lib.cozyq_cache_attend_workspace_bytes(tokens, q_heads, requests, heads, page, width, columns, most)
@@ -1254,9 +1257,10 @@ class Prebuilt:
     def _heads(self, op: str, name: str, x: Tensor) -> tuple[int, int, int, int, int]:
         """Tokens, heads, width and the token and head strides of a `[tokens, heads, width]` operand that
         the kernels read 16 bytes at a time; ValueError for another."""
-        if x.dim() != 3:
-            raise ValueError(f"{op}: {name} must be [tokens, heads, width], not {list(x.shape)}")
-        tokens, heads, width = x.shape
+        shape = x.shape
+        if len(shape) != 3:
+            raise ValueError(f"{op}: {name} must be [tokens, heads, width], not {list(shape)}")
+        tokens, heads, width = shape
         by_token, by_head, dense = x.stride()
         if (by_token | by_head) & 7 or dense != 1 or x.data_ptr() & 15:
             # The stride of an extent of one is never taken.
@@ -1268,17 +1272,17 @@ class Prebuilt:
     def _gain(self, gain: Tensor, dtype: Dtype, width: int) -> int:
         """The address of a head gain; ValueError unless it is dense `[width]` of `dtype`."""
         at = gain.data_ptr()
-        if gain.dtype is not dtype or gain.dim() != 1 or gain.shape[0] != width or not gain.is_contiguous() or at & 15:
+        if gain.dtype is not dtype or gain.shape != (width,) or not gain.is_contiguous() or at & 15:
             raise ValueError(f"norm_rope: gains are dense [{width}], 16-byte aligned, both float32 or of q's type")
         return at
 
     def _ints(self, op: str, name: str, x: Tensor, count: int) -> int:
         """The address of `count` dense int32 numbers; ValueError for other tensors."""
-        if x.dtype is not self.torch.int32 or x.dim() != 1 or x.shape[0] != count or not x.is_contiguous():
+        if x.dtype is not self._int32 or x.shape != (count,) or not x.is_contiguous():
             raise ValueError(f"{op}: {name} must be dense int32 [{count}], not {x.dtype} {list(x.shape)}")
         return x.data_ptr()
 
-    def _elsewhere(self, *tensors: Tensor | None) -> bool:
+    def _elsewhere(self, tensors: tuple[Tensor | None, ...]) -> bool:
         """Whether any of the given tensors is not on this card (a CPU tensor's device number is -1)."""
         index = self.index
         for t in tensors:
@@ -1300,7 +1304,7 @@ class Prebuilt:
         if (v.shape != (pages, heads, width, page) or page not in (16, 32, 64, 128, 256) or width not in (64, 128, 256)
                 or not k.is_contiguous() or not v.is_contiguous() or (k_at | v_at) & 15):  # fmt: skip
             raise ValueError(f"{op}: no cache of dense, 16-byte aligned keys {list(k.shape)} and values {list(v.shape)}")
-        shape, f32 = (pages, heads), torch.float32
+        shape, f32 = (pages, heads), self._float32
         if (k_scale.dtype is not f32 or v_scale.dtype is not f32 or k_scale.shape != shape or v_scale.shape != shape
                 or not k_scale.is_contiguous() or not v_scale.is_contiguous()):  # fmt: skip
             raise ValueError(f"{op}: the cache's scales are dense float32 [{pages}, {heads}]")
