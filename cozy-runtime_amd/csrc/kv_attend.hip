@@ -137,9 +137,9 @@ struct Share {
 // c = max(least, N / shares) of one row tile's, so that there are at most shares + tiles workgroups
 // and at most 2 · shares places (a tile of more than c steps splits into less than 2 · steps / c),
 // whatever the requests' lengths are: the host sizes the launch and the workspace without knowing them.
-// Finds workgroup `id`'s share (kById), or row tile `id`'s first; false past the last, and for row tiles
-// where none is split. A request's last
-// tile comes first: where causal it has the most to do. Every wave scans all requests, 64 at a time.
+// Finds workgroup `id`'s share (kById), or the first of split row tile number `id`; false past the last. A
+// request's last tile comes first: where causal it has the most to do. Every wave scans all requests, 64 at
+// a time.
 template <bool kById>
 __device__ bool find_share(const CacheAttend& p, const Part& part, int id, Share& out) {
     const int lane = threadIdx.x & 63;
@@ -161,8 +161,8 @@ __device__ bool find_share(const CacheAttend& p, const Part& part, int id, Share
         Extent e = e0;
         if (base) e = base + lane < p.requests ? extent(p, part, base + lane) : Extent{0, 0};
         const int splits = max(1, (e.steps + c - 1) / c);
-        const int ids = wave_prefix(kById ? e.tiles * splits : e.tiles);
         const int places = wave_prefix(splits > 1 ? e.tiles * splits : 0);
+        const int ids = wave_prefix(kById ? e.tiles * splits : splits > 1 ? e.tiles : 0);
         const uint64_t past = __ballot(ids_before + ids > id);
         if (past) {
             const int at = __ffsll(static_cast<unsigned long long>(past)) - 1;
@@ -990,16 +990,17 @@ __device__ __forceinline__ void add_all(const Parts& parts, int width, int quad,
 // threads a row, its parts one after another. Which thread sums which parts is fixed: a call's result does
 // not vary.
 template <int kWidth>
-__global__ __launch_bounds__(256) void join_kernel(CacheAttend p, Part few, Part many, int few_rows, int few_items, int many_items) {
+__global__ __launch_bounds__(256) void join_kernel(CacheAttend p, Part few, Part many, int few_rows, int many_rows, int few_items, int many_items) {
     constexpr int kQuads = kWidth / 4, kParts = 256 / kQuads;
     __shared__ f32x4 sums[kParts][kQuads];
     __shared__ float totals[kParts];
     const int thread = threadIdx.x, slice = thread / kQuads, quad = thread % kQuads;
     const bool wide = blockIdx.y != 0;
     const Part part = wide ? many : few;
-    const int rows_all = 1 << part.shift, groups = wide ? rows_all / kParts : few_rows;
+    const int rows_all = 1 << part.shift, groups = wide ? many_rows : few_rows;
     const int items = wide ? many_items : few_items;
     const int64_t row_floats = kWidth + 4, place_floats = static_cast<int64_t>(p.heads) * rows_all * row_floats;
+    if (blockIdx.x >= items) return;
     Survey sv;
     if (!wide) {
         sv = survey(p, part);
@@ -1027,7 +1028,7 @@ __global__ __launch_bounds__(256) void join_kernel(CacheAttend p, Part few, Part
         if (parts.count == 1) continue;
         const int first = row_start(p, request), rows = (row_start(p, request + 1) - first) * p.group;
         const int row0 = tile << part.shift, count = min(rows_all, rows - row0);
-        for (int r = wide ? group * kParts + slice : group; r < count; r += wide ? rows_all : groups) {
+        for (int r = wide ? group * kParts + slice : group; r < count; r += wide ? groups * kParts : groups) {
             const int64_t at = (static_cast<int64_t>(kv) * rows_all + r) * row_floats;
             const Parts row = {parts.first + at, parts.others + at, parts.next, parts.count};
             float best = kNoScore, sum;
@@ -1081,6 +1082,7 @@ constexpr int kFewShares = 512;   // few_kernel's workgroups over all heads: two
 constexpr int kFewSteps = 8;      // of which each takes so many steps at the least,
 constexpr int kWholeSteps = 16;   // but a whole tile where none can have more than these: no join then
 constexpr int kManySteps = 16;    // many_kernel's, whose parts are larger
+constexpr int64_t kJoinGroups = 1024;  // join_kernel's workgroups for each of the two launches
 constexpr int kFewRows = 64;      // up to here a request's rows are few_kernel's alone,
 constexpr int kFewAllRows = 1024; // and so are all, up to here: one launch less (60 tokens of 8 requests 48 -> 31 us)
 constexpr int kBesideRows = 16;   // up to here they are few_kernel's beside requests of more,
@@ -1145,12 +1147,16 @@ hipError_t attend(const CacheAttend& p, const AttendShape& a, hipStream_t s) {
         kernel<<<groups, 256, 0, s>>>(p, few, !a.many.on);
     }
     if (a.splits) {
-        const int64_t most = 0x7fffffff;
+        const int64_t most = 0x7fffffff, one = 1;
         const int64_t few_items = a.few.on ? min(most, a.few.tiles * p.heads * a.few.row_groups) : 0;
-        const int64_t many_items = a.many.on ? min(most, a.many.tiles * p.heads * (a.many.rows * kWidth / 1024)) : 0;
-        const unsigned groups = static_cast<unsigned>(min(max(few_items, many_items), static_cast<int64_t>(1024)));
-        join_kernel<kWidth><<<dim3(groups, a.many.on ? 2 : 1), 256, 0, s>>>(p, few, many, a.few.row_groups, static_cast<int>(few_items),
-                                                                           static_cast<int>(many_items));
+        // A split tile has more steps than a share, so that there are no more of them than shares; and no more
+        // groups of rows than workgroups, as each looks its tile up.
+        const int64_t tiles = a.many.on ? min(a.many.tiles, static_cast<int64_t>(a.many.shares)) * p.heads : 0;
+        const int64_t row_groups = max(one, min(kJoinGroups / max(tiles, one), static_cast<int64_t>(a.many.rows * kWidth / 1024)));
+        const int64_t many_items = tiles * row_groups;
+        const unsigned groups = static_cast<unsigned>(min(max(few_items, many_items), kJoinGroups));
+        join_kernel<kWidth><<<dim3(groups, a.many.on ? 2 : 1), 256, 0, s>>>(
+            p, few, many, a.few.row_groups, static_cast<int>(row_groups), static_cast<int>(few_items), static_cast<int>(many_items));
     }
     return hipGetLastError();
 }
