@@ -47,7 +47,7 @@ class Plan:
     slot -1 where no page was left; `runs` `[N, 4]`: the new tokens of one page each (first row, count,
     page or -1, first place in the page), unused ones last as (0, 0, -1, 0); `spare` `[2]`: free pages
     left, and pages wanted and not got. `most`: the most rows a request has, as far as the host knows
-    (0: not at all); attention chooses its kernel by it, with the same results for any value."""
+    (0: not at all); attention chooses its kernels by it, and any value is right."""
 
     page: int
     most: int

@@ -11,9 +11,8 @@
 // weight's exponent, p = 2^(s·log2(e) + log2(vs) − m), so that m bounds what a token adds to the
 // output rather than its probability, and the denominator takes p/vs. A query row is brought near
 // 2^12 by a power of two and is then exact in f16, but for what lies below 2^-26 of its largest
-// element. Weights are
-// rounded to f16 (11 bits, three more than bf16) for the second product alone; maxima, sums and both
-// products' accumulators are float32.
+// element. Weights are rounded to f16 (11 bits, three more than bf16) for the second product alone; maxima,
+// sums and both products' accumulators are float32.
 #include <hip/hip_runtime.h>
 
 #include "common.h"
@@ -344,8 +343,12 @@ __device__ __forceinline__ void query8(const CacheAttend& p, const uint16_t* x, 
 // unit; nothing of the cache passes through LDS but its pages' numbers and scales, read once a tile.
 // A step's keys are loaded over the previous step's second product and its values over its first.
 // kOnce (pages of up to 64 tokens): every line of codes is read by one load alone and marked so, which leaves
-// the caches to what is read again: one token for each of 40 requests 86 -> 76 us. The values of a larger
+// the caches to what is read again: one token for each of 40 requests 86 -> 75 us. The values of a larger
 // page's channel fill a line that two steps share: with the mark 53 us became 57 at 131071 tokens.
+// Bound by the codes' way from memory: those 40 requests' up to 12001 tokens, 8 heads of 128, are 437 MB in 75 us,
+// 5.8 TB/s of the 6.05 that a large read reaches; 131071 tokens of one request, 268 MB, 53 us, 5.1 TB/s, with
+// some 5 us before the first codes arrive (the requests' survey, the pages' numbers and scales) and after the
+// last. 700 tokens of one request are 10.9 us on 8 workgroups of 11 steps: that chain alone.
 template <int kWidth, int kTiles, bool kFp8, bool kOnce>
 __global__ __launch_bounds__(256, kWidth == 256 ? 1 : 2) void few_kernel(CacheAttend p, Part part, bool clears) {
     constexpr int kWaves = 4, kBlocks = kWidth / 64, kOut = kWidth / 16, kRows = 16 * kTiles;
@@ -637,6 +640,12 @@ __device__ __forceinline__ int exchanged(int m) { return (m & ~12) | ((m & 4) <<
 // the keys at token π(m), score register 8a + e of half h = l/32 is that of token 16a + 8h + e, in the order
 // that the second product reads its weights in. Bytes past the request's tokens and pages that the cache has
 // not become zeros on the way to LDS.
+// Bound by no unit alone: 14003 tokens of two requests, 32 heads of 128 over 8, are 857 GFLOP in 0.94 to 1.07 ms
+// as the clock allows, 0.80 to 0.91 PFLOP/s where a large f16 product reaches 1.18; of a SIMD's cycles the
+// matrix unit is busy in 42%, the vector unit in 54% (a fifth in both at once), of a CU's the LDS in 43%.
+// Without the exponentials it was 6% faster, without the conversions 9%, without loads 3%. At width 64 (2311
+// tokens of 12 requests, 16 heads over 4, a window of 4096: 30 GFLOP in 74 us) a score costs the vector unit
+// as much for half the products: VALU 47%, matrix unit 20%.
 template <int kWidth, int kWaves, bool kFp8>
 __global__ __launch_bounds__(64 * kWaves, kWidth == 256 ? 1 : 2) void many_kernel(CacheAttend p, Part part, bool clears) {
     constexpr int kRows = 32 * kWaves, kThreads = 64 * kWaves, kOut = kWidth / 32, kDepth = kWidth / 16;
@@ -988,7 +997,8 @@ __device__ __forceinline__ void add_all(const Parts& parts, int width, int quad,
 // largest reference; blockIdx.y says of which launch. few_kernel's rows are few and their parts many: a
 // workgroup a row, kWidth/4 threads a part. many_kernel's rows are many and their parts few: kWidth/4
 // threads a row, its parts one after another. Which thread sums which parts is fixed: a call's result does
-// not vary.
+// not vary. Bound by latency, of the survey and two trips to memory: one row of 32 heads for each of 40 requests
+// 6.5 us (1.9 MB), 64 rows of up to 65 parts 7.7 us, the parts of 2311 tokens at width 64 10.2 us (22 MB).
 template <int kWidth>
 __global__ __launch_bounds__(256) void join_kernel(CacheAttend p, Part few, Part many, int few_rows, int many_rows, int few_items, int many_items) {
     constexpr int kQuads = kWidth / 4, kParts = 256 / kQuads;
