@@ -998,7 +998,7 @@ __device__ __forceinline__ void add_all(const Parts& parts, int width, int quad,
 // workgroup a row, kWidth/4 threads a part. many_kernel's rows are many and their parts few: kWidth/4
 // threads a row, its parts one after another. Which thread sums which parts is fixed: a call's result does
 // not vary. Bound by latency, of the survey and two trips to memory: one row of 32 heads for each of 40 requests
-// 6.5 us (1.9 MB), 64 rows of up to 65 parts 7.7 us, the parts of 2311 tokens at width 64 10.2 us (22 MB).
+// 6.5 us (1.9 MB), 64 rows of 64 parts 7.7 us, the parts of 2311 tokens at width 64 10.2 us (22 MB).
 template <int kWidth>
 __global__ __launch_bounds__(256) void join_kernel(CacheAttend p, Part few, Part many, int few_rows, int many_rows, int few_items, int many_items) {
     constexpr int kQuads = kWidth / 4, kParts = 256 / kQuads;

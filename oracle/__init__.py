@@ -3,7 +3,8 @@
 This package restates, on the CPU, the laws of cozy-runtime's quantized-linear path (activation
 rotation, per-token int8 / fp8 quantization, MX block scaling, the W8A8 products) plus the two
 laws this build defines where the reference has none (the 128-block rotation and the int4-g64
-SVDQuant variant). It is the checker that the HIP kernels are compared against.
+SVDQuant variant) and, in `cache.py`, the language-model operators' formulas. It is the checker
+that the HIP kernels are compared against.
 
 Only `tests/`, `__graft_entry__.smoke()` and `bench.py`'s `cpu_baseline` leg may import it, and
 there only as the checker or as the timed CPU baseline — never as the thing measured for the GPU
