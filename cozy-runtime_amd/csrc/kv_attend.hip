@@ -99,6 +99,16 @@ __device__ __forceinline__ T wave_prefix(T x) {
     return x;
 }
 
+// The largest of a wave's numbers, none of them negative, in its last lane.
+__device__ __forceinline__ int wave_top(int x) {
+    x = max(x, dpp_or_zero<0x111, 0xF>(x));
+    x = max(x, dpp_or_zero<0x112, 0xF>(x));
+    x = max(x, dpp_or_zero<0x114, 0xF>(x));
+    x = max(x, dpp_or_zero<0x118, 0xF>(x));
+    x = max(x, dpp_or_zero<0x142, 0xA>(x));
+    return max(x, dpp_or_zero<0x143, 0xC>(x));
+}
+
 // --------------------------------------------------------------------- sharing the work out
 
 constexpr int kStep = 64;       // tokens taken at a time
@@ -110,6 +120,7 @@ struct Part {
     int least;    // steps a workgroup takes at the least
     int shift;    // a row tile is 1 << shift rows
     float* work;  // places of a row tile's rows · (width + 4) floats: a row's sums, reference, denominator
+    int cuts;     // how many of kCuts a long tile's steps may be cut by
 };
 
 // A request's part of the work: row tiles, and the 64-token steps that any of its rows sees.
@@ -132,19 +143,26 @@ struct Share {
     int request, tile, split, splits, place;
 };
 
-// All the row tiles' steps are shared out evenly: with N steps in all (a head), a workgroup takes
-// c = max(least, N / shares) of one row tile's, so that there are at most shares + tiles workgroups
-// and at most 2 · shares places (a tile of more than c steps splits into less than 2 · steps / c),
-// whatever the requests' lengths are: the host sizes the launch and the workspace without knowing them.
-// Finds workgroup `id`'s share (kById), or the first of split row tile number `id`; false past the last. A
-// request's last tile comes first: where causal it has the most to do. Every wave scans all requests, 64 at
-// a time.
-template <bool kById>
-__device__ bool find_share(const CacheAttend& p, const Part& part, int id, Share& out) {
+// A workgroup's steps are N / shares over one of these, N the steps in all (a head).
+constexpr float kCuts[] = {1.0f, 4.0f / 3.0f, 2.0f};
+constexpr int kCutCount = 3, kMostCut = 2;
+
+// All the row tiles' steps are shared out evenly: a workgroup takes c = max(least, N / (shares · cut)) of one
+// row tile's, so that there are at most shares · cut workgroups more than tiles and at most 2 · shares · cut
+// places (a tile of more than c steps splits into less than 2 · steps / c), whatever the requests' lengths
+// are: the host sizes the launch and the workspace without knowing them.
+// Where tiles are split and a CU holds one workgroup, the cut is the one of least cost: the rounds of `shares`
+// workgroups, each as long as the longest share and kStartSteps, and a part's way through memory, 1/kPartsAStep
+// of a step. (Chunks of 574 tokens among 11 requests, 64 heads over 8: at cut 1, 4/3 and 2 189, 162 and
+// 176 us; 500 among 8 137, 114 and 112; but 500 among 4 of 20000 tokens 203, 255 and 219. The choice costs 3 us, so
+// that it is not made over shares of less than 3/2 · least steps, where 54 became 57.)
+constexpr float kStartSteps = 4.0f, kPartsAStep = 48.0f;
+
+__device__ int steps_a_share(const CacheAttend& p, const Part& part, Extent& e0) {
     const int lane = threadIdx.x & 63;
     float work = 0.0f;  // in float32, which no number of steps overflows; the margin is over its rounding
     int longest = 0;
-    Extent e0 = {0, 0};
+    e0 = {0, 0};
     for (int base = 0; base < p.requests; base += 64) {
         Extent e = {0, 0};
         if (base + lane < p.requests) e = extent(p, part, base + lane);
@@ -153,13 +171,51 @@ __device__ bool find_share(const CacheAttend& p, const Part& part, int id, Share
         longest = max(longest, e.steps);
         if (base == 0) e0 = e;
     }
-    const int c = max(part.least, static_cast<int>(work * 1.001f / static_cast<float>(part.shares)) + 1);
-    if (!kById && !__any(longest > c)) return false;  // nothing is split: nothing to join
+    const float shares = static_cast<float>(part.shares), one = work * 1.001f / shares;
+    const int most = max(part.least, static_cast<int>(one) + 1);
+    if (!__any(longest > most)) return 0x7fffffff;  // nothing is split
+    if (part.cuts == 1 || 2 * most < 3 * part.least) return most;
+    int count[kCutCount] = {}, places[kCutCount] = {}, top[kCutCount] = {};
+    for (int base = 0; base < p.requests; base += 64) {
+        Extent e = e0;
+        if (base) e = base + lane < p.requests ? extent(p, part, base + lane) : Extent{0, 0};
+#pragma unroll
+        for (int k = 0; k < kCutCount; ++k) {
+            const int c = max(part.least, static_cast<int>(one / kCuts[k]) + 1);
+            const int splits = max(1, (e.steps + c - 1) / c);
+            count[k] += __builtin_amdgcn_readlane(wave_prefix(e.tiles * splits), 63);
+            places[k] += __builtin_amdgcn_readlane(wave_prefix(splits > 1 ? e.tiles * splits : 0), 63);
+            top[k] = max(top[k], __builtin_amdgcn_readlane(wave_top((e.steps + splits - 1) / splits), 63));
+        }
+    }
+    int best = most;
+    float least_cost = __builtin_inff();
+#pragma unroll
+    for (int k = 0; k < kCutCount; ++k) {
+        const float rounds = ceilf(static_cast<float>(count[k]) / shares);
+        const float cost = rounds * (static_cast<float>(top[k]) + kStartSteps) + static_cast<float>(places[k]) * p.heads / kPartsAStep;
+        if (cost < least_cost) {
+            least_cost = cost;
+            best = max(part.least, static_cast<int>(one / kCuts[k]) + 1);
+        }
+    }
+    return __builtin_amdgcn_readfirstlane(best);
+}
+
+// Finds workgroup `id`'s share (kById), or the first of split row tile number `id`; false past the last. A
+// request's last tile comes first: where causal it has the most to do. Every wave scans all requests, 64 at
+// a time.
+template <bool kById>
+__device__ bool find_share(const CacheAttend& p, const Part& part, int id, Share& out) {
+    const int lane = threadIdx.x & 63;
+    Extent e0;
+    const int c = steps_a_share(p, part, e0);
+    if (!kById && c == 0x7fffffff) return false;  // nothing to join
     int ids_before = 0, places_before = 0;
     for (int base = 0; base < p.requests; base += 64) {
         Extent e = e0;
         if (base) e = base + lane < p.requests ? extent(p, part, base + lane) : Extent{0, 0};
-        const int splits = max(1, (e.steps + c - 1) / c);
+        const int splits = e.steps > c ? (e.steps + c - 1) / c : 1;
         const int places = wave_prefix(splits > 1 ? e.tiles * splits : 0);
         const int ids = wave_prefix(kById ? e.tiles * splits : splits > 1 ? e.tiles : 0);
         const uint64_t past = __ballot(ids_before + ids > id);
@@ -1074,9 +1130,12 @@ __global__ __launch_bounds__(256) void join_kernel(CacheAttend p, Part few, Part
 // One of a call's launches: its row tiles' rows, their number at the most, and where its places begin.
 struct Launch {
     bool on;
-    int rows, over, upto, shares, least, row_groups;
+    int rows, over, upto, shares, least, row_groups, cuts;
     int64_t tiles, offset;
 };
+
+// Workgroups that a launch's steps are cut into, at the most.
+int most_shares(const Launch& l) { return l.cuts == 1 ? l.shares : kMostCut * l.shares; }
 
 // Eight waves share a step's tiles; at width 64 those are too small for so many, at 256 a wave takes 512
 // registers.
@@ -1092,6 +1151,7 @@ constexpr int kFewShares = 512;   // few_kernel's workgroups over all heads: two
 constexpr int kFewSteps = 8;      // of which each takes so many steps at the least,
 constexpr int kWholeSteps = 16;   // but a whole tile where none can have more than these: no join then
 constexpr int kManySteps = 16;    // many_kernel's, whose parts are larger
+constexpr int kCutSteps = 64;     // with more, and a CU to a workgroup, many_kernel chooses among kCuts
 constexpr int64_t kJoinGroups = 1024;  // join_kernel's workgroups for each of the two launches
 constexpr int kFewRows = 64;      // up to here a request's rows are few_kernel's alone,
 constexpr int kFewAllRows = 1024; // and so are all, up to here: one launch less (60 tokens of 8 requests 48 -> 31 us)
@@ -1127,26 +1187,27 @@ AttendShape shape_of(int64_t tokens, int group, int requests, int heads, int col
     a.many.upto = all;
     a.many.least = kManySteps;
     a.many.shares = max(1, (width == 64 ? 512 : 256) / heads);
+    a.many.cuts = width > 64 && steps > kCutSteps ? kCutCount : 1;
     a.many.tiles = (tokens * group + a.many.rows - 1) / a.many.rows + requests - 1;
     a.splits = steps > kWholeSteps;
     if (a.splits) {
         if (a.few.on) a.floats += 2ll * a.few.shares * heads * a.few.rows * (width + 4);
         a.many.offset = a.floats;
-        if (a.many.on) a.floats += 2ll * a.many.shares * heads * a.many.rows * (width + 4);
+        if (a.many.on) a.floats += 2ll * most_shares(a.many) * heads * a.many.rows * (width + 4);
     }
     return a;
 }
 
 int log2_of(int n) { return n > 1 ? 1 + log2_of(n / 2) : 0; }
 
-Part part_of(const CacheAttend& p, const Launch& l) { return {l.over, l.upto, l.shares, l.least, log2_of(l.rows), p.work + l.offset}; }
+Part part_of(const CacheAttend& p, const Launch& l) { return {l.over, l.upto, l.shares, l.least, log2_of(l.rows), p.work + l.offset, l.cuts}; }
 
 template <int kWidth, bool kFp8>
 hipError_t attend(const CacheAttend& p, const AttendShape& a, hipStream_t s) {
     const Part few = part_of(p, a.few), many = part_of(p, a.many);
     if (a.many.on) {
         constexpr int kWaves = many_waves(kWidth);
-        const unsigned groups = static_cast<unsigned>((a.many.shares + a.many.tiles + 1) * p.heads);
+        const unsigned groups = static_cast<unsigned>((most_shares(a.many) + a.many.tiles + 1) * p.heads);
         many_kernel<kWidth, kWaves, kFp8><<<groups, 64 * kWaves, 0, s>>>(p, many, true);
     }
     if (a.few.on) {
@@ -1161,7 +1222,7 @@ hipError_t attend(const CacheAttend& p, const AttendShape& a, hipStream_t s) {
         const int64_t few_items = a.few.on ? min(most, a.few.tiles * p.heads * a.few.row_groups) : 0;
         // A split tile has more steps than a share, so that there are no more of them than shares; and no more
         // groups of rows than workgroups, as each looks its tile up.
-        const int64_t tiles = a.many.on ? min(a.many.tiles, static_cast<int64_t>(a.many.shares)) * p.heads : 0;
+        const int64_t tiles = a.many.on ? min(a.many.tiles, static_cast<int64_t>(most_shares(a.many))) * p.heads : 0;
         const int64_t row_groups = max(one, min(kJoinGroups / max(tiles, one), static_cast<int64_t>(a.many.rows * kWidth / 1024)));
         const int64_t many_items = tiles * row_groups;
         const unsigned groups = static_cast<unsigned>(min(max(few_items, many_items), kJoinGroups));
