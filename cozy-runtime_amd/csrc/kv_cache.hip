@@ -94,7 +94,7 @@ __global__ __launch_bounds__(kThreads) void plan_kernel(CachePlan p) {
     int *starts = shared, *taken = starts + R + 1, *first_run = taken + R + 1, *held_of = first_run + R + 1;
     for (int r = threadIdx.x; r < R; r += kThreads) {
         starts[r] = min(max(p.fresh[r], 0), p.tokens);
-        held_of[r] = max(p.held[r], 0);
+        held_of[r] = min(max(p.held[r], 0), kMostTokens - 256);  // with new ones and a page's rest below 2^31
     }
     __syncthreads();
     prefix(starts, R, p.tokens, wave_sums);

@@ -504,7 +504,8 @@ int cozyq_head_norm_rope(int device, const void* q, const void* k, int half, int
  * `fresh` [requests] int32: tokens it brings. The step's rows are the requests' new tokens one request
  * after another; `tokens` rows in all, those past the last request's belonging to none (a request whose
  * tokens would pass the last row has its count cut there). A page that a request does not hold yet comes
- * off the end of `free` [free_count], of which spare[0] are free, in row order. Negative counts are 0.
+ * off the end of `free` [free_count], of which spare[0] are free, in row order. Negative counts are 0,
+ * and held ones at the most 2^30 - 256.
  * Writes: the new pages into `table` [requests, width]; starts [requests + 1] (each request's first
  * row), lengths [requests] (tokens held after the step); positions, requests_out, slots [tokens] (the
  * token's position, request and page · page size + place in the page; 0, -1 and -1 for a row of none, slot

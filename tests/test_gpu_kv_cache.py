@@ -77,6 +77,19 @@ def test_plan_without_enough_pages_columns_or_rows(kv):
     check_plan(kv, table, [4, 5, 6, 7], 4, [16, 0, 30], [2**31 - 1, 2**31 - 1, 1], 9, 16)  # sums past 32 bits
 
 
+@pytest.mark.parametrize("page", [16, 256])
+def test_plan_of_counts_past_any_cache(kv, page):
+    # What a request may hold is cut at 2^30 - 256: its sums stay below 2^31, its rows get no page, others' do.
+    t = ints([[3, 4], [5, -1]])
+    got = kv.plan(torch, t, ints([8, 9]), ints([2]), ints([2**31 - 1, page]), ints([3, 2]), tokens=5, page=page)
+    held = 2**30 - 256
+    assert got.lengths.tolist() == [held + 3, page + 2]
+    assert got.positions.tolist() == [held, held + 1, held + 2, page, page + 1]
+    assert got.slots.tolist() == [-1, -1, -1, 9 * page, 9 * page + 1]
+    assert got.runs.tolist()[:2] == [[0, 3, -1, 0], [3, 2, 9, 0]]
+    assert t.tolist() == [[3, 4], [5, 9]] and int(got.spare[0]) == 1
+
+
 def test_plan_written_again_and_in_a_graph(kv):
     """`out` takes the next step's plan; captured, each replay gives the eager plan's answer."""
     table, free = [[5, -1, -1], [-1, -1, -1]], [0, 1, 2, 3, 4]
