@@ -119,7 +119,7 @@ struct Part {
     int over, upto, shares;
     int least;    // steps a workgroup takes at the least
     int shift;    // a row tile is 1 << shift rows
-    float* work;  // places of a row tile's rows · (width + 4) floats: a row's sums, reference, denominator
+    float* work;  // places of a row tile's rows · (width + 4) floats: a row's sums, reference, denominator; or none
     int cuts;     // how many of kCuts a long tile's steps may be cut by
 };
 
@@ -277,7 +277,8 @@ __device__ Survey survey(const CacheAttend& p, const Part& part) {
         sv.total += __builtin_amdgcn_readlane(wave_prefix(e.tiles * units), 63);
         runs += __builtin_amdgcn_readlane(wave_prefix(e.tiles * ((units + sv.c - 1) / sv.c)), 63);
     }
-    sv.aligned = runs <= part.shares;
+    // Without places for parts (no tile can be cut) runs hold whole tiles, however many rows `starts` speaks of.
+    sv.aligned = !part.work || runs <= part.shares;
     if (sv.aligned) sv.total = runs * sv.c;
     else sv.c = max(sv.c, (sv.total + part.shares - 1) / part.shares);
     return sv;
@@ -338,7 +339,8 @@ __device__ __forceinline__ Span span_of(const CacheAttend& p, int row0, int rows
     s.low_least = p.window > 0 ? max(0, before + t0 + 1 - p.window) : 0;
     s.low_most = p.window > 0 ? max(0, before + t1 + 1 - p.window) : 0;
     s.high_least = p.causal ? before + t0 + 1 : length;
-    s.high_most = p.causal ? before + t1 + 1 : length;
+    // Past what the table's row has pages for there is nothing to see, whatever the length says.
+    s.high_most = min(p.causal ? before + t1 + 1 : length, p.width << p.shift);
     const int from = s.low_least / kStep, steps = max(0, (s.high_most + kStep - 1) / kStep - from);
     s.begin = from + static_cast<int>(static_cast<int64_t>(steps) * split / splits);
     s.end = from + static_cast<int>(static_cast<int64_t>(steps) * (split + 1) / splits);
@@ -1200,11 +1202,13 @@ AttendShape shape_of(int64_t tokens, int group, int requests, int heads, int col
 
 int log2_of(int n) { return n > 1 ? 1 + log2_of(n / 2) : 0; }
 
-Part part_of(const CacheAttend& p, const Launch& l) { return {l.over, l.upto, l.shares, l.least, log2_of(l.rows), p.work + l.offset, l.cuts}; }
+Part part_of(const CacheAttend& p, const AttendShape& a, const Launch& l) {
+    return {l.over, l.upto, l.shares, l.least, log2_of(l.rows), a.splits ? p.work + l.offset : nullptr, l.cuts};
+}
 
 template <int kWidth, bool kFp8>
 hipError_t attend(const CacheAttend& p, const AttendShape& a, hipStream_t s) {
-    const Part few = part_of(p, a.few), many = part_of(p, a.many);
+    const Part few = part_of(p, a, a.few), many = part_of(p, a, a.many);
     if (a.many.on) {
         constexpr int kWaves = many_waves(kWidth);
         const unsigned groups = static_cast<unsigned>((most_shares(a.many) + a.many.tiles + 1) * p.heads);

@@ -519,6 +519,19 @@ def test_attend_rows_of_no_request_and_missing_pages(kv):
         assert ((got.double() - want).abs() <= 2.0**-8 * want.abs() + 2.0**-10 * size).all()
 
 
+@pytest.mark.parametrize("new", [[1, 2], [90, 5], [300, 150]], ids=["one", "few", "many"])
+def test_attend_lengths_past_any_table(kv, new):
+    # Steps end where the table's row does, so that such a call is as short as one over full rows.
+    cache, table, value = filled(kv, [96, 192], 16, 2, 64, torch.int8, 61)
+    plan, starts, tokens = make_plan(kv, table, [2**31 - 1] * 2, new, 16, max(new))
+    q = torch.randn(tokens, 8, 64, generator=torch.Generator().manual_seed(62)).bfloat16()
+    got = cache.attend(torch, q.to(DEV), plan, causal=False).cpu()
+    want, size = law.attend(q, value[0], value[1], table, starts, [96, 192], 16, None, False)
+    error = (got.double() - want).abs()
+    assert (error <= UNIT[torch.bfloat16] * want.abs() + (2.0**-11 + 2.0**-12) * size).all()
+    assert (cache.attend(torch, q.to(DEV), plan, window=40) == 0).all()
+
+
 @BOTH
 @pytest.mark.parametrize("kind", ["keys", "values"])
 @pytest.mark.parametrize("bad", [math.nan, math.inf])
