@@ -154,7 +154,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         [c_int, c_int, _P, _P, _P, _P, c_int, c_int, c_int, c_int, _P, c_int64, _P, _P, c_int, _P],
     ),
     "cozyq_cache_attend_workspace_bytes": (
-        c_int64, [c_int64, c_int, c_int, c_int, c_int, c_int, c_int, c_int64]
+        c_int64, [c_int64, c_int, c_int, c_int, c_int, c_int, c_int, c_int64, c_int]
     ),
     "cozyq_cache_attend": (
         c_int,

@@ -1242,7 +1242,7 @@ class Prebuilt:
         if self._elsewhere((cache.k, cache.v, cache.k_scale, cache.v_scale, q, table, starts, lengths)):
             raise ValueError(f"attend: every tensor must be on cuda:{self.index}")
         out = q.new_empty((tokens, q_heads, width))
-        size = self._lib.cozyq_cache_attend_workspace_bytes(tokens, q_heads, requests, heads, page, width, columns, most)
+        size = self._lib.cozyq_cache_attend_workspace_bytes(tokens, q_heads, requests, heads, page, width, columns, most, window)
         work = q.new_empty(size // 2) if size > 0 else None
         code = self._lib.cozyq_cache_attend(
             self.index, fp8, q.data_ptr(), half, tokens, q_heads, q_token, q_head, k_codes, v_codes, k_scale, v_scale,

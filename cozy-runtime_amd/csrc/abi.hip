@@ -803,9 +803,10 @@ static bool attend_shape(int64_t tokens, int q_heads, int requests, int table_wi
 }
 
 int64_t cozyq_cache_attend_workspace_bytes(int64_t tokens, int q_heads, int requests, int heads, int page, int width,
-                                           int table_width, int64_t most) {
-    if (!attend_shape(tokens, q_heads, requests, table_width, 1, heads, page, width) || most < 0) return -1;
-    return cozyq::cache_attend_work(tokens, q_heads / heads, requests, heads, table_width, page, width, most);
+                                           int table_width, int64_t most, int window) {
+    if (!attend_shape(tokens, q_heads, requests, table_width, 1, heads, page, width) || most < 0 || window < 0)
+        return -1;
+    return cozyq::cache_attend_work(tokens, q_heads / heads, requests, heads, table_width, page, width, most, window);
 }
 
 int cozyq_cache_attend(int device, int fp8, const void* q, int half, int64_t tokens, int q_heads, int64_t q_token,
@@ -821,7 +822,7 @@ int cozyq_cache_attend(int device, int fp8, const void* q, int half, int64_t tok
         !aligned16(v_codes) || !k_scale || !v_scale || !table || !starts || !lengths || !out || !aligned16(out) ||
         !aligned16(workspace))
         return hipErrorInvalidValue;
-    if (!workspace && cozyq_cache_attend_workspace_bytes(tokens, q_heads, requests, heads, page, width, table_width, most))
+    if (!workspace && cozyq_cache_attend_workspace_bytes(tokens, q_heads, requests, heads, page, width, table_width, most, window))
         return hipErrorInvalidValue;
     const OnDevice guard(device);
     if (guard.error() != hipSuccess) return guard.error();

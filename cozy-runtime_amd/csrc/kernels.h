@@ -385,7 +385,7 @@ struct CacheAttend {
     bool half, causal;
     float* work;  // cache_attend_work bytes
 };
-int64_t cache_attend_work(int64_t tokens, int group, int requests, int heads, int columns, int page, int width, int64_t most);
+int64_t cache_attend_work(int64_t tokens, int group, int requests, int heads, int columns, int page, int width, int64_t most, int window);
 hipError_t cache_attend(const CacheAttend& p, int64_t most, bool fp8, hipStream_t s);
 
 }  // namespace cozyq

@@ -1156,24 +1156,39 @@ constexpr int kManySteps = 16;    // many_kernel's, whose parts are larger
 constexpr int kCutSteps = 64;     // with more, and a CU to a workgroup, many_kernel chooses among kCuts
 constexpr int64_t kJoinGroups = 1024;  // join_kernel's workgroups for each of the two launches
 constexpr int kFewRows = 64;      // up to here a request's rows are few_kernel's alone,
-constexpr int kFewAllRows = 1024; // and so are all, up to here: one launch less (60 tokens of 8 requests 48 -> 31 us)
+constexpr int kFewWork = 24000;   // and so are all, up to so much work (`few_work`): one launch less
 constexpr int kBesideRows = 16;   // up to here they are few_kernel's beside requests of more,
 constexpr int kManyRows = 1024;   // unless so many a request on average leave few such requests
 
+// What the few rows' kernel has to do, in rows of a key head: twice as much at width 256, where a CU holds one
+// workgroup and not two; where tiles are split, times the root of a row's steps (at the most kLongSteps, as a
+// table may be much wider than the requests are long), since the many rows' kernel then costs its join and parts first
+// and codes made f16 once for 256 rows later. Timed over 730 steps of 128 to 12000 rows, 200 to 20000 tokens held, 1
+// to 30 requests and six head layouts, it takes 1.011 of the faster side's time (geometric mean; a
+// limit of 1024 rows for all 1.115). Few / many rows' kernel, us, 32 heads over 8 of width 128: 100 tokens over 300
+// 14 / 23, over 2500 41 / 43, over 7000 55 / 50, over 20000 101 / 68; 250 over 7000 86 / 60; 500 over 300 24 / 35, over
+// 7000 159 / 92; 1750 tokens of 8 requests over 200 54 / 31; 16 heads over 2 of 256: 125 over 2500 68 / 59, over 300 28 / 34.
+constexpr int64_t kLongSteps = 128;
+float few_work(int64_t all_rows, int heads, int width, int64_t steps) {
+    const float rows = static_cast<float>(all_rows) * static_cast<float>(heads) * (width == 256 ? 2.0f : 1.0f);
+    return steps > kWholeSteps ? rows * sqrtf(static_cast<float>(min(steps, kLongSteps))) : rows;
+}
+
 // The shape of a call, which its workspace goes by too. Where a request may have more than kFewRows
 // rows, those of more than kBesideRows go to many_kernel and the others, if there are others, to few_kernel.
-// (With kFewAllRows at 2048 chunks of 300 tokens among 8 requests took 70 us for 57; with kManyRows at 256
-// the chunks of 2311 tokens among 12 took 99 for 87, as their single tokens then run a wave a workgroup.)
-AttendShape shape_of(int64_t tokens, int group, int requests, int heads, int columns, int page, int width, int64_t most) {
+// (With kManyRows at 256 the chunks of 2311 tokens among 12 requests took 99 us for 87, as their single tokens then
+// run a wave a workgroup.)
+AttendShape shape_of(int64_t tokens, int group, int requests, int heads, int columns, int page, int width, int64_t most, int window) {
     const int64_t rows = (most > 0 && most < tokens ? most : tokens) * group;
     const int all = 0x7fffffff;
     AttendShape a = {};
     const int64_t all_rows = tokens * group;
-    a.many.on = rows > kFewRows && all_rows > kFewAllRows;
+    const int64_t steps = (static_cast<int64_t>(columns) * page + kStep - 1) / kStep;  // of a tile, at the most
+    const int64_t seen = window > 0 ? min(steps, static_cast<int64_t>(window) / kStep + 2) : steps;  // by a row, about
+    a.many.on = rows > kFewRows && few_work(all_rows, heads, width, seen) > kFewWork;
     a.few.on = !a.many.on || (requests > 1 && all_rows < kManyRows * requests);
     a.few.rows = rows > 16 && !a.many.on ? 32 : 16;
     a.few.upto = a.many.on ? kBesideRows : all;
-    const int64_t steps = (static_cast<int64_t>(columns) * page + kStep - 1) / kStep;  // of a tile, at the most
     a.few.tiles = a.many.on ? requests : (tokens * group + a.few.rows - 1) / a.few.rows + requests - 1;
     if (steps <= kWholeSteps) {
         a.few.least = kWholeSteps;
@@ -1245,12 +1260,12 @@ hipError_t attend(const CacheAttend& p, const AttendShape& a, hipStream_t s) {
 
 }  // namespace
 
-int64_t cache_attend_work(int64_t tokens, int group, int requests, int heads, int columns, int page, int width, int64_t most) {
-    return 4 * shape_of(tokens, group, requests, heads, columns, page, width, most).floats;
+int64_t cache_attend_work(int64_t tokens, int group, int requests, int heads, int columns, int page, int width, int64_t most, int window) {
+    return 4 * shape_of(tokens, group, requests, heads, columns, page, width, most, window).floats;
 }
 
 hipError_t cache_attend(const CacheAttend& p, int64_t most, bool fp8, hipStream_t s) {
-    const AttendShape a = shape_of(p.tokens, p.group, p.requests, p.heads, p.width, p.page, p.head_width, most);
+    const AttendShape a = shape_of(p.tokens, p.group, p.requests, p.heads, p.width, p.page, p.head_width, most, p.window);
     return fp8 ? attend<true>(p, a, s) : attend<false>(p, a, s);
 }
 

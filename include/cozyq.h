@@ -550,7 +550,7 @@ int cozyq_cache_read(int device, int fp8, const void* k_codes, const void* v_cod
  * cozyq_cache_attend_workspace_bytes bytes, uninitialised (NULL where that is 0; -1 for a bad
  * argument). */
 int64_t cozyq_cache_attend_workspace_bytes(int64_t tokens, int q_heads, int requests, int heads, int page, int width,
-                                           int table_width, int64_t most);
+                                           int table_width, int64_t most, int window);
 int cozyq_cache_attend(int device, int fp8, const void* q, int half, int64_t tokens, int q_heads, int64_t q_token,
                        int64_t q_head, const void* k_codes, const void* v_codes, const float* k_scale,
                        const float* v_scale, int pages, int heads, int page, int width, const int* table,

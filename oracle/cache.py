@@ -123,11 +123,9 @@ def attend(q, k, v, table, starts, lengths, page: int, scale=None, causal=True, 
                 seen &= at > position - window
             if not seen.any():
                 continue
-            for h in range(q_heads):
-                g = h // (q_heads // heads)
-                score = kk[g, seen] @ q[t, h].double() * scale
-                p = (score - score.max()).exp() if not score.isnan().any() else score * math.nan
-                p = p / p.sum()
-                out[t, h] = p @ vv[g, seen]
-                size[t, h] = p @ vv[g, seen].abs()
+            score = q[t].double().view(heads, -1, width) @ kk[:, seen].transpose(1, 2) * scale
+            p = (score - score.amax(-1, keepdim=True)).exp()
+            p = torch.where(score.isnan().any(-1, keepdim=True), math.nan, p / p.sum(-1, keepdim=True))
+            out[t] = (p @ vv[:, seen]).view(q_heads, width)
+            size[t] = (p @ vv[:, seen].abs()).view(q_heads, width)
     return out, size

@@ -119,8 +119,8 @@ def test_entries_refuse_bad_arguments_before_the_device():
                 dict(width=80), dict(table=None), dict(requests=0), dict(requests=4001), dict(columns=0), dict(most=-1),
                 dict(window=-1), dict(causal=0, window=4), dict(out=None), dict(out=p + 4), dict(tokens=-1)):  # fmt: skip
         assert attend(**bad) == INVALID, bad
-    assert lib.cozyq_cache_attend_workspace_bytes(1, 3, 1, 2, 16, 64, 4, 1) == -1
-    assert lib.cozyq_cache_attend_workspace_bytes(1, 2, 1, 2, 16, 64, 4, 1) >= 0
+    assert lib.cozyq_cache_attend_workspace_bytes(1, 3, 1, 2, 16, 64, 4, 1, 0) == -1
+    assert lib.cozyq_cache_attend_workspace_bytes(1, 2, 1, 2, 16, 64, 4, 1, 0) >= 0
     del keep
 
 

@@ -425,14 +425,14 @@ def test_attend_pages_of_very_different_scales(kv, new, codes):
     check_attend(kv, [700, 1300], new, 16, 4, 2, 64, codes, torch.float16, spread=12, scale=2.0**-14)
 
 
-#: Steps of more than 1024 rows, which the kernel for many rows takes: a whole tile and parts of one, a request
-#: of one token beside, contexts past the steps that one workgroup takes, none at all.
-MANY = [([1500, 40, 3], [150, 1, 33]), ([0, 2100, 17], [260, 1, 0]), ([700], [129])]
+#: Steps of so many rows over so many heads that the kernel for many rows takes them: a whole tile and parts of
+#: one, a request of one token beside, contexts past the steps that one workgroup takes, none at all.
+MANY = [([1500, 40, 3], [150, 1, 33]), ([0, 2100, 17], [260, 1, 0]), ([1200], [201])]
 
 
 @BOTH
 @pytest.mark.parametrize("page,dtype", [(16, torch.float16), (64, torch.bfloat16), (256, torch.bfloat16)], ids=["16", "64", "256"])
-@pytest.mark.parametrize("q_heads,heads,width", [(16, 2, 64), (8, 1, 128), (8, 1, 256), (11, 1, 128)])
+@pytest.mark.parametrize("q_heads,heads,width", [(32, 4, 64), (32, 4, 128), (32, 4, 256), (33, 3, 128)])
 @pytest.mark.parametrize("held,new", MANY, ids=["beside", "begins", "alone"])
 def test_attend_many_rows(kv, held, new, q_heads, heads, width, page, dtype, codes):
     check_attend(kv, [h + n for h, n in zip(held, new)], new, page, q_heads, heads, width, codes, dtype, tokens=sum(new) + 3)
@@ -442,32 +442,32 @@ def test_attend_many_rows(kv, held, new, q_heads, heads, width, page, dtype, cod
 @pytest.mark.parametrize("width", [64, 128])
 def test_attend_many_rows_with_a_window(kv, width, window):
     held, new = [1500, 40, 3], [150, 1, 33]
-    check_attend(kv, [h + n for h, n in zip(held, new)], new, 32, 8, 1, width, torch.int8, torch.bfloat16, window=window)
+    check_attend(kv, [h + n for h, n in zip(held, new)], new, 32, 32, 4, width, torch.int8, torch.bfloat16, window=window)
 
 
 @BOTH
 def test_attend_many_rows_of_all_tokens_and_of_very_different_scales(kv, codes):
     lengths, new = [400, 0, 1300], [140, 2, 5]
-    got = check_attend(kv, lengths, new, 32, 8, 1, 64, codes, torch.bfloat16, causal=False)
+    got = check_attend(kv, lengths, new, 32, 48, 6, 64, codes, torch.bfloat16, causal=False)
     assert (got[140:142] == 0).all()
-    check_attend(kv, [700, 1300], [66, 140], 16, 8, 1, 128, codes, torch.float16, spread=12, scale=2.0**-14)
+    check_attend(kv, [700, 1300], [66, 140], 16, 32, 4, 128, codes, torch.float16, spread=12, scale=2.0**-14)
 
 
 @BOTH
 @pytest.mark.parametrize("width", [64, 128, 256])
 def test_attend_many_rows_over_missing_and_not_finite_pages(kv, width, codes):
     lengths, new, page = [1250, 90], [160, 1], 16
-    cache, table, value = filled(kv, lengths, page, 1, width, codes, 13)
+    cache, table, value = filled(kv, lengths, page, 5, width, codes, 13)
     for index in (3, 5, 11, 74):
         table[0][index] = (-1, 10**6, -7, -1)[index % 4]
     for index, bad in ((70, math.nan), (71, math.inf)):  # tokens 1120 .. 1151
-        cache.v_scale[table[0][index], 0] = bad
-        cache.k_scale[table[0][index + 2], 0] = bad  # 1152 .. 1183
+        cache.v_scale[table[0][index]] = bad
+        cache.k_scale[table[0][index + 2]] = bad  # 1152 .. 1183
     plan, starts, tokens = make_plan(kv, table, lengths, new, page, 160)
-    q = torch.randn(tokens, 8, width, generator=torch.Generator().manual_seed(14)).bfloat16()
+    q = torch.randn(tokens, 40, width, generator=torch.Generator().manual_seed(14)).bfloat16()
     got = cache.attend(torch, q.to(DEV), plan).cpu()
     want, size = law.attend(q, value[0], value[1], table, starts, lengths, page)
-    sees = torch.zeros(tokens, 8, dtype=torch.bool)
+    sees = torch.zeros(tokens, 40, dtype=torch.bool)
     sees[30:160] = True  # request 0's rows from position 1120 on
     assert torch.equal(got.isnan().all(-1), sees) and torch.equal(got.isnan().any(-1), sees)
     error = (got.double() - want).abs()
@@ -481,9 +481,9 @@ def test_attend_many_rows_over_missing_and_not_finite_pages(kv, width, codes):
 
 def test_attend_many_rows_is_the_same_every_time_and_in_a_graph(kv):
     lengths, new = [3000, 5, 900], [200, 1, 1]
-    cache, table, _ = filled(kv, lengths, 64, 1, 128, torch.int8, 31)
+    cache, table, _ = filled(kv, lengths, 64, 4, 128, torch.int8, 31)
     plan, _, tokens = make_plan(kv, table, lengths, new, 64, 200)
-    q = torch.randn(tokens, 8, 128, generator=torch.Generator().manual_seed(32)).bfloat16().to(DEV)
+    q = torch.randn(tokens, 32, 128, generator=torch.Generator().manual_seed(32)).bfloat16().to(DEV)
     first = cache.attend(torch, q, plan)
     graph = torch.cuda.CUDAGraph()
     torch.cuda.synchronize()
