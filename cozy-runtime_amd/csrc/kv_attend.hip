@@ -1166,8 +1166,8 @@ constexpr int kManyRows = 1024;   // unless so many a request on average leave f
 // and codes made f16 once for 256 rows later. Timed over 730 steps of 128 to 12000 rows, 200 to 20000 tokens held, 1
 // to 30 requests and six head layouts, it takes 1.011 of the faster side's time (geometric mean; a
 // limit of 1024 rows for all 1.115). Few / many rows' kernel, us, 32 heads over 8 of width 128: 100 tokens over 300
-// 14 / 23, over 2500 41 / 43, over 7000 55 / 50, over 20000 101 / 68; 250 over 7000 86 / 60; 500 over 300 24 / 35, over
-// 7000 159 / 92; 1750 tokens of 8 requests over 200 54 / 31; 16 heads over 2 of 256: 125 over 2500 68 / 59, over 300 28 / 34.
+// 14 / 23, over 2500 41 / 43, over 7000 55 / 50, over 20000 101 / 68; 256 over 7000 86 / 60; 500 over 300 24 / 35, over
+// 7000 159 / 92; 1750 tokens of 8 requests over 200 54 / 31; 16 heads over 2 of 256: 128 over 2500 68 / 59, over 300 28 / 34.
 constexpr int64_t kLongSteps = 128;
 float few_work(int64_t all_rows, int heads, int width, int64_t steps) {
     const float rows = static_cast<float>(all_rows) * static_cast<float>(heads) * (width == 256 ? 2.0f : 1.0f);
