@@ -125,9 +125,10 @@ def main() -> None:
     torch.cuda.synchronize()
     print(f"prompts: {sum(lengths)} tokens of {args.requests} requests through {args.layers} layers")
     x, y, graph = server.recorded_step()
-    torch.cuda.synchronize()
-    began = time.perf_counter()
-    for _ in range(args.steps):
+    for step in range(args.steps + 1):
+        if step == 1:  # the first one loads the norm's kernel and the graph
+            torch.cuda.synchronize()
+            began = time.perf_counter()
         graph.replay()
         x.copy_(torch.nn.functional.rms_norm(y, (server.hidden,)))
     torch.cuda.synchronize()
