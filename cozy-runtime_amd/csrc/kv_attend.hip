@@ -202,14 +202,15 @@ __device__ int steps_a_share(const CacheAttend& p, const Part& part, Extent& e0)
     return __builtin_amdgcn_readfirstlane(best);
 }
 
-// Finds workgroup `id`'s share (kById), or the first of split row tile number `id`; false past the last. A
-// request's last tile comes first: where causal it has the most to do. Every wave scans all requests, 64 at
+// Finds workgroup `id`'s share (kById), or the first of split row tile number `id`; false past the last, with
+// `count` how many there are. A request's last tile comes first: where causal it has the most to do. Every wave scans all requests, 64 at
 // a time.
 template <bool kById>
-__device__ bool find_share(const CacheAttend& p, const Part& part, int id, Share& out) {
+__device__ bool find_share(const CacheAttend& p, const Part& part, int id, Share& out, int& count) {
     const int lane = threadIdx.x & 63;
     Extent e0;
     const int c = steps_a_share(p, part, e0);
+    count = 0;
     if (!kById && c == 0x7fffffff) return false;  // nothing to join
     int ids_before = 0, places_before = 0;
     for (int base = 0; base < p.requests; base += 64) {
@@ -231,6 +232,7 @@ __device__ bool find_share(const CacheAttend& p, const Part& part, int id, Share
         ids_before += __builtin_amdgcn_readlane(ids, 63);
         places_before += __builtin_amdgcn_readlane(places, 63);
     }
+    count = ids_before;
     return false;
 }
 
@@ -313,18 +315,15 @@ __device__ bool find_item(const CacheAttend& p, const Part& part, const Survey& 
     return false;
 }
 
-// Rows of the step that no request has (past the last one's) are zeros: the workgroups past the last
-// share, one at the least, write them.
-__device__ void clear_rest(const CacheAttend& p, int width, int group, int groups) {
+// Rows of the step that no request has (before the first one's and past the last one's) are zeros: the
+// workgroups without a share write them, those from number `busy` on. There are `heads` at the least: a launch
+// has that many more than it can have shares.
+__device__ void clear_rest(const CacheAttend& p, int width, int busy) {
     const int64_t row = static_cast<int64_t>(p.q_heads) * width / 8;
-    const int64_t from = row_start(p, p.requests) * row, to = p.tokens * row;
-    for (int64_t i = from + static_cast<int64_t>(group) * blockDim.x + threadIdx.x; i < to; i += static_cast<int64_t>(groups) * blockDim.x)
-        reinterpret_cast<i32x4*>(p.out)[i] = i32x4{0, 0, 0, 0};
-}
-
-__device__ void clear_rest(const CacheAttend& p, int width) {
-    const int groups = min(static_cast<int>(gridDim.x), 256), mine = gridDim.x - 1 - blockIdx.x;
-    if (mine < groups) clear_rest(p, width, mine, groups);
+    const int64_t before = row_start(p, 0) * row, after = row_start(p, p.requests) * row, count = before + p.tokens * row - after;
+    const int64_t stride = static_cast<int64_t>(gridDim.x - busy) * blockDim.x;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x - busy) * blockDim.x + threadIdx.x; i < count; i += stride)
+        reinterpret_cast<i32x4*>(p.out)[i < before ? i : i - before + after] = i32x4{0, 0, 0, 0};
 }
 
 // Where a row tile's tokens lie: steps [begin, end) of the share; rows see tokens from low_least on and
@@ -419,7 +418,7 @@ __global__ __launch_bounds__(256, kWidth == 256 ? 1 : 2) void few_kernel(CacheAt
     const Survey sv = survey(p, part);
     const int64_t run_begin = static_cast<int64_t>(id) * sv.c;
     if (run_begin >= sv.total) {
-        if (clears) clear_rest(p, kWidth);
+        if (clears) clear_rest(p, kWidth, (sv.total + sv.c - 1) / sv.c * p.heads);
         return;
     }
     const int run_from = static_cast<int>(run_begin), run_to = static_cast<int>(min(run_begin + sv.c, static_cast<int64_t>(sv.total)));
@@ -715,8 +714,9 @@ __global__ __launch_bounds__(64 * kWaves, kWidth == 256 ? 1 : 2) void many_kerne
     const int col = lane & 31, h = lane >> 5;
     const int kv = blockIdx.x % p.heads, id = blockIdx.x / p.heads;
     Share share;
-    if (!find_share<true>(p, part, id, share)) {
-        if (clears) clear_rest(p, kWidth);
+    int shares;
+    if (!find_share<true>(p, part, id, share, shares)) {
+        if (clears) clear_rest(p, kWidth, shares * p.heads);
         return;
     }
     const int first = row_start(p, share.request), fresh = row_start(p, share.request + 1) - first;
@@ -1080,7 +1080,8 @@ __global__ __launch_bounds__(256) void join_kernel(CacheAttend p, Part few, Part
         Parts parts;
         if (wide) {
             Share share;
-            if (!find_share<false>(p, part, id, share)) return;
+            int count;
+            if (!find_share<false>(p, part, id, share, count)) return;
             request = share.request;
             tile = share.tile;
             parts = {part.work + share.place * place_floats, part.work + share.place * place_floats, place_floats, share.splits};

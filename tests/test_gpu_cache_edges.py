@@ -1,0 +1,112 @@
+"""GPU tests of the paged cache where rows, plans and requests do not fit one another: steps of more rows than
+the requests bring.
+
+Bars as in test_gpu_kv_cache.py: the output's one rounding, and of Σ p·|v| the weights' 2^-11 and the exponents'
+2^-12."""
+
+from __future__ import annotations
+
+import math
+import random
+
+import pytest
+import torch
+
+from test_gpu_kv_cache import DEV, E4M3, UNIT, filled, ints, kv, make_plan  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+def expected(q, value, table, starts, lengths, page, causal=True, window=0):
+    """float64 on the GPU, a request at a time: (out, Σ p·|v|). A request's rows are its last tokens."""
+    tokens, q_heads, width = q.shape
+    heads = value.shape[2]
+    group = q_heads // heads
+    out = torch.zeros(tokens, q_heads, width, dtype=torch.float64, device=DEV)
+    size = torch.zeros_like(out)
+    for r, length in enumerate(lengths):
+        first, last = starts[r], min(starts[r + 1], tokens)
+        if last <= first or length <= 0:
+            continue
+        numbers = torch.tensor(table[r][: -(-length // page)])
+        k, v = (x[numbers].to(DEV).double().transpose(0, 1).reshape(heads, -1, width)[:, :length] for x in value)
+        position = length - (starts[r + 1] - first) + torch.arange(last - first, device=DEV)
+        at = torch.arange(length, device=DEV)
+        hidden = torch.zeros(last - first, length, dtype=torch.bool, device=DEV)
+        if causal:
+            hidden |= at > position[:, None]
+        if window:
+            hidden |= at <= position[:, None] - window
+        for h in range(heads):
+            mine = slice(h * group, (h + 1) * group)
+            x = q[first:last, mine].to(DEV).double().reshape(-1, width)
+            score = (x @ k[h].T.contiguous() * width**-0.5).view(last - first, group, length)
+            p = score.masked_fill(hidden[:, None], -math.inf).softmax(-1).nan_to_num(0.0).view(-1, length)
+            out[first:last, mine] = (p @ v[h]).view(last - first, group, width)
+            size[first:last, mine] = (p @ v[h].abs()).view(last - first, group, width)
+    return out, size
+
+
+def over_nan(cache, q, plan, **how):
+    """attend's result, in memory that held NaN before the call."""
+    torch.cuda.empty_cache()
+    junk = [torch.full(q.shape, math.nan, dtype=q.dtype, device=DEV) for _ in range(4)]
+    where = {x.data_ptr() for x in junk}
+    del junk
+    out = cache.attend(torch, q, plan, **how)
+    assert out.data_ptr() in where
+    return out
+
+
+def check(kv, lengths, new, page, q_heads, heads, width, codes, dtype, tokens, lead=0, most=None, columns=0, window=0,
+          causal=True):  # fmt: skip
+    """Every row against the formula; rows of no request, `lead` of them before the first request's, are 0."""
+    seed = sum(lengths) + 31 * sum(new) + page + width
+    cache, table, value = filled(kv, lengths, page, heads, width, codes, seed)
+    table = [row + [-1] * (columns - len(row)) for row in table]
+    plan, starts, _ = make_plan(kv, table, lengths, new, page, max(new) if most is None else most)
+    starts = [lead + s for s in starts]
+    plan.starts = ints(starts)
+    q = torch.randn(tokens, q_heads, width, generator=torch.Generator().manual_seed(seed)).to(dtype).to(DEV)
+    got = over_nan(cache, q, plan, window=window, causal=causal)
+    assert (got[:lead] == 0).all() and (got[starts[-1] :] == 0).all()
+    want, size = expected(q, value, table, starts, lengths, page, causal, window)
+    bar = UNIT[dtype] * want.abs() + (2.0**-11 + 2.0**-12) * size + (2.0**-25 if dtype is torch.float16 else 0)
+    assert ((got.double() - want).abs() <= bar).all()
+
+
+# ------------------------------------------------------------------- rows of no request
+
+#: Decode steps of a fixed number of rows of which some requests are gone, and prompts shorter than their step.
+PADDED = {
+    "40 of 64, long": dict(lengths=[200 + 17 * i for i in range(40)], new=[1] * 40, tokens=64, columns=40, most=1),
+    "1 of 8, long": dict(lengths=[30000], new=[1], tokens=8, most=1),
+    "1 of 64, long": dict(lengths=[30000], new=[1], tokens=64, most=1),
+    "32 of 64": dict(lengths=[4000] * 32, new=[1] * 32, tokens=64, columns=100, most=1),
+    "8 of 64, a short table": dict(lengths=[200], new=[8], tokens=64, columns=4, most=0),
+    "574 of 704, many rows": dict(lengths=[3774], new=[574], tokens=704),
+    "300 of 2000, many rows": dict(lengths=[3000, 70, 900], new=[100, 1, 199], tokens=2000),
+    "none of 700": dict(lengths=[500, 90], new=[0, 0], tokens=700, most=0),
+}
+
+
+@pytest.mark.parametrize("codes", [torch.int8, E4M3], ids=["int8", "fp8"])
+@pytest.mark.parametrize("lead", [0, 37])
+@pytest.mark.parametrize("step", list(PADDED), ids=list(PADDED))
+def test_rows_of_no_request_are_zero(kv, step, lead, codes):  # noqa: F811
+    how = dict(PADDED[step])
+    how["tokens"] += lead
+    check(kv, page=64, q_heads=32, heads=8, width=64, codes=codes, dtype=torch.bfloat16, lead=lead, **how)
+
+
+@pytest.mark.parametrize("seed", range(24))
+def test_rows_of_no_request_are_zero_in_drawn_steps(kv, seed):  # noqa: F811
+    rng = random.Random(seed)
+    q_heads, heads, width = rng.choice(((32, 8, 128), (16, 16, 64), (28, 4, 128), (64, 8, 128), (16, 2, 256), (8, 1, 64)))
+    requests = rng.choice((1, 2, 7, 30, 70))
+    held = [rng.randrange(1, 40000 // requests) for _ in range(requests)]
+    new = [rng.choice((0, 1, 1, 1, 4)) for _ in held] if rng.random() < 0.6 else [rng.randrange(400 // requests + 2) for _ in held]
+    page, lead = rng.choice((16, 64, 256)), rng.choice((0, 0, 1, 90))
+    check(kv, [h + n for h, n in zip(held, new)], new, page, q_heads, heads, width, rng.choice((torch.int8, E4M3)),
+          rng.choice((torch.bfloat16, torch.float16)), lead + sum(new) + rng.choice((1, 9, 60, 700)), lead,
+          rng.choice((None, 0)), columns=rng.choice((0, 600)), window=rng.choice((0, 0, 300)))  # fmt: skip
