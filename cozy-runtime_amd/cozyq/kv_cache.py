@@ -130,6 +130,8 @@ class PagedCache:
         `heads.norm_rope` takes them) over their requests' pages, `[T, q_heads, D]` in q's type: query
         head h reads key head h // (q_heads / heads). Row t sees its request's tokens up to its own
         position, with a `window` the last `window` of them; without `causal`, all of them. `scale`
-        multiplies the scores (None: D^-1/2). A row that sees nothing, or belongs to no request, is 0."""
+        multiplies the scores (None: D^-1/2). A row that sees nothing, or belongs to no request, is 0. A plan
+        put together without its rows' slots (an empty tensor) goes by `starts`: q may then have fewer rows than
+        that speaks of, or more."""
         index = _dispatch.card(OP, q)
         return _dispatch.library(index).cache_attend(self, q, plan, scale, causal, window)

@@ -1235,8 +1235,9 @@ class Prebuilt:
         requests, columns = table.shape
         starts_at = self._ints("attend", "starts", starts, requests + 1)
         lengths_at = self._ints("attend", "lengths", lengths, requests)
-        if plan.page != page:
-            raise ValueError(f"attend: the plan has pages of {plan.page} tokens, the cache of {page}")
+        rows = plan.slots.shape[0]
+        if plan.page != page or (rows != tokens and rows):
+            raise ValueError(f"attend: the plan is of {rows} rows in pages of {plan.page}, not of {tokens} in pages of {page}")
         if window < 0 or (window and not causal):
             raise ValueError(f"attend: a window of {window} tokens{'' if causal else ' without causal'}")
         if self._elsewhere((cache.k, cache.v, cache.k_scale, cache.v_scale, q, table, starts, lengths)):

@@ -81,6 +81,18 @@ __device__ __forceinline__ void store_row(const CacheAttend& p, int token, int h
 // Where request r's rows begin, never past the step's.
 __device__ __forceinline__ int row_start(const CacheAttend& p, int r) { return min(max(p.starts[r], 0), p.tokens); }
 
+// Request r in the step: its first row, how many of its rows the step has, the tokens before the first of them, and
+// its tokens in all. A step that ends before a request's rows do cuts the last ones off: those before stay where
+// they are.
+struct Rows {
+    int first, fresh, before, length;
+};
+
+__device__ __forceinline__ Rows rows_of(const CacheAttend& p, int r) {
+    const int first = row_start(p, r), end = max(p.starts[r + 1], first), length = max(p.lengths[r], 0);
+    return {first, min(end, p.tokens) - first, length - (end - first), length};
+}
+
 // x from the lane that DPP control kCtrl names, 0 where it names none or the row is masked out.
 template <int kCtrl, int kRowMask, typename T>
 __device__ __forceinline__ T dpp_or_zero(T x) {
@@ -129,10 +141,11 @@ struct Extent {
 };
 
 __device__ __forceinline__ Extent extent(const CacheAttend& p, const Part& part, int r) {
-    const int fresh = row_start(p, r + 1) - row_start(p, r), length = p.lengths[r], rows = fresh * p.group;
+    const Rows own = rows_of(p, r);
+    const int rows = own.fresh * p.group;
     if (rows <= part.over || rows > part.upto) return {0, 0};
-    const int low = p.window > 0 ? max(0, length - fresh + 1 - p.window) : 0;
-    const int held = min(max(length, 0), p.width << p.shift);  // what the table's row has pages for
+    const int low = p.window > 0 ? max(0, own.before + 1 - p.window) : 0;
+    const int held = min(own.length, p.width << p.shift);  // what the table's row has pages for
     const int steps = (held + kStep - 1) / kStep - low / kStep;
     return {(rows + (1 << part.shift) - 1) >> part.shift, max(steps, 0)};
 }
@@ -332,8 +345,8 @@ struct Span {
     int begin, end, low_least, low_most, high_least, high_most;
 };
 
-__device__ __forceinline__ Span span_of(const CacheAttend& p, int row0, int rows, int fresh, int length, int split = 0, int splits = 1) {
-    const int before = length - fresh, t0 = row0 / p.group, t1 = (rows - 1) / p.group;
+__device__ __forceinline__ Span span_of(const CacheAttend& p, int row0, int rows, const Rows& own, int split = 0, int splits = 1) {
+    const int before = own.before, length = own.length, t0 = row0 / p.group, t1 = (rows - 1) / p.group;
     Span s;
     s.low_least = p.window > 0 ? max(0, before + t0 + 1 - p.window) : 0;
     s.low_most = p.window > 0 ? max(0, before + t1 + 1 - p.window) : 0;
@@ -429,8 +442,8 @@ __global__ __launch_bounds__(256, kWidth == 256 ? 1 : 2) void few_kernel(CacheAt
 
     Item item;
     for (int at = run_from; at < run_to && find_item<true>(p, part, sv, at, item);) {
-        const int first = row_start(p, item.request), fresh = row_start(p, item.request + 1) - first;
-        const int length = p.lengths[item.request], rows = fresh * p.group;
+        const Rows own = rows_of(p, item.request);
+        const int first = own.first, length = own.length, rows = own.fresh * p.group;
         const int stop = min(item.start + item.units, run_to);
         const bool split = item.start < run_from || item.start + item.units > run_to;
         const int place = 2 * id + (at != run_from);
@@ -444,7 +457,7 @@ __global__ __launch_bounds__(256, kWidth == 256 ? 1 : 2) void few_kernel(CacheAt
             const bool live = row < rows;
             token[n] = live ? row / p.group : 0;
             head[n] = kv * p.group + (live ? row - token[n] * p.group : 0);
-            const int position = length - fresh + token[n];
+            const int position = own.before + token[n];
             high[n] = live ? max(p.causal ? position + 1 : length, 0) : 0;
             low[n] = live && p.window > 0 ? max(0, position + 1 - p.window) : 0;
         }
@@ -461,8 +474,8 @@ __global__ __launch_bounds__(256, kWidth == 256 ? 1 : 2) void few_kernel(CacheAt
             }
         };
         if constexpr (kTiles == 1) read_rows();
-        const Span span = span_of(p, kRows * item.tile, min(rows, kRows * (item.tile + 1)), fresh, length);
-        const int base = (p.window > 0 ? max(0, length - fresh + 1 - p.window) : 0) / kStep;
+        const Span span = span_of(p, kRows * item.tile, min(rows, kRows * (item.tile + 1)), own);
+        const int base = (p.window > 0 ? max(0, own.before + 1 - p.window) : 0) / kStep;
         const int begin = max(span.begin, base + ((at - item.start) << sv.shift));
         const int end = stop == item.start + item.units ? span.end : min(span.end, base + ((stop - item.start) << sv.shift));
         const int* table = p.table + static_cast<int64_t>(item.request) * p.width;
@@ -719,16 +732,16 @@ __global__ __launch_bounds__(64 * kWaves, kWidth == 256 ? 1 : 2) void many_kerne
         if (clears) clear_rest(p, kWidth, shares * p.heads);
         return;
     }
-    const int first = row_start(p, share.request), fresh = row_start(p, share.request + 1) - first;
-    const int length = p.lengths[share.request], rows = fresh * p.group;
+    const Rows of = rows_of(p, share.request);
+    const int first = of.first, length = of.length, rows = of.fresh * p.group;
     const int row0 = kRows * share.tile, mine0 = row0 + 32 * wave, row = mine0 + col;
-    const Span span = span_of(p, row0, min(rows, row0 + kRows), fresh, length, share.split, share.splits);
+    const Span span = span_of(p, row0, min(rows, row0 + kRows), of, share.split, share.splits);
     // The wave's own rows; one without rows only helps to load.
     const bool busy = mine0 < rows;
-    const Span own = span_of(p, busy ? mine0 : 0, min(rows, mine0 + 32), fresh, length);
+    const Span own = span_of(p, busy ? mine0 : 0, min(rows, mine0 + 32), of);
     const bool live = row < rows;
     const int token = live ? row / p.group : 0, head = kv * p.group + (live ? row - token * p.group : 0);
-    const int position = length - fresh + token;
+    const int position = of.before + token;
     const int high = live ? max(p.causal ? position + 1 : length, 0) : 0;
     const int low = live && p.window > 0 ? max(0, position + 1 - p.window) : 0;
 
@@ -1095,7 +1108,8 @@ __global__ __launch_bounds__(256) void join_kernel(CacheAttend p, Part few, Part
                      2 * place_floats, last - run + 1};
         }
         if (parts.count == 1) continue;
-        const int first = row_start(p, request), rows = (row_start(p, request + 1) - first) * p.group;
+        const Rows own = rows_of(p, request);
+        const int first = own.first, rows = own.fresh * p.group;
         const int row0 = tile << part.shift, count = min(rows_all, rows - row0);
         for (int r = wide ? group * kParts + slice : group; r < count; r += wide ? groups * kParts : groups) {
             const int64_t at = (static_cast<int64_t>(kv) * rows_all + r) * row_floats;

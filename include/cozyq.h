@@ -541,14 +541,14 @@ int cozyq_cache_read(int device, int fp8, const void* k_codes, const void* v_cod
 
 /* Attention over the cache: q [tokens, q_heads, width] (16-bit, strides as above), query heads in equal
  * groups of up to 64 a key head; request r's rows are starts[r] .. starts[r + 1] − 1, its last tokens of
- * lengths[r]. out [tokens, q_heads, width], contiguous, in q's type: softmax(scale · q·k) · v over the
- * tokens that the row sees: causal, those up to its own, with a window > 0 the last `window` of them;
- * otherwise all of the request's. Tokens whose table entry is no page of the cache are not seen; a row
- * that sees none, or belongs to no request, is 0. What pages hold past a request's tokens is not read
- * into any result. `most`: the most rows a request has, as far as the caller knows (0: not at all); it
- * sets the launch's shape and speed, never its results. The workspace is of
- * cozyq_cache_attend_workspace_bytes bytes, uninitialised (NULL where that is 0; -1 for a bad
- * argument). */
+ * lengths[r] (rows past the step's `tokens` are cut off; those before keep their positions). out [tokens,
+ * q_heads, width], contiguous, in q's type: softmax(scale · q·k) · v over the tokens that the row sees:
+ * causal, those up to its own, with a window > 0 the last `window` of them; otherwise all of the request's.
+ * Tokens whose table entry is no page of the cache are not seen; a row that sees none, or belongs to no
+ * request, is 0. What pages hold past a request's tokens is not read into any result. `most`: the most rows
+ * a request has, as far as the caller knows (0: not at all); it sets the launch's shape and speed, never its
+ * results. The workspace is of cozyq_cache_attend_workspace_bytes bytes, uninitialised (NULL where that is 0;
+ * -1 for a bad argument). */
 int64_t cozyq_cache_attend_workspace_bytes(int64_t tokens, int q_heads, int requests, int heads, int page, int width,
                                            int table_width, int64_t most, int window);
 int cozyq_cache_attend(int device, int fp8, const void* q, int half, int64_t tokens, int q_heads, int64_t q_token,

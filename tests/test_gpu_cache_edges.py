@@ -1,5 +1,5 @@
 """GPU tests of the paged cache where rows, plans and requests do not fit one another: steps of more rows than
-the requests bring.
+the requests bring, queries of another number of rows than the plan's.
 
 Bars as in test_gpu_kv_cache.py: the output's one rounding, and of Σ p·|v| the weights' 2^-11 and the exponents'
 2^-12."""
@@ -110,3 +110,30 @@ def test_rows_of_no_request_are_zero_in_drawn_steps(kv, seed):  # noqa: F811
     check(kv, [h + n for h, n in zip(held, new)], new, page, q_heads, heads, width, rng.choice((torch.int8, E4M3)),
           rng.choice((torch.bfloat16, torch.float16)), lead + sum(new) + rng.choice((1, 9, 60, 700)), lead,
           rng.choice((None, 0)), columns=rng.choice((0, 600)), window=rng.choice((0, 0, 300)))  # fmt: skip
+
+
+# ------------------------------------------------------- queries of other rows than the plan's
+
+
+@pytest.mark.parametrize("new,tokens", [([5, 1, 9], 10), ([5, 1, 9], 3), ([40, 300], 200), ([40, 300], 17)],
+                         ids=["few", "few, first", "many", "many, first"])  # fmt: skip
+@pytest.mark.parametrize("window", [0, 50])
+def test_rows_past_the_queries_move_no_position(kv, new, tokens, window):  # noqa: F811
+    """A step cut short: the rows that are there see what they see in the whole step."""
+    lengths = [n + 60 * (i + 1) for i, n in enumerate(new)]
+    cache, table, value = filled(kv, lengths, 16, 4, 64, torch.int8, 5)
+    plan, starts, whole = make_plan(kv, table, lengths, new, 16, max(new))
+    q = torch.randn(whole, 32, 64, generator=torch.Generator().manual_seed(6)).bfloat16().to(DEV)
+    got = cache.attend(torch, q[:tokens], plan, window=window)
+    want, size = expected(q[:tokens], value, table, starts, lengths, 16, window=window)
+    assert ((got.double() - want).abs() <= 2.0**-8 * want.abs() + (2.0**-11 + 2.0**-12) * size).all()
+
+
+def test_queries_of_another_number_of_rows_are_refused(kv):  # noqa: F811
+    cache = kv.empty(torch, 4, 2, 64, page=16, device=DEV)
+    plan = kv.plan(torch, ints([[-1, -1]]), ints([0, 1]), ints([2]), ints([0]), ints([20]), tokens=20, page=16)
+    q = torch.zeros(21, 4, 64, dtype=torch.bfloat16, device=DEV)
+    for rows in (0, 1, 19, 21):
+        with pytest.raises(ValueError, match="20 rows"):
+            cache.attend(torch, q[:rows], plan)
+    assert cache.attend(torch, q[:20], plan).shape == (20, 4, 64)
