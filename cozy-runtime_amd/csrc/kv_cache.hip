@@ -144,12 +144,12 @@ __global__ __launch_bounds__(kThreads) void plan_kernel(CachePlan p) {
         if (r < R) p.lengths[r] = held_of[r] + starts[r + 1] - starts[r];
     }
     if (blockIdx.x == 0) {
-        // Pages wanted and not got: those past the free list's end, and those past a row of the table.
+        // Pages wanted and not got: of those that the step's tokens begin, tokens / page + R at the most, those past
+        // the free list's end and those past a row of the table.
         int past = 0;
         for (int r = threadIdx.x; r < R; r += kThreads) {
             const int held = held_of[r], n = starts[r + 1] - starts[r];
-            const int have = min((held + p.page - 1) >> p.shift, p.width);
-            past += ((held + n + p.page - 1) >> p.shift) - have;
+            past += ((held + n + p.page - 1) >> p.shift) - ((held + p.page - 1) >> p.shift);
         }
         for (int step = 1; step < 64; step *= 2) past += __shfl_xor(past, step);
         __syncthreads();

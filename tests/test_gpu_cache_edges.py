@@ -1,5 +1,6 @@
 """GPU tests of the paged cache where rows, plans and requests do not fit one another: steps of more rows than
-the requests bring, queries of another number of rows than the plan's.
+the requests bring, queries of another number of rows than the plan's, requests that hold more than their row of
+the table names.
 
 Bars as in test_gpu_kv_cache.py: the output's one rounding, and of Σ p·|v| the weights' 2^-11 and the exponents'
 2^-12."""
@@ -12,7 +13,7 @@ import random
 import pytest
 import torch
 
-from test_gpu_kv_cache import DEV, E4M3, UNIT, filled, ints, kv, make_plan  # noqa: F401
+from test_gpu_kv_cache import DEV, E4M3, UNIT, check_plan, filled, ints, kv, make_plan  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -137,3 +138,15 @@ def test_queries_of_another_number_of_rows_are_refused(kv):  # noqa: F811
         with pytest.raises(ValueError, match="20 rows"):
             cache.attend(torch, q[:rows], plan)
     assert cache.attend(torch, q[:20], plan).shape == (20, 4, 64)
+
+
+# ------------------------------------------------------------------------ a plan's last pages
+
+
+@pytest.mark.parametrize("held,new", [([40], [1]), ([40, 5], [0, 0]), ([32, 5, 70], [1, 12, 30]), ([47, 31, 0], [2, 2, 60]),
+                                      ([2**30 - 256] * 40, [1, 0, 16, 17] * 10)])  # fmt: skip
+@pytest.mark.parametrize("spare", [0, 1, 9])
+def test_pages_wanted_are_those_of_new_tokens(kv, held, new, spare):  # noqa: F811
+    """Requests that hold more than their row of the table names want a page where a new token begins one."""
+    table = [[2 * i, 2 * i + 1] if n >= 32 else [2 * i, -1] if n else [-1, -1] for i, n in enumerate(held)]
+    check_plan(kv, table, list(range(100, 109)), spare, held, new, sum(new) + 2, 16)
