@@ -19,12 +19,9 @@ constexpr int kWaves = kThreads / 64;
 
 // ------------------------------------------------------------------------------------ plan
 
-// min(a + b, top) for a, b <= top < 2^30: a sum that saturates, so that no request's count can
-// carry the prefix past the step's rows.
-__device__ __forceinline__ int capped(int a, int b, int top) {
-    const int sum = a + b;
-    return sum < top ? sum : top;
-}
+// min(a + b, top) for 0 <= a, b <= top, whatever top is: a sum that saturates, so that no request's count can
+// carry the prefix past the step's rows, of which there may be 2^30.
+__device__ __forceinline__ int capped(int a, int b, int top) { return a < top - b ? a + b : top; }
 
 // In place, the exclusive prefix sums of v[0, n) in shared memory, the whole sum in v[n]; sums
 // saturate at `top`. Called by the whole workgroup.

@@ -150,3 +150,15 @@ def test_pages_wanted_are_those_of_new_tokens(kv, held, new, spare):  # noqa: F8
     """Requests that hold more than their row of the table names want a page where a new token begins one."""
     table = [[2 * i, 2 * i + 1] if n >= 32 else [2 * i, -1] if n else [-1, -1] for i, n in enumerate(held)]
     check_plan(kv, table, list(range(100, 109)), spare, held, new, sum(new) + 2, 16)
+
+
+def test_plan_of_the_most_rows(kv):  # noqa: F811
+    """2^30 rows, the first two requests asking for more than there are: their counts add up past 31 bits."""
+    rows = 2**30
+    got = kv.plan(torch, ints([[-1, -1], [7, -1], [-1, -1]]), ints([3, 4]), ints([2]), ints([0, 9, 0]),
+                  ints([rows, 2**31 - 1, 5]), tokens=rows, page=16)  # fmt: skip
+    assert got.starts.tolist() == [0, rows, rows, rows] and got.lengths.tolist() == [rows, 9, 0]
+    assert got.runs[:3].tolist() == [[0, 16, 4, 0], [16, 16, 3, 0], [32, 16, -1, 0]] and got.table.tolist()[0] == [4, 3]
+    assert got.slots[:33].tolist() == [*range(64, 80), *range(48, 64), -1]
+    assert got.positions[-1].item() == rows - 1 and got.requests[-1].item() == 0
+    assert got.spare.tolist() == [0, rows // 16 - 2]
