@@ -115,6 +115,9 @@ def main() -> None:
         ask.add_argument(f"--{name}", type=int, default=value)
     ask.add_argument("--codes", choices=("int8", "fp8"), default="int8")
     args = ask.parse_args()
+    for name in ("layers", "requests", "prompt", "steps"):
+        if getattr(args, name) < 1:
+            ask.error(f"--{name} is at least 1")
     longest = args.prompt + args.steps + 1
     pages = args.requests * (-(-longest // 64) + 1)
     server = Server(args.layers, args.requests, pages=pages, longest=longest,
