@@ -1240,6 +1240,7 @@ class Prebuilt:
             raise ValueError(f"attend: the plan is of {rows} rows in pages of {plan.page}, not of {tokens} in pages of {page}")
         if window < 0 or (window and not causal):
             raise ValueError(f"attend: a window of {window} tokens{'' if causal else ' without causal'}")
+        window = min(window, 0x7FFFFFFF)  # the C entry's int; no position is past it
         if self._elsewhere((cache.k, cache.v, cache.k_scale, cache.v_scale, q, table, starts, lengths)):
             raise ValueError(f"attend: every tensor must be on cuda:{self.index}")
         out = q.new_empty((tokens, q_heads, width))

@@ -121,6 +121,11 @@ __device__ __forceinline__ int wave_top(int x) {
     return max(x, dpp_or_zero<0x143, 0xC>(x));
 }
 
+// The first token that a row at `position` sees, whatever numbers the two are.
+__device__ __forceinline__ int low_of(const CacheAttend& p, int position) {
+    return p.window > 0 && position >= p.window ? position + 1 - p.window : 0;
+}
+
 // --------------------------------------------------------------------- sharing the work out
 
 constexpr int kStep = 64;       // tokens taken at a time
@@ -144,7 +149,7 @@ __device__ __forceinline__ Extent extent(const CacheAttend& p, const Part& part,
     const Rows own = rows_of(p, r);
     const int rows = own.fresh * p.group;
     if (rows <= part.over || rows > part.upto) return {0, 0};
-    const int low = p.window > 0 ? max(0, own.before + 1 - p.window) : 0;
+    const int low = low_of(p, own.before);
     const int held = min(own.length, p.width << p.shift);  // what the table's row has pages for
     const int steps = (held + kStep - 1) / kStep - low / kStep;
     return {(rows + (1 << part.shift) - 1) >> part.shift, max(steps, 0)};
@@ -348,8 +353,8 @@ struct Span {
 __device__ __forceinline__ Span span_of(const CacheAttend& p, int row0, int rows, const Rows& own, int split = 0, int splits = 1) {
     const int before = own.before, length = own.length, t0 = row0 / p.group, t1 = (rows - 1) / p.group;
     Span s;
-    s.low_least = p.window > 0 ? max(0, before + t0 + 1 - p.window) : 0;
-    s.low_most = p.window > 0 ? max(0, before + t1 + 1 - p.window) : 0;
+    s.low_least = low_of(p, before + t0);
+    s.low_most = low_of(p, before + t1);
     s.high_least = p.causal ? before + t0 + 1 : length;
     // Past what the table's row has pages for there is nothing to see, whatever the length says.
     s.high_most = min(p.causal ? before + t1 + 1 : length, p.width << p.shift);
@@ -459,7 +464,7 @@ __global__ __launch_bounds__(256, kWidth == 256 ? 1 : 2) void few_kernel(CacheAt
             head[n] = kv * p.group + (live ? row - token[n] * p.group : 0);
             const int position = own.before + token[n];
             high[n] = live ? max(p.causal ? position + 1 : length, 0) : 0;
-            low[n] = live && p.window > 0 ? max(0, position + 1 - p.window) : 0;
+            low[n] = live ? low_of(p, position) : 0;
         }
         // The rows, read before the pages are looked up where there is one tile of them.
         const auto read_rows = [&]() {
@@ -475,7 +480,7 @@ __global__ __launch_bounds__(256, kWidth == 256 ? 1 : 2) void few_kernel(CacheAt
         };
         if constexpr (kTiles == 1) read_rows();
         const Span span = span_of(p, kRows * item.tile, min(rows, kRows * (item.tile + 1)), own);
-        const int base = (p.window > 0 ? max(0, own.before + 1 - p.window) : 0) / kStep;
+        const int base = low_of(p, own.before) / kStep;
         const int begin = max(span.begin, base + ((at - item.start) << sv.shift));
         const int end = stop == item.start + item.units ? span.end : min(span.end, base + ((stop - item.start) << sv.shift));
         const int* table = p.table + static_cast<int64_t>(item.request) * p.width;
@@ -743,7 +748,7 @@ __global__ __launch_bounds__(64 * kWaves, kWidth == 256 ? 1 : 2) void many_kerne
     const int token = live ? row / p.group : 0, head = kv * p.group + (live ? row - token * p.group : 0);
     const int position = of.before + token;
     const int high = live ? max(p.causal ? position + 1 : length, 0) : 0;
-    const int low = live && p.window > 0 ? max(0, position + 1 - p.window) : 0;
+    const int low = live ? low_of(p, position) : 0;
 
     f16x8 q[kDepth];
     float sharp;

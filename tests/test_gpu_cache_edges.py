@@ -162,3 +162,29 @@ def test_plan_of_the_most_rows(kv):  # noqa: F811
     assert got.slots[:33].tolist() == [*range(64, 80), *range(48, 64), -1]
     assert got.positions[-1].item() == rows - 1 and got.requests[-1].item() == 0
     assert got.spare.tolist() == [0, rows // 16 - 2]
+
+
+# ------------------------------------------------------------------------------- arguments
+
+
+@pytest.mark.parametrize("window", [2**31 - 1, 2**31, 2**32, 2**32 + 5, 2**40])
+@pytest.mark.parametrize("new", [[1, 2], [150, 90]], ids=["few", "many"])
+def test_windows_past_32_bits_hide_nothing(kv, new, window):  # noqa: F811
+    lengths = [200, 700]
+    cache, table, _ = filled(kv, lengths, 16, 2, 64, torch.int8, 7)
+    plan, _, tokens = make_plan(kv, table, lengths, new, 16, max(new))
+    q = torch.randn(tokens, 16, 64, generator=torch.Generator().manual_seed(8)).bfloat16().to(DEV)
+    assert torch.equal(cache.attend(torch, q, plan, window=window), cache.attend(torch, q, plan, window=2**20))
+
+
+@pytest.mark.parametrize("new", [[5, 2], [150, 90]], ids=["few", "many"])
+def test_windows_of_any_size_over_lengths_below_the_rows(kv, new):  # noqa: F811
+    """Rows at positions below zero see nothing, and those at zero and above what they would without a window."""
+    lengths = [1, 2]
+    cache, table, _ = filled(kv, lengths, 16, 2, 64, torch.int8, 9)
+    plan, _, tokens = make_plan(kv, table, lengths, new, 16, max(new))
+    q = torch.randn(tokens, 16, 64, generator=torch.Generator().manual_seed(10)).bfloat16().to(DEV)
+    plain = cache.attend(torch, q, plan)
+    assert (plain[: new[0] - 1] == 0).all() and (plain[new[0] - 1] != 0).any() and (plain[-1] != 0).any()
+    for window in (2**31 - 1, 2**31 - 2, 2**30):
+        assert torch.equal(cache.attend(torch, q, plan, window=window), plain)
