@@ -1304,7 +1304,7 @@ class Prebuilt:
         pages, heads, page, width = k.shape
         k_at, v_at = k.data_ptr(), v.data_ptr()
         if (v.shape != (pages, heads, width, page) or page not in (16, 32, 64, 128, 256) or width not in (64, 128, 256)
-                or not k.is_contiguous() or not v.is_contiguous() or (k_at | v_at) & 15):  # fmt: skip
+                or not pages or not heads or not k.is_contiguous() or not v.is_contiguous() or (k_at | v_at) & 15):  # fmt: skip
             raise ValueError(f"{op}: no cache of dense, 16-byte aligned keys {list(k.shape)} and values {list(v.shape)}")
         shape, f32 = (pages, heads), self._float32
         if (k_scale.dtype is not f32 or v_scale.dtype is not f32 or k_scale.shape != shape or v_scale.shape != shape

@@ -188,3 +188,16 @@ def test_windows_of_any_size_over_lengths_below_the_rows(kv, new):  # noqa: F811
     assert (plain[: new[0] - 1] == 0).all() and (plain[new[0] - 1] != 0).any() and (plain[-1] != 0).any()
     for window in (2**31 - 1, 2**31 - 2, 2**30):
         assert torch.equal(cache.attend(torch, q, plan, window=window), plain)
+
+
+def test_caches_of_no_pages_or_heads_are_refused(kv):  # noqa: F811
+    for pages, heads in ((0, 2), (2, 0)):
+        codes = torch.zeros(pages, heads, 64, 64, dtype=torch.int8, device=DEV)
+        scale = torch.zeros(pages, heads, device=DEV)
+        cache = kv.PagedCache(codes, codes, scale, scale)
+        plan = kv.plan(torch, ints([[-1]]), ints([0]), ints([0]), ints([0]), ints([2]), tokens=2, page=64)
+        x = torch.zeros(2, max(heads, 1), 64, dtype=torch.bfloat16, device=DEV)
+        for call in (lambda: cache.append(torch, x[:, :heads], x[:, :heads], plan), lambda: cache.attend(torch, x, plan),
+                     lambda: cache.read(torch, ints([0]), torch.bfloat16)):  # fmt: skip
+            with pytest.raises(ValueError, match="cache"):
+                call()
