@@ -30,9 +30,10 @@ __device__ __forceinline__ void load8f(const float* p, float* v) {
 // the rotated part holds both elements of eight pairs, so that a rotation needs no other lane: for
 // halves the chunks u and u + rotated/16 of eight elements, otherwise the neighbours 2u and 2u + 1.
 // Bound by memory over a prompt: 8191 tokens of 32 + 8 heads of 128 in 34.8 us, 172 MB at 4.9 TB/s, where a
-// large copy runs at 5.1; the vector unit is busy 82% of that time, which is why the 16-bit type is a template
-// parameter (chosen at run time both types' conversions were worked out). 24 tokens take 3.7 us: a launch and
-// one trip to memory, and one for the tables.
+// large copy runs at 5.6; the vector unit is busy 82% of that time, which is why the 16-bit type is a template
+// parameter (chosen at run time both types' conversions were worked out). 4173 tokens of 20 + 20 heads of 64, 44 MB,
+// take 12.1 us: the vector unit, busy 71%, beside memory at 3.6 TB/s, and the launch's beginning and end. 24 tokens take
+// 3.7 us: a launch and one trip to memory, and one for the tables.
 template <bool kHalf>
 __global__ __launch_bounds__(kThreads) void norm_rope_kernel(HeadRows r) {
     const int64_t head_slot = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) / r.lanes;

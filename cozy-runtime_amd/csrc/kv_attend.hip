@@ -11,8 +11,12 @@
 // weight's exponent, p = 2^(s·log2(e) + log2(vs) − m), so that m bounds what a token adds to the
 // output rather than its probability, and the denominator takes p/vs. A query row is brought near
 // 2^12 by a power of two and is then exact in f16, but for what lies below 2^-26 of its largest
-// element. Weights are rounded to f16 (11 bits, three more than bf16) for the second product alone; maxima,
-// sums and both products' accumulators are float32.
+// element. Weights are rounded to f16 (11 bits, three more than bf16) for the second product alone: float32 runs
+// at a sixteenth of the rate there, and two f16 numbers a weight would double the product. Nothing shows of it in
+// bf16; in fp16 an output's error grows from 2.1e-4 to 2.7e-4 of its norm. Maxima, sums and both products'
+// accumulators are float32.
+// A denominator takes p/vs where p is above 2^-126 of the reference: where a request's pages have value scales
+// more than 2^110 apart, the tokens of the smallest may be missing from it.
 #include <hip/hip_runtime.h>
 
 #include "common.h"
@@ -335,7 +339,8 @@ __device__ bool find_item(const CacheAttend& p, const Part& part, const Survey& 
 
 // Rows of the step that no request has (before the first one's and past the last one's) are zeros: the
 // workgroups without a share write them, those from number `busy` on. There are `heads` at the least: a launch
-// has that many more than it can have shares.
+// has that many more than it can have shares. They run beside the others: 24 to 216 such rows of 32 heads of 128
+// added nothing to 82 us of 40 requests, 984 (8 MB) 3 us, and 4095 beside one request over 131071 tokens 36 us.
 __device__ void clear_rest(const CacheAttend& p, int width, int busy) {
     const int64_t row = static_cast<int64_t>(p.q_heads) * width / 8;
     const int64_t before = row_start(p, 0) * row, after = row_start(p, p.requests) * row, count = before + p.tokens * row - after;
@@ -417,11 +422,14 @@ __device__ __forceinline__ void query8(const CacheAttend& p, const uint16_t* x, 
 // values that the group loads for the second product. Codes go from memory to registers to the matrix
 // unit; nothing of the cache passes through LDS but its pages' numbers and scales, read once a tile.
 // A step's keys are loaded over the previous step's second product and its values over its first.
-// kOnce (pages of up to 64 tokens): every line of codes is read by one load alone and marked so, which leaves
-// the caches to what is read again: one token for each of 40 requests 86 -> 75 us. The values of a larger
-// page's channel fill a line that two steps share: with the mark 53 us became 57 at 131071 tokens.
+// kOnce: lines of codes are marked as read once, which leaves the caches to what is read again. The rule is the
+// page's size alone. Up to 64 tokens a row tile reads every line by one load: one token for each of 40 requests
+// 86 -> 75 us, and 0.93 of the time without the mark over requests of up to 32 rows. Of more, each row tile reads
+// the lines again, which the mark does not keep: 1.06 of the time without, 89 us for 74 at the worst (8 tokens of 64
+// heads over 8 and 100000). The values of a larger page's channel fill a line that two steps share: with the mark
+// 53 us became 57 at 131071 tokens.
 // Bound by the codes' way from memory: those 40 requests' up to 12001 tokens, 8 heads of 128, are 437 MB in 75 us,
-// 5.8 TB/s of the 6.05 that a large read reaches; 131071 tokens of one request, 268 MB, 53 us, 5.1 TB/s, with
+// 5.8 TB/s of the 7.2 that a large read reaches; 131071 tokens of one request, 268 MB, 53 us, 5.1 TB/s, with
 // some 5 us before the first codes arrive (the requests' survey, the pages' numbers and scales) and after the
 // last. 700 tokens of one request are 10.9 us on 8 workgroups of 11 steps: that chain alone.
 template <int kWidth, int kTiles, bool kFp8, bool kOnce>
@@ -715,8 +723,8 @@ __device__ __forceinline__ int exchanged(int m) { return (m & ~12) | ((m & 4) <<
 // the keys at token π(m), score register 8a + e of half h = l/32 is that of token 16a + 8h + e, in the order
 // that the second product reads its weights in. Bytes past the request's tokens and pages that the cache has
 // not become zeros on the way to LDS.
-// Bound by no unit alone: 14003 tokens of two requests, 32 heads of 128 over 8, are 857 GFLOP in 0.94 to 1.07 ms
-// as the clock allows, 0.80 to 0.91 PFLOP/s where a large f16 product reaches 1.18; of a SIMD's cycles the
+// Bound by no unit alone: 14003 tokens of two requests, 32 heads of 128 over 8, are 857 GFLOP in 0.93 to 1.05 ms
+// as the clock allows, 0.82 to 0.92 PFLOP/s where a large f16 product reaches 1.51; of a SIMD's cycles the
 // matrix unit is busy in 42%, the vector unit in 54% (a fifth in both at once), of a CU's the LDS in 43%.
 // Without the exponentials it was 6% faster, without the conversions 9%, without loads 3%. At width 64 (2311
 // tokens of 12 requests, 16 heads over 4, a window of 4096: 30 GFLOP in 74 us) a score costs the vector unit
@@ -1183,9 +1191,11 @@ constexpr int kManyRows = 1024;   // unless so many a request on average leave f
 // What the few rows' kernel has to do, in rows of a key head: twice as much at width 256, where a CU holds one
 // workgroup and not two; where tiles are split, times the root of a row's steps (at the most kLongSteps, as a
 // table may be much wider than the requests are long), since the many rows' kernel then costs its join and parts first
-// and codes made f16 once for 256 rows later. Timed over 730 steps of 128 to 12000 rows, 200 to 20000 tokens held, 1
-// to 30 requests and six head layouts, it takes 1.011 of the faster side's time (geometric mean; a
-// limit of 1024 rows for all 1.115). Few / many rows' kernel, us, 32 heads over 8 of width 128: 100 tokens over 300
+// and codes made f16 once for 256 rows later. Timed over 755 steps of 125 to 12000 rows, up to 20000 tokens held, 1
+// to 30 requests and six head layouts (int8, bf16, pages of 64), it takes 1.012 of the faster side's time (geometric
+// mean; a limit of 1024 rows for all 1.112) and more than 1.25 of it in ten, seven of them at width 256, where the
+// mean is 1.031: at the worst 76 us for 43, 1024 rows of 12 requests over 2500, and 117 for 69, 400 of one over
+// 20000. Few / many rows' kernel, us, 32 heads over 8 of width 128: 100 tokens over 300
 // 14 / 23, over 2500 41 / 43, over 7000 55 / 50, over 20000 101 / 68; 256 over 7000 86 / 60; 500 over 300 24 / 35, over
 // 7000 159 / 92; 1750 tokens of 8 requests over 200 54 / 31; 16 heads over 2 of 256: 128 over 2500 68 / 59, over 300 28 / 34.
 constexpr int64_t kLongSteps = 128;

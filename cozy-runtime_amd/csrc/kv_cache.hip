@@ -81,9 +81,10 @@ struct PageOf {
 // tokens and of the runs, finding each one's request by bisection of the prefix sums: one launch,
 // and nothing passes between workgroups. No entry of the table is both read and written: a page that
 // was held is read, one that is new is written.
-// Bound by latency: 48 requests' tokens 5.3 us (one workgroup: three prefix sums after one trip to memory, a
-// second trip for the pages), 20011 tokens of 1000 requests 11.8 us on 20 workgroups. Its bytes, 0.3 MB
-// then, would take 0.1 us.
+// Bound by latency: 48 requests' tokens 5.4 us (one workgroup: three prefix sums after one trip to memory, a
+// second trip for the pages), 20011 tokens of 1000 requests 12.1 us on 20 workgroups, whose threads take four tokens
+// one after another, each a bisection in LDS and a trip for its page (waves wait for 70% of their life). Its
+// bytes, 0.3 MB then, would take 0.1 us.
 __global__ __launch_bounds__(kThreads) void plan_kernel(CachePlan p) {
     extern __shared__ int shared[];
     __shared__ int wave_sums[kWaves];
@@ -223,10 +224,11 @@ constexpr int kFewTokens = 4;
 // A thread reads eight elements at a time, kHeld times before it looks at any: a page of up to 16384 elements
 // is in the workgroup's registers after one trip to memory and is coded from there; a larger one is read
 // twice. New values are turned in LDS, four tokens of a channel a dword, rows of page/4 + 1 dwords.
-// Bound by latency at one token a request (96 requests, 8 heads of 128: 8.6 us, 3 MB read and 6 written, for a
-// run's chain of its numbers, its elements, the page's codes where the scale grows, and their write), and over
-// prompts by that chain and the vector unit (6001 tokens, 8 heads of 128: 14.0 us, 25 MB read and 13 written,
-// VALU busy 39%, on 832 workgroups, a run and head each: 3328 waves, where the chip holds 8192 of them).
+// At one token a request bound by a run's chain (its numbers, its elements, the page's codes where the scale grows,
+// and their write) and by the vector unit, busy 49%: 16 of 256 threads have an element, and all four waves go
+// through the loops (96 requests, 8 heads of 128: 8.6 us, 3 MB read and 6 written). Over prompts by that chain on too
+// few waves (6001 tokens, 8 heads of 128: 14.0 us, 25 MB read and 13 written, VALU busy 39%: 832 workgroups, a run
+// and head each, are 3328 waves, where the chip holds 8192 of them).
 template <bool kFp8, bool kHalf, bool kValues>
 __device__ void append(const CacheAppend& p, int width_shift, int page_shift, const i32x4& run, uint32_t* turned, uint32_t* wave_most) {
     constexpr int kHeld = 8;

@@ -547,8 +547,12 @@ int cozyq_cache_read(int device, int fp8, const void* k_codes, const void* v_cod
  * Tokens whose table entry is no page of the cache are not seen; a row that sees none, or belongs to no
  * request, is 0. What pages hold past a request's tokens is not read into any result. `most`: the most rows
  * a request has, as far as the caller knows (0: not at all); it sets the launch's shape and speed, never its
- * results. The workspace is of cozyq_cache_attend_workspace_bytes bytes, uninitialised (NULL where that is 0;
- * -1 for a bad argument). */
+ * results. A request's value scales are within 2^110 of one another; where they are not, tokens of the smallest may
+ * be missing from a row's denominator. The workspace is of cozyq_cache_attend_workspace_bytes bytes, uninitialised
+ * (NULL where that is 0; -1 for a bad argument). It goes by shapes alone, as the lengths are on the GPU, whether or
+ * not a tile is split then: none where the table's rows are of up to 1024 tokens; otherwise 9 to 17 MB for few rows
+ * a request at width 128, and where a request may have many 138 MB more (69 over rows of up to 4096 tokens; 36 MB at
+ * width 64, 136 at 256). */
 int64_t cozyq_cache_attend_workspace_bytes(int64_t tokens, int q_heads, int requests, int heads, int page, int width,
                                            int table_width, int64_t most, int window);
 int cozyq_cache_attend(int device, int fp8, const void* q, int half, int64_t tokens, int q_heads, int64_t q_token,
