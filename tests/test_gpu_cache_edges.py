@@ -201,3 +201,24 @@ def test_caches_of_no_pages_or_heads_are_refused(kv):  # noqa: F811
                      lambda: cache.read(torch, ints([0]), torch.bfloat16)):  # fmt: skip
             with pytest.raises(ValueError, match="cache"):
                 call()
+
+
+@pytest.mark.parametrize("codes", [torch.int8, E4M3], ids=["int8", "fp8"])
+@pytest.mark.parametrize("apart", [0, 64, 109])
+@pytest.mark.parametrize("new", [[1, 3], [150, 90]], ids=["few", "many"])
+def test_value_scales_far_apart_share_one_denominator(kv, new, apart, codes):  # noqa: F811
+    """Pages whose value scales are 2^`apart` apart in turn, equal keys: the small ones' tokens weigh as much."""
+    lengths, page = [400, 1700], 16
+    cache, table, value = filled(kv, lengths, page, 4, 64, codes, 15)
+    cache.k_scale.zero_()
+    value[0].nan_to_num_(0.0).zero_()
+    for row in table:
+        for i, number in enumerate(n for n in row if n >= 0):
+            power = 2.0 ** (apart - 40 if i % 3 == 1 else -40)
+            cache.v_scale[number] *= power
+            value[1, number] *= power
+    plan, starts, tokens = make_plan(kv, table, lengths, new, page, max(new))
+    q = torch.randn(tokens, 32, 64, generator=torch.Generator().manual_seed(16)).bfloat16().to(DEV)
+    got = cache.attend(torch, q, plan)
+    want, size = expected(q, value, table, starts, lengths, page)
+    assert ((got.double() - want).abs() <= 2.0**-8 * want.abs() + (2.0**-11 + 2.0**-12) * size).all()
