@@ -138,6 +138,14 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         [c_int, _P, _P, c_int, c_int64, c_int, c_int, c_int, c_int64, c_int64, c_int64, c_int64, c_int, _P, _P,
          c_int, c_float, _P, _P, c_int64, c_int, c_int, _P, _P, _P, _P],
     ),
+    "cozyq_head_norm_rope_axes": (
+        c_int,
+        [c_int, _P, _P, c_int, c_int64, c_int, c_int, c_int, c_int64, c_int64, c_int64, c_int64, c_int, _P, _P,
+         c_int, c_float, _P, _P, c_int64, c_int, c_int, _P, c_int, _P, c_int, _P, _P, _P],
+    ),
+    "cozyq_add_rms": (
+        c_int, [c_int, c_int, _P, _P, c_int, _P, c_int, c_float, _P, _P, _P, c_int64, c_int, _P]
+    ),
     "cozyq_cache_most_requests": (c_int, []),
     "cozyq_cache_runs": (c_int64, [c_int64, c_int, c_int]),
     "cozyq_cache_plan": (

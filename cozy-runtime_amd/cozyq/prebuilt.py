@@ -1063,8 +1063,9 @@ class Prebuilt:
     def head_norm_rope(
         self, q: Tensor, k: Tensor | None, q_gain: Tensor | None, k_gain: Tensor | None, cos: Tensor | None,
         sin: Tensor | None, positions: Tensor | None, eps: float | None, interleaved: bool,
+        sections: Any = None, cycled: bool = False,
     ) -> tuple[Tensor, Tensor | None]:
-        """`heads.norm_rope` on this card (`cozyq_head_norm_rope`)."""
+        """`heads.norm_rope` on this card (`cozyq_head_norm_rope_axes`)."""
         f32 = self._float32
         dtype = q.dtype
         half = self._half(dtype)
@@ -1106,19 +1107,92 @@ class Prebuilt:
                                  "tokens (R a multiple of 16)")  # fmt: skip
         elif cos is not None or sin is not None:
             raise ValueError("norm_rope: cos and sin go together")
-        if positions is not None:
+        axes, shares = 1, None
+        if sections is not None:
+            axes, shares = self._sections(sections, cycled, rotated // 2, positions, tokens)
+            rows_at = positions.data_ptr()
+        elif cycled:
+            raise ValueError("norm_rope: cycled axes have sections")
+        elif positions is not None:
             rows_at = self._ints("norm_rope", "positions", positions, tokens)
         if self._elsewhere((q, k, q_gain, k_gain, cos, sin, positions)):
             raise ValueError(f"norm_rope: every tensor must be on cuda:{self.index}")
         q_out = q.new_empty((tokens, q_heads, width))
-        code = self._lib.cozyq_head_norm_rope(
+        code = self._lib.cozyq_head_norm_rope_axes(
             self.index, q.data_ptr(), k_at, half, tokens, q_heads, k_heads, width, q_token, q_head, k_token, k_head,
-            eps is not None, q_by, k_by, wide, eps or 0.0, cos_at, sin_at, rows, rotated, interleaved, rows_at,
-            q_out.data_ptr(), k_to, self._stream(),
+            eps is not None, q_by, k_by, wide, eps or 0.0, cos_at, sin_at, rows, rotated, interleaved, rows_at, axes,
+            shares, cycled, q_out.data_ptr(), k_to, self._stream(),
         )  # fmt: skip
         if code:
             self._check(code, "the head norm and rotation")
         return q_out, k_out
+
+    def _sections(self, sections: Any, cycled: bool, pairs: int, positions: Tensor | None, tokens: int) -> tuple[int, Any]:
+        """How many axes `sections` names and their counts of pairs as the C entry reads them; ValueError unless they
+        share out `pairs` pairs and `positions` has a row for each axis."""
+        shares = tuple(sections)
+        axes = len(shares)
+        if not 2 <= axes <= 4 or not pairs or sum(shares) != pairs or min(shares) < 0:
+            raise ValueError(f"norm_rope: sections {list(shares)} do not share {pairs} pairs out over two to four axes")
+        if cycled and any(n and a + axes * (n - 1) >= pairs for a, n in enumerate(shares) if a):
+            raise ValueError(f"norm_rope: taken in turns, {pairs} pairs do not reach sections {list(shares)}")
+        if (positions is None or positions.dtype is not self._int32 or positions.shape != (axes, tokens)
+                or not positions.is_contiguous()):  # fmt: skip
+            raise ValueError(f"norm_rope: positions must be dense int32 [{axes}, {tokens}]")
+        return axes, (_lib.c_int * axes)(*shares)
+
+    def add_rms(
+        self, x: Tensor, residual: Tensor | None, gain: Tensor | None, fp8: bool, eps: float, out: Tensor | None
+    ) -> tuple[Tensor, Tensor, Tensor]:
+        """`norms.add_rms` on this card (`cozyq_add_rms`): codes, scales and the sum."""
+        if x.dim() == 0 or not x.shape[-1]:
+            raise ValueError(f"add_rms: x must be rows of at least one element, not {list(x.shape)}")
+        flat = self._rows(FP8 if fp8 else INT8, x)
+        rows, width = flat.shape
+        half = self._half(flat.dtype)
+        if not eps > 0.0:
+            raise ValueError(f"add_rms: eps is above 0, not {eps}")
+        total, other = x, None
+        if residual is None:
+            if out is not None and out is not x:
+                raise ValueError("add_rms: without a residual the sum is x itself")
+        else:
+            if residual.shape != x.shape or residual.dtype is not x.dtype or residual.get_device() != self.index:
+                raise ValueError(f"add_rms: the residual must be {x.dtype} {list(x.shape)} on cuda:{self.index}, not "
+                                 f"{residual.dtype} {list(residual.shape)} on {residual.device}")  # fmt: skip
+            other = self._rows(FP8 if fp8 else INT8, residual)
+            total = self._total(x, residual, out)
+        gain_at, wide = None, False
+        if gain is not None:
+            wide = gain.dtype is self._float32
+            gain_at = gain.data_ptr()
+            if ((not wide and gain.dtype is not x.dtype) or gain.shape != (width,) or not gain.is_contiguous() or gain_at & 15
+                    or gain.get_device() != self.index):  # fmt: skip
+                raise ValueError(f"add_rms: the gain is dense [{width}] on cuda:{self.index}, 16-byte aligned, float32 or of x's type")
+        codes = flat.new_empty((rows, width), dtype=self.torch.float8_e4m3fn if fp8 else self.torch.int8)
+        scales = flat.new_empty(rows, dtype=self._float32)
+        code = self._lib.cozyq_add_rms(
+            self.index, fp8, flat.data_ptr(), _ptr(other), half, gain_at, wide, eps, None if other is None else total.data_ptr(),
+            codes.data_ptr(), scales.data_ptr(), rows, width, self._stream(),
+        )  # fmt: skip
+        if code:
+            self._check(code, "the residual norm")
+        return codes, scales, total
+
+    def _total(self, x: Tensor, residual: Tensor, out: Tensor | None) -> Tensor:
+        """Where the sum of `x` and `residual` goes: a new tensor, or `out`; ValueError for one that the kernel cannot
+        write, or that shares memory with either without being it."""
+        if out is None:
+            return x.new_empty(x.shape)
+        if (out.dtype is not x.dtype or out.shape != x.shape or out.get_device() != self.index or not out.is_contiguous()
+                or out.data_ptr() & 15):  # fmt: skip
+            raise ValueError(f"add_rms: out must be a dense, 16-byte aligned {x.dtype} {list(x.shape)} on cuda:{self.index}")
+        for t in (x, residual):
+            # (One that is not dense or aligned is read from a copy.)
+            if t.is_contiguous() and not t.data_ptr() & 15 and t.data_ptr() != out.data_ptr():
+                if abs(t.data_ptr() - out.data_ptr()) < out.numel() * out.element_size():
+                    raise ValueError("add_rms: out may be x or the residual, whole, but not share a part of either")
+        return out
 
     def cache_plan(
         self, table: Tensor, free: Tensor, spare: Tensor, held: Tensor, new: Tensor, tokens: int, page: int,

@@ -691,14 +691,59 @@ int cozyq_bake_stats(int device, int form, const void* before, const void* after
                              static_cast<int>(rank), partial, on(stream));
 }
 
+int cozyq_add_rms(int device, int fp8, const void* x, const void* residual, int half, const void* gain, int gain_wide,
+                  float eps, void* total, void* codes, float* scales, int64_t rows, int width, void* stream) {
+    if (!fits(width, fp8 ? 16 : 256) || rows < 0 || rows > cozyq::kMostTokens || !(eps > 0.0f))
+        return hipErrorInvalidValue;
+    if (rows == 0) return hipSuccess;
+    if (!x || !aligned16(x) || !aligned16(residual) || !aligned16(gain) || (residual && !total) || !aligned16(total) ||
+        !codes || !aligned16(codes) || !scales)
+        return hipErrorInvalidValue;
+    const OnDevice guard(device);
+    if (guard.error() != hipSuccess) return guard.error();
+    return cozyq::add_rms({static_cast<const uint16_t*>(x), static_cast<const uint16_t*>(residual), gain,
+                           static_cast<uint16_t*>(total), static_cast<uint8_t*>(codes), scales, static_cast<int>(rows),
+                           width, eps, half != 0, gain_wide != 0},
+                          fp8 != 0, on(stream));
+}
+
 int cozyq_head_norm_rope(int device, const void* q, const void* k, int half, int64_t tokens, int q_heads,
                          int k_heads, int width, int64_t q_token, int64_t q_head, int64_t k_token,
                          int64_t k_head, int norm, const void* q_gain, const void* k_gain, int gain_wide,
                          float eps, const float* cos, const float* sin, int64_t table_rows, int rotated,
                          int interleaved, const int* positions, void* q_out, void* k_out, void* stream) {
+    return cozyq_head_norm_rope_axes(device, q, k, half, tokens, q_heads, k_heads, width, q_token, q_head, k_token,
+                                     k_head, norm, q_gain, k_gain, gain_wide, eps, cos, sin, table_rows, rotated,
+                                     interleaved, positions, 1, nullptr, 0, q_out, k_out, stream);
+}
+
+// Which axis each pair belongs to, eight a word (HeadRows::axis_of); false for sections that are not `pairs` in all,
+// or that the turns do not reach.
+static bool axes_of_pairs(int axes, const int* sections, int cycled, int pairs, uint16_t* words) {
+    uint8_t axis[128] = {};
+    int64_t sum = 0;
+    for (int a = 0; a < axes; ++a) {
+        if (sections[a] < 0 || sections[a] > pairs) return false;
+        for (int i = 0; i < sections[a] && (a || !cycled); ++i) {
+            const int64_t at = cycled ? a + static_cast<int64_t>(axes) * i : sum + i;
+            if (at >= pairs) return false;
+            axis[at] = static_cast<uint8_t>(a);
+        }
+        sum += sections[a];
+    }
+    for (int j = 0; j < pairs; ++j) words[j / 8] = static_cast<uint16_t>(words[j / 8] | axis[j] << (2 * (j % 8)));
+    return sum == pairs;
+}
+
+int cozyq_head_norm_rope_axes(int device, const void* q, const void* k, int half, int64_t tokens, int q_heads,
+                              int k_heads, int width, int64_t q_token, int64_t q_head, int64_t k_token,
+                              int64_t k_head, int norm, const void* q_gain, const void* k_gain, int gain_wide,
+                              float eps, const float* cos, const float* sin, int64_t table_rows, int rotated,
+                              int interleaved, const int* positions, int axes, const int* sections, int cycled,
+                              void* q_out, void* k_out, void* stream) {
     if (tokens < 0 || tokens > cozyq::kMostTokens || q_heads < 0 || k_heads < 0 || q_heads > 4096 ||
         k_heads > 4096 || width < 16 || width > 256 || width % 16 || rotated < 0 || rotated > width ||
-        rotated % 16)
+        rotated % 16 || axes < 1 || axes > 4 || (axes > 1 && (!sections || !rotated)))
         return hipErrorInvalidValue;
     if (tokens == 0 || q_heads + k_heads == 0) return hipSuccess;
     if ((q_heads && (!q || !q_out || !aligned16(q) || !aligned16(q_out) || q_token % 8 || q_head % 8)) ||
@@ -706,16 +751,17 @@ int cozyq_head_norm_rope(int device, const void* q, const void* k, int half, int
         !aligned16(q_gain) || !aligned16(k_gain))
         return hipErrorInvalidValue;
     if (rotated && (!cos || !sin || !aligned16(cos) || !aligned16(sin) || table_rows < 1 ||
-                    table_rows > cozyq::kMostTokens || (!positions && table_rows < tokens)))
+                    table_rows > cozyq::kMostTokens || (!positions && (axes > 1 || table_rows < tokens))))
         return hipErrorInvalidValue;
+    cozyq::HeadRows rows{static_cast<const uint16_t*>(q), static_cast<const uint16_t*>(k),
+                         static_cast<uint16_t*>(q_out), static_cast<uint16_t*>(k_out), q_gain, k_gain,
+                         cos, sin, positions, q_token, q_head, k_token, k_head, static_cast<int>(tokens),
+                         q_heads, k_heads, width, rotated, static_cast<int>(table_rows), axes, eps, half != 0,
+                         norm != 0, gain_wide != 0, interleaved != 0, {}, 0, 0};
+    if (axes > 1 && !axes_of_pairs(axes, sections, cycled, rotated / 2, rows.axis_of)) return hipErrorInvalidValue;
     const OnDevice guard(device);
     if (guard.error() != hipSuccess) return guard.error();
-    return cozyq::head_norm_rope({static_cast<const uint16_t*>(q), static_cast<const uint16_t*>(k),
-                                  static_cast<uint16_t*>(q_out), static_cast<uint16_t*>(k_out), q_gain, k_gain,
-                                  cos, sin, positions, q_token, q_head, k_token, k_head, static_cast<int>(tokens),
-                                  q_heads, k_heads, width, rotated, static_cast<int>(table_rows), 0, eps, half != 0,
-                                  norm != 0, gain_wide != 0, interleaved != 0},
-                                 on(stream));
+    return cozyq::head_norm_rope(rows, on(stream));
 }
 
 // log2 of a page's tokens, or -1 for a size that the cache does not take.

@@ -111,6 +111,19 @@ __device__ __forceinline__ float wave_max_nan(float v) {
     return nan_max(nan_max(r0, r1), nan_max(r2, r3));
 }
 
+// The sum over a wave, uniform, by DPP within 16-lane rows (wave_max's pattern), then the rows.
+__device__ __forceinline__ float wave_sum(float v) {
+    v += dpp_move<0xB1>(v);
+    v += dpp_move<0x4E>(v);
+    v += dpp_move<0x124>(v);
+    v += dpp_move<0x128>(v);
+    const int b = __builtin_bit_cast(int, v);
+    float r[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(b, 16 * i));
+    return (r[0] + r[1]) + (r[2] + r[3]);
+}
+
 // The sum over a wave of a value that is zero outside lanes 0-3, 20-23, 40-43 and 60-63: the
 // diagonal of a 16x16 MFMA result (lane l holds rows 4·(l/16) + r of column l%16), one quad of
 // each 16-lane row. Each quad is summed by two DPP quad swaps, then the four quad sums are read

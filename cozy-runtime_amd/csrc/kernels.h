@@ -301,7 +301,9 @@ hipError_t rotate_factor(const float* down, float* out, int64_t groups, hipStrea
 // Queries and keys [tokens, heads, width] (16-bit, rows `*_token` and heads `*_head` elements apart)
 // normed a head (RMS, eps inside the root, times `gain` [width] in x's type or, with gain_wide,
 // float32) and rotated over their first `rotated` elements by the cos / sin tables' row
-// positions[token] (or token), into contiguous q_out / k_out. `lanes` is the launcher's.
+// positions[token] (or token), into contiguous q_out / k_out. With more than one axis, positions are
+// [axes, tokens] and pair j of the rotated part takes axis (axis_of[j / 8] >> 2·(j % 8)) & 3. `lanes` and
+// `runs` are the launcher's.
 struct HeadRows {
     const uint16_t* q;
     const uint16_t* k;
@@ -313,11 +315,29 @@ struct HeadRows {
     const float* sin;
     const int* positions;
     int64_t q_token, q_head, k_token, k_head;
-    int tokens, q_heads, k_heads, width, rotated, table_rows, lanes;
+    int tokens, q_heads, k_heads, width, rotated, table_rows, axes;
     float eps;
     bool half, norm, gain_wide, interleaved;
+    uint16_t axis_of[16];
+    int lanes, runs;
 };
 hipError_t head_norm_rope(HeadRows rows, hipStream_t s);
+
+// A residual stream's next norm in 8 bits (cozyq_add_rms): total = x + residual rounded to the rows' type (no
+// residual: x, and total is not written), then total · rsqrt(mean(total²) + eps) · gain as E4M3 (fp8) or rotated
+// int8 codes with a scale a row. x, residual and total may be one buffer.
+struct AddRms {
+    const uint16_t* x;
+    const uint16_t* residual;
+    const void* gain;
+    uint16_t* total;
+    uint8_t* codes;
+    float* scales;
+    int rows, width;
+    float eps;
+    bool half, gain_wide;
+};
+hipError_t add_rms(const AddRms& p, bool fp8, hipStream_t s);
 
 // The most rows, table rows or cache slots that the head and cache kernels index: int32 with room.
 constexpr int kMostTokens = 1 << 30;

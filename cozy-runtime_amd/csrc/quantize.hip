@@ -40,19 +40,6 @@ __device__ __forceinline__ void load8(const uint16_t* p, float* v) {
     }
 }
 
-// The sum over a wave, uniform, by DPP within 16-lane rows (wave_max's pattern), then the rows.
-__device__ __forceinline__ float wave_sum(float v) {
-    v += dpp_move<0xB1>(v);
-    v += dpp_move<0x4E>(v);
-    v += dpp_move<0x124>(v);
-    v += dpp_move<0x128>(v);
-    const int b = __builtin_bit_cast(int, v);
-    float r[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) r[i] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(b, 16 * i));
-    return (r[0] + r[1]) + (r[2] + r[3]);
-}
-
 __device__ __forceinline__ float block_sum(float v, float* red) {
     v = wave_sum(v);
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;

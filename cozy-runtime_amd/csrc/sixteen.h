@@ -28,6 +28,16 @@ __device__ __forceinline__ void load8(const uint16_t* p, float* v) {
     widen8<kHalf>(*reinterpret_cast<const i32x4*>(p), v);
 }
 
+// Eight float32 elements at a 16-byte address.
+__device__ __forceinline__ void load8f(const float* p, float* v) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const f32x4 raw = *reinterpret_cast<const f32x4*>(p + 4 * i);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[4 * i + j] = raw[j];
+    }
+}
+
 // Two float32 values rounded to nearest even, the first in the low half: v_cvt_pk_bf16_f32 for bf16; for
 // fp16 each float32 value stands on its own first (see narrow).
 template <bool kHalf>

@@ -494,6 +494,30 @@ int cozyq_head_norm_rope(int device, const void* q, const void* k, int half, int
                          float eps, const float* cos, const float* sin, int64_t table_rows, int rotated,
                          int interleaved, const int* positions, void* q_out, void* k_out, void* stream);
 
+/* The same with a position on each of `axes` axes (1 to 4; time, height and width of images and video): positions
+ * int32 [axes, tokens], and pair j of the rotated/2 turns by cos / sin [positions[axis of j][token], j]. sections
+ * [axes] (host memory) says how many pairs each axis has, rotated/2 in all: in runs, axis 0's first; or with `cycled`
+ * in turns, axis a > 0 having pairs a, a + axes, a + 2 · axes, .. (each below rotated/2) and axis 0 the others.
+ * axes 1 is the entry above, sections then unused. */
+int cozyq_head_norm_rope_axes(int device, const void* q, const void* k, int half, int64_t tokens, int q_heads,
+                              int k_heads, int width, int64_t q_token, int64_t q_head, int64_t k_token,
+                              int64_t k_head, int norm, const void* q_gain, const void* k_gain, int gain_wide,
+                              float eps, const float* cos, const float* sin, int64_t table_rows, int rotated,
+                              int interleaved, const int* positions, int axes, const int* sections, int cycled,
+                              void* q_out, void* k_out, void* stream);
+
+/* The residual's addition, the RMS norm of the sum and its quantization in one pass (the reference's fused norm and
+ * quantize kernels, kernels/csrc/gemm/rotate.cu:195-282, take no residual): rows of `width` 16-bit numbers, dense.
+ *   total = x + residual rounded to the rows' type (residual NULL: x itself, and total is not written),
+ *   n = total · rsqrt(mean(total²) + eps) · gain, gain [width] in the rows' type or, with gain_wide, float32 (NULL: 1),
+ *   fp8: scale = max(amax(n) / 448, 1e-12), codes E4M3 of n / scale (width % 16 == 0);
+ *   otherwise n is rotated by the block Hadamard of 256, scale = max(amax / 127, 1e-12) and codes are int8 rounded to
+ *   nearest even (width % 256 == 0): the operands of cozyq_gemm.
+ * codes [rows, width], scales [rows]. total may be x or residual. width up to cozyq_max_k(), eps above 0. A row that
+ * holds a NaN or an infinity has the scale NaN. */
+int cozyq_add_rms(int device, int fp8, const void* x, const void* residual, int half, const void* gain, int gain_wide,
+                  float eps, void* total, void* codes, float* scales, int64_t rows, int width, void* stream);
+
 /* The paged 8-bit cache of keys and values (no reference counterpart: the reference's LM keeps a static
  * 16-bit cache). `pages` pages of `page` tokens (16, 32, 64, 128 or 256) of every key head: k_codes
  * [pages, heads, page, width], v_codes [pages, heads, width, page] (values stand transposed), int8 or
