@@ -169,6 +169,12 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         [c_int, c_int, _P, c_int, c_int64, c_int, c_int64, c_int64, _P, _P, _P, _P, c_int, c_int, c_int, c_int, _P,
          c_int, c_int, _P, _P, c_int64, c_float, c_int, c_int, _P, _P, _P],
     ),
+    "cozyq_cross_attend_workspace_bytes": (c_int64, [c_int64, c_int, c_int, c_int, c_int, c_int, c_int64]),
+    "cozyq_cross_attend": (
+        c_int,
+        [c_int, _P, c_int, c_int64, c_int, c_int64, c_int64, _P, _P, c_int, c_int, c_int, c_int, c_int64, c_int64,
+         c_int64, c_int64, c_int64, c_int64, _P, _P, _P, c_int64, c_int64, c_float, _P, _P, _P],
+    ),
     "cozyq_host_e4m3": (None, [_P, _P, c_int64]),
     "cozyq_host_mx_byte": (None, [_P, _P, c_int64]),
     "cozyq_probe_div": (c_int, [c_int, _P, _P, _P, c_int64, _P]),

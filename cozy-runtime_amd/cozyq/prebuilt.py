@@ -1330,6 +1330,74 @@ class Prebuilt:
             self._check(code, "attention over the cache")
         return out
 
+    def cross_attend(
+        self, q: Tensor, k: Tensor, v: Tensor, starts: Tensor | None, lengths: Tensor | None, mask: Tensor | None,
+        most: int, scale: float | None,
+    ) -> Tensor:
+        """`attention.cross` on this card (`cozyq_cross_attend`)."""
+        dtype = q.dtype
+        half = self._half(dtype)
+        tokens, q_heads, width, q_token, q_head = self._heads("cross", "q", q)
+        shape = k.shape
+        if len(shape) != 4 or k.dtype is not dtype or v.dtype is not dtype or v.shape != shape or shape[3] != width:
+            raise ValueError(f"cross: k and v must be {dtype} [requests, states, heads, {width}] alike, not {k.dtype} "
+                             f"{list(k.shape)} and {v.dtype} {list(v.shape)}")  # fmt: skip
+        requests, states, heads, _ = shape
+        if not requests:
+            raise ValueError("cross: there is no request")
+        if not heads or not q_heads or q_heads % heads or not width or width > 256 or width % 8:
+            raise ValueError(f"cross: {q_heads} query heads over {heads} of {width}: query heads are a multiple of the key "
+                             "heads, heads a multiple of 8 up to 256 wide")  # fmt: skip
+        k_request, k_state, k_head = self._states("k", k)
+        v_request, v_state, v_head = self._states("v", v)
+        starts_at = lengths_at = mask_at = None
+        by_mask = 0
+        if starts is not None:
+            starts_at = self._ints("cross", "starts", starts, requests + 1)
+        elif tokens % requests:
+            raise ValueError(f"cross: {tokens} rows are not as many for each of {requests} requests; starts says whose they are")
+        else:
+            most = tokens // requests
+        if lengths is not None:
+            lengths_at = self._ints("cross", "lengths", lengths, requests)
+        if mask is not None:
+            if mask.dtype is not self.torch.bool or mask.shape != (requests, states) or (states > 1 and mask.stride(1) != 1):
+                raise ValueError(f"cross: the mask must be bool [{requests}, {states}] with a dense last axis")
+            mask_at, by_mask = mask.data_ptr(), mask.stride(0)
+        if most < 0:
+            raise ValueError(f"cross: a request has no {most} rows")
+        if self._elsewhere((q, k, v, starts, lengths, mask)):
+            raise ValueError(f"cross: every tensor must be on cuda:{self.index}")
+        out = q.new_empty((tokens, q_heads, width))
+        size = self._lib.cozyq_cross_attend_workspace_bytes(tokens, q_heads, requests, states, heads, width, most)
+        if size < 0:
+            raise ValueError(f"cross: {tokens} rows of {q_heads} heads over {states} states of {requests} requests are too many")
+        work = q.new_empty(size // 2) if size > 0 else None
+        code = self._lib.cozyq_cross_attend(
+            self.index, q.data_ptr(), half, tokens, q_heads, q_token, q_head, k.data_ptr(), v.data_ptr(), requests, states,
+            heads, width, k_request, k_state, k_head, v_request, v_state, v_head, starts_at, lengths_at, mask_at, by_mask,
+            most, width**-0.5 if scale is None else scale, out.data_ptr(), None if work is None else work.data_ptr(),
+            self._stream(),
+        )  # fmt: skip
+        if code:
+            self._check(code, "attention to the states")
+        return out
+
+    def _states(self, name: str, x: Tensor) -> tuple[int, int, int]:
+        """The request, state and head strides of keys or values `[requests, states, heads, width]` that the kernels read
+        16 bytes at a time; ValueError for others."""
+        by_request, by_state, by_head, dense = x.stride()
+        if (by_request | by_state | by_head) & 7 or dense != 1 or x.data_ptr() & 15 or by_state >= 1 << 23:
+            requests, states, heads, width = x.shape
+            # The stride of an extent of one is never taken.
+            by_request = by_request if requests > 1 else 0
+            by_state = by_state if states > 1 else 0
+            by_head = by_head if heads > 1 else 0
+            if (by_request | by_state | by_head) & 7 or dense != 1 or x.data_ptr() & 15 or by_state >= 1 << 23:
+                raise ValueError(f"cross: {name}'s last axis must be dense, its other strides and address multiples of 16 bytes, "
+                                 "its states less than 2^23 elements apart")  # fmt: skip
+        return by_request, by_state, by_head
+
     def _heads(self, op: str, name: str, x: Tensor) -> tuple[int, int, int, int, int]:
         """Tokens, heads, width and the token and head strides of a `[tokens, heads, width]` operand that
         the kernels read 16 bytes at a time; ValueError for another."""

@@ -880,6 +880,49 @@ int cozyq_cache_attend(int device, int fp8, const void* q, int half, int64_t tok
                                most, fp8 != 0, on(stream));
 }
 
+static bool cross_shape(int64_t tokens, int q_heads, int requests, int states, int kv_heads, int width, int64_t most) {
+    if (tokens < 0 || tokens > cozyq::kMostTokens || requests < 1 || requests > 65535 || states < 0 ||
+        states > cozyq::kMostTokens || kv_heads < 1 || kv_heads > 4096 || q_heads < 1 || q_heads > 4096 ||
+        q_heads % kv_heads || width < 8 || width > 256 || width % 8 || most < 0)
+        return false;
+    // Rows of a key head, and workgroups, are counted in 32 bits.
+    return tokens * (q_heads / kv_heads) <= cozyq::kMostTokens &&
+           (tokens * (q_heads / kv_heads) / 16 + requests + 64) * kv_heads < cozyq::kMostTokens;
+}
+
+int64_t cozyq_cross_attend_workspace_bytes(int64_t tokens, int q_heads, int requests, int states, int kv_heads, int width,
+                                           int64_t most) {
+    if (!cross_shape(tokens, q_heads, requests, states, kv_heads, width, most)) return -1;
+    return cozyq::cross_attend_work(tokens, q_heads / kv_heads, requests, kv_heads, states, width, most);
+}
+
+int cozyq_cross_attend(int device, const void* q, int half, int64_t tokens, int q_heads, int64_t q_token, int64_t q_head,
+                       const void* k, const void* v, int requests, int states, int kv_heads, int width, int64_t k_request,
+                       int64_t k_state, int64_t k_head, int64_t v_request, int64_t v_state, int64_t v_head,
+                       const int* starts, const int* lengths, const void* mask, int64_t mask_request, int64_t most,
+                       float scale, void* out, void* workspace, void* stream) {
+    constexpr int64_t kFar = 1 << 23;  // elements between states: a step of them is within a buffer's 2 GiB
+    if (!cross_shape(tokens, q_heads, requests, states, kv_heads, width, most) || k_state < 0 || k_state >= kFar ||
+        v_state < 0 || v_state >= kFar || (!starts && tokens % requests))
+        return hipErrorInvalidValue;
+    if (tokens == 0) return hipSuccess;
+    if (!q || !aligned16(q) || q_token % 8 || q_head % 8 || !out || !aligned16(out) || !aligned16(workspace) ||
+        (states && (!k || !v || !aligned16(k) || !aligned16(v))) || k_request % 8 || k_state % 8 || k_head % 8 ||
+        v_request % 8 || v_state % 8 || v_head % 8)
+        return hipErrorInvalidValue;
+    if (!workspace && cozyq_cross_attend_workspace_bytes(tokens, q_heads, requests, states, kv_heads, width, most))
+        return hipErrorInvalidValue;
+    const OnDevice guard(device);
+    if (guard.error() != hipSuccess) return guard.error();
+    return cozyq::cross_attend({static_cast<const uint16_t*>(q), static_cast<const uint16_t*>(k),
+                                static_cast<const uint16_t*>(v), static_cast<uint16_t*>(out), starts, lengths,
+                                static_cast<const uint8_t*>(mask), q_token, q_head, k_request, k_state, k_head, v_request,
+                                v_state, v_head, mask_request, static_cast<int>(tokens), requests,
+                                starts ? 0 : static_cast<int>(tokens / requests), states, kv_heads, q_heads,
+                                q_heads / kv_heads, width, scale, half != 0, static_cast<float*>(workspace), 1},
+                               most, on(stream));
+}
+
 void cozyq_host_e4m3(const float* in, uint8_t* out, int64_t n) {
     for (int64_t i = 0; i < n; ++i) out[i] = cozyq::e4m3_rn(in[i]);
 }

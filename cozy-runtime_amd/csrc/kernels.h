@@ -339,6 +339,28 @@ struct AddRms {
 };
 hipError_t add_rms(const AddRms& p, bool fp8, hipStream_t s);
 
+// Attention to an encoder's states (cozyq_cross_attend): request b's rows are starts[b] .. starts[b + 1] − 1 (no
+// starts: `each` rows a request), its states the first lengths[b] (no lengths: all) of `states` that its row of the
+// mask has. `splits` is the launcher's.
+struct CrossAttend {
+    const uint16_t* q;
+    const uint16_t* k;
+    const uint16_t* v;
+    uint16_t* out;
+    const int* starts;
+    const int* lengths;
+    const uint8_t* mask;
+    int64_t q_token, q_head, k_request, k_state, k_head, v_request, v_state, v_head, mask_request;
+    int tokens, requests, each, states, kv_heads, q_heads, group, width;
+    float scale;
+    bool half;
+    float* work;
+    int splits;
+};
+// Bytes of workspace; `most`: the most rows a request has, as far as the caller knows (0: not at all).
+int64_t cross_attend_work(int64_t tokens, int group, int requests, int kv_heads, int states, int width, int64_t most);
+hipError_t cross_attend(CrossAttend p, int64_t most, hipStream_t s);
+
 // The most rows, table rows or cache slots that the head and cache kernels index: int32 with room.
 constexpr int kMostTokens = 1 << 30;
 // The most requests a plan takes: four prefix sums of them in 64 KiB of LDS.

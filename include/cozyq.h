@@ -585,6 +585,24 @@ int cozyq_cache_attend(int device, int fp8, const void* q, int half, int64_t tok
                        int requests, int table_width, const int* starts, const int* lengths, int64_t most, float scale,
                        int causal, int window, void* out, void* workspace, void* stream);
 
+/* Attention of a decoder's rows to an encoder's states (no reference counterpart on the quantized-linear path): q
+ * [tokens, q_heads, width], k and v [requests, states, kv_heads, width], 16-bit, by strides in elements (multiples of
+ * 8, states less than 2^23 apart; elements dense; 16-byte aligned), query heads in equal groups a key head; width a
+ * multiple of 8 up to 256. Request b's rows are starts[b] .. starts[b + 1] − 1 (int32 [requests + 1], ascending; NULL:
+ * tokens / requests each); it sees the first lengths[b] of its states (int32 [requests]; NULL: all) that mask has
+ * (bytes [requests, states], mask_request apart, nonzero: seen; NULL: all). out [tokens, q_heads, width], contiguous:
+ * softmax(scale · q·k) · v over what is seen; 0 where nothing is and for a row of no request. Nothing of a state that
+ * is not seen reaches a result, whatever it holds. `most`: the most rows a request has, as far as the caller knows
+ * (0: not at all); it sets the launch's shape and speed, never its results. The workspace is of
+ * cozyq_cross_attend_workspace_bytes bytes, uninitialised (NULL where that is 0; -1 for a bad argument). */
+int64_t cozyq_cross_attend_workspace_bytes(int64_t tokens, int q_heads, int requests, int states, int kv_heads, int width,
+                                           int64_t most);
+int cozyq_cross_attend(int device, const void* q, int half, int64_t tokens, int q_heads, int64_t q_token, int64_t q_head,
+                       const void* k, const void* v, int requests, int states, int kv_heads, int width, int64_t k_request,
+                       int64_t k_state, int64_t k_head, int64_t v_request, int64_t v_state, int64_t v_head,
+                       const int* starts, const int* lengths, const void* mask, int64_t mask_request, int64_t most,
+                       float scale, void* out, void* workspace, void* stream);
+
 /* Test entries (no reference counterpart): the kernels' scalar conversions run on the host,
  * so CPU tests can hold the device code's arithmetic against torch without a GPU. */
 void cozyq_host_e4m3(const float* in, uint8_t* out, int64_t n);

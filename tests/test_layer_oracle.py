@@ -104,3 +104,22 @@ def test_operators_refuse_tensors_off_the_gpu_and_unknown_operands():
     x = torch.zeros(2, 256, dtype=torch.bfloat16)
     with pytest.raises(ValueError):
         norms.add_rms(torch, x, x, None)
+
+
+def test_cross_entry_refuses_bad_arguments_before_the_device():
+    lib = _lib.load()
+    keep, p = _buffer()
+
+    def call(q=p, tokens=4, q_heads=4, q_token=256, k=p, v=p, requests=2, states=8, kv_heads=2, width=64, k_state=128, v_state=128,
+             starts=p, most=0, out=p, k_head=64):  # fmt: skip
+        return lib.cozyq_cross_attend(0, q, 0, tokens, q_heads, q_token, 64, k, v, requests, states, kv_heads, width, 1024, k_state,
+                                      k_head, 1024, v_state, 64, starts, p, None, 0, most, 0.1, out, None, None)  # fmt: skip
+
+    for bad in (dict(q=None), dict(q=p + 2), dict(k=None), dict(v=p + 8), dict(out=None), dict(out=p + 4), dict(tokens=-1), dict(tokens=2**30 + 1),
+                dict(tokens=2**29, q_heads=8), dict(q_heads=3), dict(q_heads=0), dict(kv_heads=0), dict(requests=0), dict(requests=65536),
+                dict(states=-1), dict(width=0), dict(width=12), dict(width=264), dict(q_token=100), dict(k_state=100), dict(k_head=4),
+                dict(k_state=1 << 23), dict(v_state=-8), dict(most=-1), dict(starts=None, tokens=5)):  # fmt: skip
+        assert call(**bad) == INVALID, bad
+    assert call(tokens=0) == 0
+    size = lib.cozyq_cross_attend_workspace_bytes
+    assert size(4, 4, 0, 8, 2, 64, 0) == -1 and size(4, 4, 2, 8, 2, 64, -1) == -1 and size(4, 4, 2, 8, 2, 64, 0) == 0
