@@ -919,7 +919,7 @@ int cozyq_cross_attend(int device, const void* q, int half, int64_t tokens, int 
                                 static_cast<const uint8_t*>(mask), q_token, q_head, k_request, k_state, k_head, v_request,
                                 v_state, v_head, mask_request, static_cast<int>(tokens), requests,
                                 starts ? 0 : static_cast<int>(tokens / requests), states, kv_heads, q_heads,
-                                q_heads / kv_heads, width, scale, half != 0, static_cast<float*>(workspace), 1},
+                                q_heads / kv_heads, width, scale, half != 0, static_cast<float*>(workspace), 1, 0, 0},
                                most, on(stream));
 }
 

@@ -20,6 +20,7 @@ namespace {
 
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 LdsFour;
 
@@ -73,6 +74,29 @@ __device__ __forceinline__ Rows rows_of(const CrossAttend& p, int b) {
     return r;
 }
 
+// Tiles and steps of a call are fewer than kMany, and sums end there, so that no `starts`, in order or not, carries an
+// index past its request.
+constexpr int kMany = 1 << 30;
+
+// x from the lane that DPP control kCtrl names, 0 where it names none or the row is masked out.
+template <int kCtrl, int kRowMask>
+__device__ __forceinline__ uint32_t dpp_or_zero(uint32_t x) {
+    return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), kCtrl, kRowMask, 0xF, false));
+}
+
+// Inclusive sums over a wave of numbers of up to kMany: within rows of 16 lanes, then a row's last sum into the next.
+__device__ __forceinline__ int wave_prefix(int n) {
+    const uint32_t most = kMany;
+    uint32_t x = static_cast<uint32_t>(n);
+    x = min(x + dpp_or_zero<0x111, 0xF>(x), most);  // row_shr:1
+    x = min(x + dpp_or_zero<0x112, 0xF>(x), most);  // row_shr:2
+    x = min(x + dpp_or_zero<0x114, 0xF>(x), most);  // row_shr:4
+    x = min(x + dpp_or_zero<0x118, 0xF>(x), most);  // row_shr:8
+    x = min(x + dpp_or_zero<0x142, 0xA>(x), most);  // row_bcast:15 into rows 1 and 3
+    x = min(x + dpp_or_zero<0x143, 0xC>(x), most);  // row_bcast:31 into rows 2 and 3
+    return static_cast<int>(x);
+}
+
 // The tile number `id` of all requests' row tiles of kRows rows, one request after another; false past the last.
 template <int kRows>
 __device__ bool find_tile(const CrossAttend& p, int id, int& request, int& tile, int& count) {
@@ -82,22 +106,17 @@ __device__ bool find_tile(const CrossAttend& p, int id, int& request, int& tile,
         int tiles = 0;
         if (base + lane < p.requests)
             tiles = static_cast<int>((static_cast<int64_t>(rows_of(p, base + lane).count) * p.group + kRows - 1) / kRows);
-        int sum = tiles;
-#pragma unroll
-        for (int step = 1; step < 64; step *= 2) {
-            const int other = __shfl_up(sum, step);
-            if (lane >= step) sum += other;
-        }
-        const uint64_t past = __ballot(before + sum > id);
+        const int sum = wave_prefix(tiles);
+        const uint64_t past = __ballot(min(before, kMany) - id > -sum);
         if (past) {
             const int at = __ffsll(static_cast<unsigned long long>(past)) - 1;
             request = base + at;
             tile = id - before - (__builtin_amdgcn_readlane(sum, at) - __builtin_amdgcn_readlane(tiles, at));
             return true;
         }
-        before += __builtin_amdgcn_readlane(sum, 63);
+        before = min(before, kMany) + __builtin_amdgcn_readlane(sum, 63);
     }
-    count = before;
+    count = min(before, kMany);
     return false;
 }
 
@@ -112,24 +131,13 @@ __device__ void clear_rest(const CrossAttend& p, int busy) {
         reinterpret_cast<i32x4*>(p.out)[i < from ? i : i - from + after] = i32x4{0, 0, 0, 0};
 }
 
-// Four elements of a row's result from d on, of the sums v with the denominator `total`: the result, or this split's
-// part of it with its reference `ref`. `some`: whether a state was seen; nothing seen is 0, nothing but scores of minus
-// infinity the quotient 0 / 0.
-template <int kWidth, bool kHalf>
-__device__ __forceinline__ void store_row(const CrossAttend& p, int split, int64_t at, int d, f32x4 v, float ref, float total, bool some) {
-    if (p.splits == 1) {
-        if (d >= p.width) return;
-        const float inv = some ? 1.0f / total : 0.0f;
-        *reinterpret_cast<i32x2*>(p.out + at * p.width + d) = i32x2{pack2<kHalf>(v[0] * inv, v[1] * inv), pack2<kHalf>(v[2] * inv, v[3] * inv)};
-    } else {
-        const int64_t places = static_cast<int64_t>(p.tokens) * p.q_heads;
-        *reinterpret_cast<f32x4*>(p.work + (split * places + at) * kWidth + d) = v;
-        if (d == 0) {
-            float* parts = p.work + p.splits * places * kWidth + 2 * (split * places + at);
-            parts[0] = some ? ref : -__builtin_inff();
-            parts[1] = total;
-        }
-    }
+// Four elements of a row's result from d on, of the sums v with the denominator `total`. `some`: whether a state was
+// seen; nothing seen is 0, nothing but scores of minus infinity the quotient 0 / 0.
+template <bool kHalf>
+__device__ __forceinline__ void store_row(const CrossAttend& p, int64_t at, int d, f32x4 v, float total, bool some) {
+    if (d >= p.width) return;
+    const float inv = some ? 1.0f / total : 0.0f;
+    *reinterpret_cast<i32x2*>(p.out + at * p.width + d) = i32x2{pack2<kHalf>(v[0] * inv, v[1] * inv), pack2<kHalf>(v[2] * inv, v[3] * inv)};
 }
 
 // A view of `left` rows (none below 1) of `width` 16-bit elements, `stride` apart, from `base` on: what lies past them
@@ -343,9 +351,19 @@ __global__ __launch_bounds__(64 * kWaves, kWidth == 256 ? 1 : 2) void cross_kern
 #pragma unroll
     for (int o = 0; o < kOut; ++o) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            store_row<kWidth, kHalf>(p, split, at, 32 * o + 8 * i + 4 * h, f32x4{acc[o][4 * i], acc[o][4 * i + 1], acc[o][4 * i + 2], acc[o][4 * i + 3]},
-                                     bound > 0.0f ? ref : kNoScore, total, any);
+        for (int i = 0; i < 4; ++i) {
+            const f32x4 v = {acc[o][4 * i], acc[o][4 * i + 1], acc[o][4 * i + 2], acc[o][4 * i + 3]};
+            const int d = 32 * o + 8 * i + 4 * h;
+            if (p.splits == 1) {
+                store_row<kHalf>(p, at, d, v, total, any);
+            } else {
+                const int64_t places = static_cast<int64_t>(p.tokens) * p.q_heads;
+                *reinterpret_cast<f32x4*>(p.work + (split * places + at) * kWidth + d) = v;
+                if (d == 0)
+                    *reinterpret_cast<f32x2*>(p.work + p.splits * places * kWidth + 2 * (split * places + at)) =
+                        f32x2{any ? (bound > 0.0f ? ref : kNoScore) : -__builtin_inff(), total};
+            }
+        }
     }
 }
 
@@ -367,16 +385,121 @@ __device__ __forceinline__ void wave_sync() {
     fence();
 }
 
-// Waves of a workgroup: as many as leave each the registers that it needs.
-constexpr int few_waves(int width, int tiles) { return width * tiles > 128 ? 4 : 8; }
+// The eight XCDs take workgroups in turn: one share's heads begin further on than the last one's, so that each XCD reads
+// rows of all key heads at a time. One head's rows alone, which are the heads' number times their bytes apart, may all
+// lie in one of the 16 channels of an XCD's L2.
+__device__ __forceinline__ int turn(int share, int kv_heads) { return (kv_heads >= 8 ? share : share / (8 / kv_heads)) % kv_heads; }
 
-// kWaves waves take the rows of one request and key head, 16 · kTiles at a time, over a share of its states: each wave
-// every kWaves-th step of 32, by itself. Keys go from memory into registers as the matrix unit wants them, values
-// through a tile of the wave's own in LDS, whose transposed read makes them the second product's operand. The waves'
-// sums are joined in LDS.
+// Few rows' work is the steps of 32 states of all row tiles, one tile after another, the same for every key head: cut
+// into `shares` equal runs, one a workgroup and head, wherever the cuts fall, so that requests of any lengths keep
+// every CU at its share of the reading (one CU alone draws some 30 GB/s). A workgroup takes the end of one tile,
+// whole tiles and the beginning of another, and leaves sums to be joined for the first and the last alone: two places
+// each.
+constexpr int kFewStep = 32;
+// The loads' mark of what is read once.
+constexpr int kOnce = 2;
+// Steps of a tile that are not cut, and those of a run at the least.
+constexpr int kWholeSteps = 24, kLeastSteps = 8;
+
+// A request's row tiles, and a tile's steps: at the least one, so that a tile that sees nothing is written too.
+struct Extent {
+    int tiles, steps;
+    Rows of;
+};
+
+template <int kRows>
+__device__ __forceinline__ Extent extent_of(const CrossAttend& p, int b) {
+    if (b >= p.requests) return {0, 0, {0, 0, 0}};
+    const Rows r = rows_of(p, b);
+    const int steps = max(1, (r.length + kFewStep - 1) / kFewStep);
+    return {min((r.count * p.group + kRows - 1) / kRows, kMany / steps), steps, r};
+}
+
+// How the steps are cut: runs of `run`, at the least p.cut. Where runs of p.cut are few enough even if none of them holds
+// two tiles' steps (`apart`), none does: the second tile would only wait for the first. Without cuts a run is a tile.
+struct Cuts {
+    Extent first;  // of the lane's request among the first 64
+    int run;
+    bool apart;
+};
+
+template <int kRows>
+__device__ __forceinline__ Extent extent_at(const CrossAttend& p, const Cuts& c, int base) {
+    return base == 0 ? c.first : extent_of<kRows>(p, base + static_cast<int>(threadIdx.x & 63));
+}
+
+// A tile's steps as they are counted.
+__device__ __forceinline__ int counted(const Extent& e, const Cuts& c) {
+    return c.apart ? (e.steps + c.run - 1) / c.run * c.run : e.steps;
+}
+
+template <int kRows>
+__device__ Cuts cuts_of(const CrossAttend& p) {
+    Cuts c = {extent_of<kRows>(p, threadIdx.x & 63), 1, !p.cut};
+    if (!p.cut) {
+        c.run = kMany;
+        return c;
+    }
+    int total = 0, runs = 0;
+    bool longer = false;
+    for (int base = 0; base < p.requests; base += 64) {
+        const Extent e = extent_at<kRows>(p, c, base);
+        longer |= __any(e.steps > kWholeSteps);
+        total = min(total, kMany) + __builtin_amdgcn_readlane(wave_prefix(e.tiles * e.steps), 63);
+        runs = min(runs, kMany) + __builtin_amdgcn_readlane(wave_prefix(e.tiles * ((e.steps + p.cut - 1) / p.cut)), 63);
+    }
+    c.apart = runs <= p.shares;
+    c.run = c.apart ? (longer ? p.cut : kWholeSteps) : max(p.cut, min(total, kMany) / p.shares + 1);
+    return c;
+}
+
+// A row tile: its request, its number there, its first step among all, its steps.
+struct Item {
+    int request, tile, start, steps;
+    Rows of;
+};
+
+// The tile that step `id` is of (kByStep), or tile number `id`; false past the last.
+template <int kRows, bool kByStep>
+__device__ bool find_item(const CrossAttend& p, const Cuts& c, int id, Item& out) {
+    int ids_before = 0, steps_before = 0;
+    for (int base = 0; base < p.requests; base += 64) {
+        const Extent e = extent_at<kRows>(p, c, base);
+        const int one = p.cut ? counted(e, c) : 0;
+        const int steps = wave_prefix(e.tiles * one), tiles = wave_prefix(e.tiles);
+        const int ids = kByStep ? steps : tiles;
+        const uint64_t past = __ballot(min(ids_before, kMany) - id > -ids);
+        if (past) {
+            const int at = __ffsll(static_cast<unsigned long long>(past)) - 1;
+            const int n = __builtin_amdgcn_readlane(one, at), t = __builtin_amdgcn_readlane(e.tiles, at);
+            const int from = id - ids_before - __builtin_amdgcn_readlane(ids, at) + (kByStep ? t * n : t);
+            const int tile = kByStep ? from / n : from;
+            out = {base + at, tile, steps_before + __builtin_amdgcn_readlane(steps, at) - (t - tile) * n, __builtin_amdgcn_readlane(e.steps, at),
+                   {__builtin_amdgcn_readlane(e.of.first, at), __builtin_amdgcn_readlane(e.of.count, at), __builtin_amdgcn_readlane(e.of.length, at)}};
+            return true;
+        }
+        ids_before = min(ids_before, kMany) + __builtin_amdgcn_readlane(ids, 63);
+        steps_before = min(steps_before, kMany) + __builtin_amdgcn_readlane(steps, 63);
+    }
+    return false;
+}
+
+// The place of a part of kRows rows: their sums, then their references and denominators.
+template <int kWidth, int kRows>
+__device__ __forceinline__ float* place_of(const CrossAttend& p, int place, int kv) {
+    return p.work + (static_cast<int64_t>(place) * p.kv_heads + kv) * (kRows * (kWidth + 2));
+}
+
+// kWaves waves take a run of steps of one key head, a row tile of 16 · kTiles rows at a time: each wave
+// every kWaves-th step by itself. Keys and values go in whole lines through registers and then, one after the other,
+// through a tile of the wave's own in LDS, from which they are read as the matrix unit wants them, values by a transposed
+// read. (Keys loaded as the first product's operand, 64 bytes of 16 rows at a time: 35.4 us for 32.9, 24 requests over 1600
+// states each.) The waves' sums are joined in LDS.
+// Bound by memory: those 157 MB at 4.8 TB/s, where reads alone of the same rows, 256 bytes at a stride of 4 KiB, reach
+// 5.1 to 5.5; before the first of them 4 us of launch and search.
 template <int kWidth, int kTiles, bool kHalf>
-__global__ __launch_bounds__(64 * few_waves(kWidth, kTiles), few_waves(kWidth, kTiles) / 4) void cross_few_kernel(CrossAttend p) {
-    constexpr int kWaves = few_waves(kWidth, kTiles), kStep = 32, kDepth = kWidth / 32, kOut = kWidth / 16, kRows = 16 * kTiles;
+__global__ __launch_bounds__(256, kWidth * kTiles > 128 ? 1 : kWidth * kTiles == 64 ? 4 : 2) void cross_few_kernel(CrossAttend p) {
+    constexpr int kWaves = 4, kStep = kFewStep, kDepth = kWidth / 32, kOut = kWidth / 16, kRows = 16 * kTiles;
     constexpr int kChunks = kWidth / 8, kPerLoad = 64 / kChunks, kLoads = kStep / kPerLoad;
     constexpr int kPad = kWidth + 4;
     __shared__ __attribute__((aligned(1024))) float merged[kWaves][16 * kPad];
@@ -384,29 +507,36 @@ __global__ __launch_bounds__(64 * few_waves(kWidth, kTiles), few_waves(kWidth, k
     static_assert(16 * kPad * 4 >= kStep * kWidth * 2, "a tile of values fits the place of a wave's sums");
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, g = lane >> 4;
-    const int kv = blockIdx.x % p.kv_heads, id = blockIdx.x / p.kv_heads, request = id / p.splits, split = id % p.splits;
-    const Rows of = rows_of(p, request);
-    const int rows = of.count * p.group, length = of.length;
-    const int steps = (length + kStep - 1) / kStep;
-    const int begin = static_cast<int>(static_cast<int64_t>(steps) * split / p.splits);
-    const int end = static_cast<int>(static_cast<int64_t>(steps) * (split + 1) / p.splits);
-    const uint16_t* k_base = p.k + request * p.k_request + kv * p.k_head;
-    const uint16_t* v_base = p.v + request * p.v_request + kv * p.v_head;
-    const __amdgpu_buffer_rsrc_t mask = __builtin_amdgcn_make_buffer_rsrc(
-        const_cast<uint8_t*>(p.mask ? p.mask + request * p.mask_request : nullptr), 0, p.mask ? length : 0, 0x00020000);
     const float sharp = p.scale * kLog2e;
-    uint8_t* const values = reinterpret_cast<uint8_t*>(merged[wave]);
+    uint8_t* const tile = reinterpret_cast<uint8_t*>(merged[wave]);
+    const int share = blockIdx.x / p.kv_heads, kv = (blockIdx.x % p.kv_heads + turn(share, p.kv_heads)) % p.kv_heads;
 
-    uint32_t k_from[kDepth];
+    int k_at[kDepth];
 #pragma unroll
-    for (int b = 0; b < kDepth; ++b)
-        k_from[b] = 32 * b + 8 * g < p.width ? 2u * (col * static_cast<uint32_t>(p.k_state) + 32 * b + 8 * g) : kNowhere;
+    for (int b = 0; b < kDepth; ++b) k_at[b] = col * 2 * kWidth + 16 * key_place<kWidth>(col, 4 * b + g);
     const int v_row = 4 * g + col / 4, v_piece = (col & 3) / 2;
     int v_at[kOut];
 #pragma unroll
     for (int o = 0; o < kOut; ++o) v_at[o] = v_row * 2 * kWidth + 16 * value_place<kWidth>(v_row, 2 * o + v_piece) + 8 * (col & 1);
 
-    for (int row0 = 0; row0 < rows; row0 += kRows) {
+    const Cuts cuts = cuts_of<kRows>(p);
+    const int run_from = static_cast<int>(min(static_cast<int64_t>(share) * cuts.run, static_cast<int64_t>(kMany)));
+    int at = p.cut ? run_from : 0, run_to = p.cut ? run_from + cuts.run : 1;
+    Item item;
+    while (at < run_to) {
+        if (p.cut ? !find_item<kRows, true>(p, cuts, at, item) : !find_item<kRows, false>(p, cuts, share, item)) break;
+        if (!p.cut) run_to = item.steps;
+        const int request = item.request, begin = at - item.start, last = min(item.steps, run_to - item.start);
+        const bool whole = begin == 0 && last == item.steps;
+        const int part = 2 * share + (begin == 0 && at != run_from ? 1 : 0);
+        at = cuts.apart ? run_to : item.start + last;
+        const Rows of = item.of;
+        const int length = of.length, row0 = kRows * item.tile, rows = min(of.count * p.group, row0 + kRows);
+        const int end = min(last, (length + kStep - 1) / kStep);
+        const uint16_t* k_base = p.k + request * p.k_request + kv * p.k_head;
+        const uint16_t* v_base = p.v + request * p.v_request + kv * p.v_head;
+        const __amdgpu_buffer_rsrc_t mask = __builtin_amdgcn_make_buffer_rsrc(
+            const_cast<uint8_t*>(p.mask ? p.mask + request * p.mask_request : nullptr), 0, p.mask ? length : 0, 0x00020000);
         i32x4 q[kTiles][kDepth];
 #pragma unroll
         for (int n = 0; n < kTiles; ++n) {
@@ -427,51 +557,53 @@ __global__ __launch_bounds__(64 * few_waves(kWidth, kTiles), few_waves(kWidth, k
         }
         bool any = false;
 
-        i32x4 k_raw[2][kDepth], v_raw[kLoads];
+        i32x4 k_raw[kLoads], v_raw[kLoads];
         uint8_t shown = 0;
         const auto load_keys = [&](int step) {
             const int64_t t0 = static_cast<int64_t>(step) * kStep;
-            const __amdgpu_buffer_rsrc_t kr =
-                states_view(k_base + t0 * p.k_state, static_cast<int>(min(length - t0, static_cast<int64_t>(kStep))), p.k_state, p.width);
+            const __amdgpu_buffer_rsrc_t kr = states_view(k_base + t0 * p.k_state, static_cast<int>(step < end ? min(length - t0, static_cast<int64_t>(kStep)) : 0), p.k_state, p.width);
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-#pragma unroll
-                for (int b = 0; b < kDepth; ++b)
-                    k_raw[j][b] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(
-                        kr, k_from[b] + j * 32u * static_cast<uint32_t>(p.k_state), 0, 0));
+            for (int i = 0; i < kLoads; ++i) {
+                const int r = i * kPerLoad + lane / kChunks, c = key_place<kWidth>(r, lane % kChunks);
+                k_raw[i] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                    kr, 8 * c < p.width ? 2u * (r * static_cast<uint32_t>(p.k_state) + 8 * c) : kNowhere, 0, kOnce));
             }
         };
         const auto load_values = [&](int step) {
             const int64_t t0 = static_cast<int64_t>(step) * kStep;
             const __amdgpu_buffer_rsrc_t vr =
-                states_view(v_base + t0 * p.v_state, static_cast<int>(min(length - t0, static_cast<int64_t>(kStep))), p.v_state, p.width);
+                states_view(v_base + t0 * p.v_state, static_cast<int>(step < end ? min(length - t0, static_cast<int64_t>(kStep)) : 0), p.v_state, p.width);
             shown = __builtin_amdgcn_raw_buffer_load_b8(mask, static_cast<int>(min(t0, static_cast<int64_t>(length))) + lane, 0, 0);
 #pragma unroll
             for (int i = 0; i < kLoads; ++i) {
                 const int r = i * kPerLoad + lane / kChunks, c = value_place<kWidth>(r, lane % kChunks);
                 v_raw[i] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(
-                    vr, 8 * c < p.width ? 2u * (r * static_cast<uint32_t>(p.v_state) + 8 * c) : kNowhere, 0, 0));
+                    vr, 8 * c < p.width ? 2u * (r * static_cast<uint32_t>(p.v_state) + 8 * c) : kNowhere, 0, kOnce));
             }
         };
-        if (begin + wave < end) {
-            load_keys(begin + wave);
-            load_values(begin + wave);
-        }
+        load_keys(begin + wave);
+        load_values(begin + wave);
         for (int step = begin + wave; step < end; step += kWaves) {
             const uint32_t seen = static_cast<uint32_t>(__ballot(step * kStep + lane < length && (!p.mask || shown)));
             any |= seen != 0;
+            wave_sync();  // the last step's reads
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) *reinterpret_cast<i32x4*>(tile + 1024 * i + 16 * lane) = k_raw[i];
+            load_keys(step + kWaves);
+            wave_sync();
             f32x4 s[kTiles][2];
 #pragma unroll
-            for (int n = 0; n < kTiles; ++n) {
+            for (int n = 0; n < kTiles; ++n) s[n][0] = s[n][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int b = 0; b < kDepth; ++b) {
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    s[n][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                    const i32x4 k = *reinterpret_cast<const i32x4*>(tile + k_at[b] + 32 * kWidth * j);
 #pragma unroll
-                    for (int b = 0; b < kDepth; ++b) s[n][j] = mfma16<kHalf>(k_raw[j][b], q[n][b], s[n][j]);
+                    for (int n = 0; n < kTiles; ++n) s[n][j] = mfma16<kHalf>(k, q[n][b], s[n][j]);
                 }
             }
-            load_keys(step + kWaves);
-            wave_sync();  // the last step's reads
+            wave_sync();  // the keys' reads
 #pragma unroll
             for (int i = 0; i < kLoads; ++i) {
                 i32x4 raw = v_raw[i];
@@ -479,7 +611,7 @@ __global__ __launch_bounds__(64 * few_waves(kWidth, kTiles), few_waves(kWidth, k
                     rarely();
                     if (!((seen >> (i * kPerLoad + lane / kChunks)) & 1)) raw = i32x4{0, 0, 0, 0};
                 }
-                *reinterpret_cast<i32x4*>(values + 1024 * i + 16 * lane) = raw;
+                *reinterpret_cast<i32x4*>(tile + 1024 * i + 16 * lane) = raw;
             }
             load_values(step + kWaves);
             i32x4 w[kTiles];
@@ -521,8 +653,8 @@ __global__ __launch_bounds__(64 * few_waves(kWidth, kTiles), few_waves(kWidth, k
             wave_sync();
 #pragma unroll
             for (int o = 0; o < kOut; ++o) {
-                const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsFour*)(values + v_at[o]));
-                const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsFour*)(values + v_at[o] + 32 * kWidth));
+                const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsFour*)(tile + v_at[o]));
+                const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsFour*)(tile + v_at[o] + 32 * kWidth));
                 const i32x2 l2 = __builtin_bit_cast(i32x2, lo), h2 = __builtin_bit_cast(i32x2, hi);
 #pragma unroll
                 for (int n = 0; n < kTiles; ++n) acc[n][o] = mfma16<kHalf>(i32x4{l2[0], l2[1], h2[0], h2[1]}, w[n], acc[n][o]);
@@ -536,9 +668,8 @@ __global__ __launch_bounds__(64 * few_waves(kWidth, kTiles), few_waves(kWidth, k
             if (n) __syncthreads();
             total[n] += __shfl_xor(total[n], 16);
             total[n] += __shfl_xor(total[n], 32);
-            const float top = bound[n] > 0.0f ? ref[n] : kNoScore;
             if (g == 0) {
-                tops[wave][col] = top;
+                tops[wave][col] = bound[n] > 0.0f ? ref[n] : kNoScore;
                 totals[wave][col] = total[n];
             }
 #pragma unroll
@@ -557,13 +688,77 @@ __global__ __launch_bounds__(64 * few_waves(kWidth, kTiles), few_waves(kWidth, k
                     v += *reinterpret_cast<const f32x4*>(&merged[w][r * kPad + d]) * factor;
                     sum += totals[w][r] * factor;
                 }
-                const int64_t at = static_cast<int64_t>(of.first + (first + r) / p.group) * p.q_heads + kv * p.group + (first + r) % p.group;
-                store_row<kWidth, kHalf>(p, split, at, d, v, most, sum, some);
+                if (whole) {
+                    const int row = first + r;
+                    store_row<kHalf>(p, static_cast<int64_t>(of.first + row / p.group) * p.q_heads + kv * p.group + row % p.group, d, v, sum, some);
+                } else {
+                    float* to = place_of<kWidth, kRows>(p, part, kv);
+                    *reinterpret_cast<f32x4*>(to + (16 * n + r) * kWidth + d) = v;
+                    if (d == 0) *reinterpret_cast<f32x2*>(to + kRows * kWidth + 2 * (16 * n + r)) = f32x2{some ? most : -__builtin_inff(), sum};
+                }
             }
         }
-        if (row0 + kRows < rows) __syncthreads();
+        __syncthreads();
     }
-    if (p.starts && p.splits == 1) clear_rest(p, 0);
+    if (p.starts) clear_rest(p, 0);
+}
+
+// Joins the parts of few rows' tiles that runs cut: a workgroup a tile and key head.
+template <int kWidth, int kRows>
+__global__ __launch_bounds__(256) void cross_few_join_kernel(CrossAttend p) {
+    constexpr int kEach = kWidth / 4;
+    const int kv = blockIdx.x % p.kv_heads;
+    const Cuts cuts = cuts_of<kRows>(p);
+    const int run = cuts.run;
+    Item item;
+    if (!find_item<kRows, false>(p, cuts, blockIdx.x / p.kv_heads, item)) return;
+    const int first = item.start / run, last = (item.start + item.steps - 1) / run;
+    if (first == last) return;  // whole
+    const Rows of = item.of;
+    const int row0 = kRows * item.tile, count = min(kRows, of.count * p.group - row0);
+    // Each wave takes every fourth part of a row, 64 / kEach rows at a time; then the waves' sums are joined in LDS.
+    constexpr int kSide = kEach < 64 ? 64 / kEach : 1;
+    __shared__ f32x4 sums[4][64];
+    __shared__ f32x2 rests[4][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (int r0 = 0; r0 < count; r0 += kSide) {
+        const int r = min(r0 + lane / kEach, count - 1), d = 4 * (lane % kEach);
+        const auto part = [&](int share) { return place_of<kWidth, kRows>(p, 2 * share + (share == first && item.start % run ? 1 : 0), kv); };
+        float most = -__builtin_inff(), total = 0.0f;
+        f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+        for (int share = first + wave; share <= last; share += 4) {
+            const float* from = part(share);
+            const f32x2 rest = *reinterpret_cast<const f32x2*>(from + kRows * kWidth + 2 * r);
+            const f32x4 one = *reinterpret_cast<const f32x4*>(from + r * kWidth + d);
+            const float up = nan_max(most, rest[0]);
+            // Nothing seen so far, and here: minus infinity less itself is no reference.
+            const float old = most == up ? 1.0f : __builtin_amdgcn_exp2f(most - up), factor = rest[0] == up ? 1.0f : __builtin_amdgcn_exp2f(rest[0] - up);
+            total = total * old + rest[1] * factor;
+            v = v * old + one * factor;
+            most = up;
+        }
+        sums[wave][lane] = v;
+        rests[wave][lane] = f32x2{most, total};
+        __syncthreads();
+        if (wave == 0 && r0 + lane / kEach < count) {
+#pragma unroll
+            for (int w = 1; w < 4; ++w) {
+                const f32x2 rest = rests[w][lane];
+                const float up = nan_max(most, rest[0]);
+                const float old = most == up ? 1.0f : __builtin_amdgcn_exp2f(most - up), factor = rest[0] == up ? 1.0f : __builtin_amdgcn_exp2f(rest[0] - up);
+                total = total * old + rest[1] * factor;
+                v = v * old + sums[w][lane] * factor;
+                most = up;
+            }
+            const int row = row0 + r;
+            const int64_t at = static_cast<int64_t>(of.first + row / p.group) * p.q_heads + kv * p.group + row % p.group;
+            const bool some = most != -__builtin_inff();
+            if (p.half) store_row<true>(p, at, d, v, total, some);
+            else store_row<false>(p, at, d, v, total, some);
+        }
+        __syncthreads();
+    }
 }
 
 // Joins a row's parts, kWidth / 4 threads a row: Σ sums · 2^(ref − most) over Σ totals · 2^(ref − most).
@@ -602,49 +797,68 @@ constexpr int waves_of(int width) { return width == 256 ? 4 : 8; }
 // up to 128 wide.
 constexpr int64_t few_rows(int width) { return width > 128 ? 16 : 32; }
 
-// The shape of a call, which its workspace goes by too: the kernel, its rows a tile, and how many workgroups a tile's
-// states are split over.
+// Whether few rows' steps are cut into equal runs, which costs a second launch and a workgroup's search for its tiles,
+// some 8 us, or every tile is one workgroup's, which then draws 30 to 40 GB/s alone. Cut / whole, us, one row a request
+// and 32 heads over 8 of 128: 24 requests over 400 to 1601 states 29.4 / 27.2, over 1600 each 40.7 / 32.9; 6 over 1601 16.3 /
+// 25.3; 8 over 6400 41 / 90; 1 over 6400 17 / 80; 20 heads of 64 over 1500 11.0 / 16.8. Past 128 steps always: the
+// lengths, which are on the GPU, may be of very different sizes.
+bool few_cut(int64_t pairs, int64_t steps, int width) {
+    return steps > kWholeSteps && (steps > 128 || (256 - pairs) * steps * width > 4096 * 128);
+}
+
+// The shape of a call, which its workspace goes by too: the kernel, its rows a tile, and how its states are shared out.
 struct Shape {
     bool few;
-    int rows, splits;
+    int rows;
+    int64_t tiles;  // at the most, of a key head
+    int splits;     // many rows: workgroups of a tile
+    int cut, shares;  // few rows: a run's steps at the least (0: runs are tiles), runs at the most
+    int64_t floats;
 };
 
 Shape shape_of(int64_t tokens, int group, int requests, int kv_heads, int states, int width, int64_t most) {
     const int64_t rows = (most > 0 && most < tokens ? most : tokens) * group;
-    Shape a = {rows <= few_rows(width), 0, 1};
-    int64_t groups, step, wanted, least;
+    Shape a = {rows <= few_rows(width), 0, 0, 1, 0, 0, 0};
     if (a.few) {
         a.rows = rows > 16 ? 32 : 16;
-        groups = static_cast<int64_t>(requests) * kv_heads;
-        step = 32 * 8;
-        wanted = 512 / groups;
-        least = 4;
-    } else {
-        a.rows = 32 * waves_of(padded(width));
-        groups = ((tokens * group + a.rows - 1) / a.rows + requests - 1) * kv_heads;
-        step = step_of(padded(width));
-        wanted = 256 / groups;
-        least = 4;
+        a.tiles = tokens * group / a.rows + requests;
+        const int64_t steps = (states + kFewStep - 1) / kFewStep;
+        a.few = a.tiles * (steps + 1) < (1 << 30);
+        if (few_cut(static_cast<int64_t>(requests) * kv_heads, steps, padded(width))) {
+            const int64_t runs = a.tiles * ((steps + kLeastSteps - 1) / kLeastSteps), shares = max((padded(width) == 64 ? 1024 : 512) / kv_heads, 1);
+            a.cut = kLeastSteps;
+            a.shares = static_cast<int>(min(runs, shares));
+            a.floats = 2ll * a.shares * kv_heads * a.rows * (padded(width) + 2);
+        }
     }
-    const int64_t fit = (states + step - 1) / step / least;
-    const int64_t splits = wanted < fit ? wanted : fit;
-    a.splits = static_cast<int>(splits < 1 ? 1 : splits > 64 ? 64 : splits);
+    if (!a.few) {
+        a = {false, 32 * waves_of(padded(width)), 0, 1, 0, 0, 0};
+        a.tiles = (tokens * group + a.rows - 1) / a.rows + requests;
+        const int64_t step = step_of(padded(width)), steps = (states + step - 1) / step;
+        const int64_t splits = min(256 / (a.tiles * kv_heads), steps / 4);
+        a.splits = static_cast<int>(splits < 1 ? 1 : splits > 64 ? 64 : splits);
+        if (a.splits > 1) a.floats = a.splits * tokens * group * kv_heads * (padded(width) + 2);
+    }
     return a;
+}
+
+template <int kWidth, int kTiles, bool kHalf>
+void attend_few(const CrossAttend& p, const Shape& a, hipStream_t s) {
+    const unsigned groups = static_cast<unsigned>((a.cut ? a.shares : a.tiles) * p.kv_heads);
+    cross_few_kernel<kWidth, kTiles, kHalf><<<groups, 256, 0, s>>>(p);
+    if (a.cut) cross_few_join_kernel<kWidth, 16 * kTiles><<<static_cast<unsigned>(a.tiles * p.kv_heads), 256, 0, s>>>(p);
 }
 
 template <int kWidth, bool kHalf>
 hipError_t attend(const CrossAttend& p, const Shape& a, hipStream_t s) {
     if (a.few) {
-        const unsigned groups = static_cast<unsigned>(p.requests) * p.kv_heads * p.splits;
-        constexpr int kMost = few_rows(kWidth) / 16;
-        if (a.rows == 16) cross_few_kernel<kWidth, 1, kHalf><<<groups, 64 * few_waves(kWidth, 1), 0, s>>>(p);
-        else cross_few_kernel<kWidth, kMost, kHalf><<<groups, 64 * few_waves(kWidth, kMost), 0, s>>>(p);
-    } else {
-        constexpr int kWaves = waves_of(kWidth), kRows = 32 * kWaves;
-        const int64_t tiles = (static_cast<int64_t>(p.tokens) * p.group + kRows - 1) / kRows + p.requests;
-        const unsigned groups = static_cast<unsigned>(tiles * p.kv_heads * p.splits);
-        cross_kernel<kWidth, kWaves, kHalf><<<groups, 64 * kWaves, 0, s>>>(p);
+        if (a.rows == 16) attend_few<kWidth, 1, kHalf>(p, a, s);
+        else attend_few<kWidth, few_rows(kWidth) / 16, kHalf>(p, a, s);
+        return hipGetLastError();
     }
+    constexpr int kWaves = waves_of(kWidth);
+    const unsigned groups = static_cast<unsigned>(a.tiles * p.kv_heads * p.splits);
+    cross_kernel<kWidth, kWaves, kHalf><<<groups, 64 * kWaves, 0, s>>>(p);
     if (p.splits > 1) {
         const int64_t rows = static_cast<int64_t>(p.tokens) * p.q_heads;
         constexpr int kEach = 256 / (kWidth / 4);
@@ -661,13 +875,14 @@ hipError_t attend(const CrossAttend& p, const Shape& a, hipStream_t s) {
 }  // namespace
 
 int64_t cross_attend_work(int64_t tokens, int group, int requests, int kv_heads, int states, int width, int64_t most) {
-    const int64_t splits = shape_of(tokens, group, requests, kv_heads, states, width, most).splits;
-    return splits == 1 ? 0 : 4 * splits * tokens * group * kv_heads * (padded(width) + 2);
+    return 4 * shape_of(tokens, group, requests, kv_heads, states, width, most).floats;
 }
 
 hipError_t cross_attend(CrossAttend p, int64_t most, hipStream_t s) {
     const Shape a = shape_of(p.tokens, p.group, p.requests, p.kv_heads, p.states, p.width, most);
     p.splits = a.splits;
+    p.cut = a.cut;
+    p.shares = a.shares;
     const int width = padded(p.width);
     if (width == 64) return attend<64>(p, a, s);
     if (width == 128) return attend<128>(p, a, s);

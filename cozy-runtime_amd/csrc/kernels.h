@@ -341,7 +341,7 @@ hipError_t add_rms(const AddRms& p, bool fp8, hipStream_t s);
 
 // Attention to an encoder's states (cozyq_cross_attend): request b's rows are starts[b] .. starts[b + 1] − 1 (no
 // starts: `each` rows a request), its states the first lengths[b] (no lengths: all) of `states` that its row of the
-// mask has. `splits` is the launcher's.
+// mask has. `splits`, `cut` and `shares` are the launcher's.
 struct CrossAttend {
     const uint16_t* q;
     const uint16_t* k;
@@ -355,7 +355,7 @@ struct CrossAttend {
     float scale;
     bool half;
     float* work;
-    int splits;
+    int splits, cut, shares;
 };
 // Bytes of workspace; `most`: the most rows a request has, as far as the caller knows (0: not at all).
 int64_t cross_attend_work(int64_t tokens, int group, int requests, int kv_heads, int states, int width, int64_t most);
