@@ -169,9 +169,32 @@ __device__ __forceinline__ int value_place(int row, int chunk) {
     return chunk ^ (kWidth == 64 ? 4 * ((row >> 1) & 1) : 4 * (row & 3));
 }
 
+// LDS accesses of the wave's own lanes, before and after: done, and in that order.
+__device__ __forceinline__ void wave_sync() {
+    fence();
+    wait_lgkmcnt0();
+    __builtin_amdgcn_wave_barrier();
+    fence();
+}
+
+// A workgroup's part of a tile of kRows rows: their sums, as the lanes hold them, then their references and denominators.
+template <int kWidth, int kRows>
+__device__ __forceinline__ float* place_of(const CrossAttend& p, int64_t group) {
+    return p.work + group * (kRows * (kWidth + 2));
+}
+
 // kWaves waves take a tile of 32 rows each of one key head over its states a step at a time, which all of them share in
 // LDS. A step's keys and values are in registers by the step before it, when they are written to LDS, and asked for a
-// step before that.
+// step before that; one barrier a step. Queries and results cross LDS too, so that memory sees whole lines: read and
+// written 8 and 16 bytes a row at a time they took 18000 rows of 24 heads of 128 over 512 states from 131 to 152 us.
+// Where tiles are fewer than CUs a tile's states are split (301 rows of 28 heads over 30000 states: six ways, 154 us, and
+// 746 in one), and cross_join_kernel adds the parts.
+// Bound by the matrix and vector units in turn: of a step's 2.0 us (256 rows, 64 states, 128 wide) the scores take 0.5,
+// their exponentials and the second product 0.75, of which the products alone 0.95 together, waiting for states 0.25,
+// writing them to LDS and the barrier 0.15. Two waves a SIMD are all that its registers hold. Tried and not faster: the
+// next step's scores over this one's exponentials; half of the waves half a step late; 4 waves of 64 rows (copies
+// between register files, +50%); 4 waves of 32, two workgroups a CU (states read twice as often, +12%); equal runs of
+// steps as few rows have them (+5%: their parts' traffic, and requests' states no longer shared in L2).
 template <int kWidth, int kWaves, bool kHalf>
 __global__ __launch_bounds__(64 * kWaves, kWidth == 256 ? 1 : 2) void cross_kernel(CrossAttend p) {
     constexpr int kRows = 32 * kWaves, kOut = kWidth / 32, kDepth = kWidth / 16;
@@ -182,30 +205,10 @@ __global__ __launch_bounds__(64 * kWaves, kWidth == 256 ? 1 : 2) void cross_kern
     __shared__ uint64_t seen_of[kStage];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 31, h = lane >> 5;
-    const int kv = blockIdx.x % p.kv_heads, id = blockIdx.x / p.kv_heads;
-    int request, tile, found;
-    if (!find_tile<kRows>(p, id / p.splits, request, tile, found)) {
-        if (p.splits == 1) clear_rest(p, found * p.kv_heads);
-        return;
-    }
-    const int split = id % p.splits;
-    const Rows of = rows_of(p, request);
-    const int rows = of.count * p.group, mine = kRows * tile + 32 * wave, row = mine + col;
-    const bool busy = mine < rows, live = row < rows;
-    const int token = of.first + (live ? row / p.group : 0), head = kv * p.group + (live ? row % p.group : 0);
-    const int steps = (of.length + kStep - 1) / kStep;
-    const int begin = static_cast<int>(static_cast<int64_t>(steps) * split / p.splits);
-    const int end = static_cast<int>(static_cast<int64_t>(steps) * (split + 1) / p.splits);
-
-    i32x4 q[kDepth];
-#pragma unroll
-    for (int b = 0; b < kDepth; ++b) q[b] = query8(p.q + token * p.q_token + head * p.q_head, live, 16 * b + 8 * h, p.width);
+    const int kv = blockIdx.x % p.kv_heads;
     const float sharp = p.scale * kLog2e;
 
     // This wave's shares of a step's keys and values: 1 KiB each, whole rows.
-    const uint16_t* k_base = p.k + request * p.k_request + kv * p.k_head;
-    const uint16_t* v_base = p.v + request * p.v_request + kv * p.v_head;
-    const uint8_t* mask = p.mask ? p.mask + request * p.mask_request : nullptr;
     uint32_t k_from[kLoads], v_from[kLoads], row_of[kLoads];
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
@@ -215,22 +218,85 @@ __global__ __launch_bounds__(64 * kWaves, kWidth == 256 ? 1 : 2) void cross_kern
         k_from[i] = 8 * kc < p.width ? 2u * (r * static_cast<uint32_t>(p.k_state) + 8 * kc) : kNowhere;
         v_from[i] = 8 * vc < p.width ? 2u * (r * static_cast<uint32_t>(p.v_state) + 8 * vc) : kNowhere;
     }
-    const auto seen_at = [&](int i) {
-        const uint64_t word = seen_of[i];
+    // The matrix unit's operands in a tile: row col of a half's 32 keys, elements 16b + 8h ..; and, transposed by the
+    // read, channel 32o + col of the states that the lane's weights are of, 4h .. and 8 + 4h .. of each 16.
+    // Chunks' places are exclusive-or's, so that of 2b or 4o chunks further on is this one's with 32b or 64o.
+    const int k_at = col * 2 * kWidth + 16 * key_place<kWidth>(col, h);
+    const int v_row = 4 * h + (lane & 15) / 4, v_piece = 2 * ((lane >> 4) & 1) + (lane & 3) / 2;
+    const int v_at = v_row * 2 * kWidth + 16 * value_place<kWidth>(v_row, v_piece) + 8 * (lane & 1);
+
+    uint8_t* const own = &tiles[0][0][0] + wave * 64 * kWidth;
+    static_assert(sizeof(tiles) >= kWaves * 64 * kWidth, "32 rows a wave");
+    const int turn_tokens = kPerLoad / p.group, turn_heads = kPerLoad % p.group;
+    const int id = blockIdx.x / p.kv_heads;
+    int request, tile, found;
+    if (!find_tile<kRows>(p, id / p.splits, request, tile, found)) {
+        if (p.splits == 1) clear_rest(p, found * p.kv_heads);
+        return;
+    }
+    const int split = id % p.splits;
+    const Rows of = rows_of(p, request);
+    const int rows = of.count * p.group, mine = kRows * tile + 32 * wave;
+    const bool busy = mine < rows;
+    const int steps = (of.length + kStep - 1) / kStep;
+    const int begin = static_cast<int>(static_cast<int64_t>(steps) * split / p.splits);
+    const int end = static_cast<int>(static_cast<int64_t>(steps) * (split + 1) / p.splits);
+    const uint16_t* k_base = p.k + request * p.k_request + kv * p.k_head;
+    const uint16_t* v_base = p.v + request * p.v_request + kv * p.v_head;
+    const uint8_t* mask = p.mask ? p.mask + request * p.mask_request : nullptr;
+    // Queries and results go through the wave's share of LDS, in whole lines to and from memory: piece i is rows
+    // kPerLoad * i + lane / kChunks of the wave, and each(i, its token, its head, its chunk) is called for those
+    // that are there.
+    const auto each_line = [&](auto&& each) {
+        int r0 = mine + lane / kChunks;
+        asm volatile("" : "+v"(r0));  // worked out anew at each call, rather than kept in registers over the steps
+        int token = of.first + r0 / p.group, head = r0 % p.group;
+#pragma unroll
+        for (int i = 0; i < 32 / kPerLoad; ++i) {
+            const int r = i * kPerLoad + lane / kChunks, chunk = key_place<kWidth>(r, lane % kChunks);
+            if (mine + r < rows && 8 * chunk < p.width) each(i, token, kv * p.group + head, 8 * chunk);
+            token += turn_tokens;
+            head += turn_heads;
+            if (head >= p.group) {
+                head -= p.group;
+                ++token;
+            }
+        }
+    };
+    i32x4 q[kDepth];
+    {
+        i32x4 raw[32 / kPerLoad];
+#pragma unroll
+        for (int i = 0; i < 32 / kPerLoad; ++i) raw[i] = i32x4{0, 0, 0, 0};
+        each_line([&](int i, int token, int head, int d) { raw[i] = *reinterpret_cast<const i32x4*>(p.q + token * p.q_token + head * p.q_head + d); });
+#pragma unroll
+        for (int i = 0; i < 32 / kPerLoad; ++i) *reinterpret_cast<i32x4*>(own + 1024 * i + 16 * lane) = raw[i];
+        wave_sync();
+#pragma unroll
+        for (int b = 0; b < kDepth; ++b) q[b] = *reinterpret_cast<const i32x4*>(own + (k_at ^ 32 * b));
+        wave_sync();
+    }
+
+    const auto same = [](uint64_t word) {
         return static_cast<uint64_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(word >> 32))) << 32 |
                static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(word)));
     };
     i32x4 k_raw[kLoads], v_raw[kLoads];
-    const auto load = [&](int step) {
-        const int64_t t0 = static_cast<int64_t>(step) * kStep;
-        const int left = static_cast<int>(min(of.length - t0, static_cast<int64_t>(kStep)));
-        const __amdgpu_buffer_rsrc_t kr = states_view(k_base + t0 * p.k_state, left, p.k_state, p.width);
-        const __amdgpu_buffer_rsrc_t vr = states_view(v_base + t0 * p.v_state, left, p.v_state, p.width);
+    const uint16_t* k_next = k_base + static_cast<int64_t>(begin) * kStep * p.k_state;
+    const uint16_t* v_next = v_base + static_cast<int64_t>(begin) * kStep * p.v_state;
+    int left = of.length - begin * kStep;
+    // The next step's share.
+    const auto load = [&] {
+        const __amdgpu_buffer_rsrc_t kr = states_view(k_next, min(left, kStep), p.k_state, p.width);
+        const __amdgpu_buffer_rsrc_t vr = states_view(v_next, min(left, kStep), p.v_state, p.width);
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
             k_raw[i] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(kr, k_from[i], 0, 0));
             v_raw[i] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(vr, v_from[i], 0, 0));
         }
+        k_next += kStep * p.k_state;
+        v_next += kStep * p.v_state;
+        left -= kStep;
     };
     // Values of states that are not seen become zeros here; their scores are made minus infinity whatever they are.
     const auto put = [&](int slot, uint64_t seen) {
@@ -255,27 +321,30 @@ __global__ __launch_bounds__(64 * kWaves, kWidth == 256 ? 1 : 2) void cross_kern
     float ref = 0.0f, bound = -__builtin_inff(), total = 0.0f;
     bool any = false;
 
-    // The matrix unit's operands in a tile: row col of a half's 32 keys, elements 16b + 8h ..; and, transposed by the
-    // read, channel 32o + col of the states that the lane's weights are of, 4h .. and 8 + 4h .. of each 16.
-    int k_at[kDepth], v_at[kOut];
-    const int v_row = 4 * h + (lane & 15) / 4, v_piece = 2 * ((lane >> 4) & 1) + (lane & 3) / 2;
-#pragma unroll
-    for (int b = 0; b < kDepth; ++b) k_at[b] = col * 2 * kWidth + 16 * key_place<kWidth>(col, 2 * b + h);
-#pragma unroll
-    for (int o = 0; o < kOut; ++o) v_at[o] = v_row * 2 * kWidth + 16 * value_place<kWidth>(v_row, 4 * o + v_piece) + 8 * (lane & 1);
-
-    const auto compute = [&](int slot, uint64_t seen) {
-        const uint8_t* keys = tiles[slot][0];
-        const uint8_t* values = tiles[slot][1];
-        f32x16 s[kStep / 32];
+    f32x16 s[kStep / 32];
+    const auto score = [&](int slot) {
+        const int at = slot * 2 * kBytes + k_at;
+        const uint8_t* keys = &tiles[0][0][0];
 #pragma unroll
         for (int i = 0; i < kScores; ++i) s[i / 16][i % 16] = 0.0f;
 #pragma unroll
         for (int b = 0; b < kDepth; ++b) {
 #pragma unroll
             for (int j = 0; j < kStep / 32; ++j)
-                s[j] = mfma32<kHalf>(*reinterpret_cast<const i32x4*>(keys + k_at[b] + 64 * kWidth * j), q[b], s[j]);
+                s[j] = mfma32<kHalf>(*reinterpret_cast<const i32x4*>(keys + (at ^ 32 * b) + 64 * kWidth * j), q[b], s[j]);
         }
+        // Eight operands read ahead: the compiler by itself reads two, and waits for LDS at each pair of products.
+        constexpr int kProducts = kDepth * (kStep / 32), kAhead = 8;
+        __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
+#pragma unroll
+        for (int i = 0; i < kProducts; i += 2) {
+            __builtin_amdgcn_sched_group_barrier(0x8, 2, 0);
+            if (i + kAhead < kProducts) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+        }
+    };
+    const auto add = [&](int slot, uint64_t seen) {
+        const int from = slot * 2 * kBytes + kBytes + v_at;
+        const uint8_t* values = &tiles[0][0][0];
         float most = -__builtin_inff();
 #pragma unroll
         for (int i = 0; i < kScores; ++i) s[i / 16][i % 16] = __builtin_fmaf(s[i / 16][i % 16], sharp, -ref);
@@ -314,7 +383,7 @@ __global__ __launch_bounds__(64 * kWaves, kWidth == 256 ? 1 : 2) void cross_kern
         for (int a = 0; a < kStep / 16; ++a) {
 #pragma unroll
             for (int o = 0; o < kOut; ++o) {
-                const uint8_t* at = values + v_at[o] + 32 * kWidth * a;
+                const uint8_t* at = values + (from ^ 64 * o) + 32 * kWidth * a;
                 const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsFour*)(at));
                 const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsFour*)(at + 16 * kWidth));
                 const i32x2 l2 = __builtin_bit_cast(i32x2, lo), h2 = __builtin_bit_cast(i32x2, hi);
@@ -325,45 +394,104 @@ __global__ __launch_bounds__(64 * kWaves, kWidth == 256 ? 1 : 2) void cross_kern
 
     for (int stage = begin; stage < end; stage += kStage) {
         const int stage_end = min(end, stage + kStage);
-        if (stage != begin) __syncthreads();
+        __syncthreads();  // the last stage's reads
         for (int i = wave; i < stage_end - stage; i += kWaves) {
             const int t = (stage + i) * kStep + lane;
             const uint64_t word = __ballot(lane < kStep && t < of.length && (!mask || mask[t]));
             if (lane == 0) seen_of[i] = word;
         }
         __syncthreads();
-        load(stage);
-        put(stage & 1, seen_at(0));
-        load(stage + 1);
+        if (stage == begin) load();
+        uint64_t seen = same(seen_of[0]);
+        put(stage & 1, seen);
+        load();
         for (int step = stage; step < stage_end; ++step) {
             __syncthreads();
-            if (step + 1 < stage_end) put((step + 1) & 1, seen_at(step + 1 - stage));
-            load(step + 2);
-            const uint64_t seen = seen_at(step - stage);
+            const uint64_t word = step + 1 < stage_end ? seen_of[step + 1 - stage] : 0;
+            if (busy) score(step & 1);
+            const uint64_t next = same(word);
+            if (step + 1 < stage_end) {
+                put((step + 1) & 1, next);
+                load();
+            }
             any |= seen != 0;
-            if (busy) compute(step & 1, seen);
+            if (busy) add(step & 1, seen);
+            seen = next;
         }
     }
 
-    if (!live) return;
     total += __shfl_xor(total, 32);
-    const int64_t at = static_cast<int64_t>(token) * p.q_heads + head;
+    if (p.splits == 1) {
+        __syncthreads();
+        const float inv = any ? 1.0f / total : 0.0f;
+#pragma unroll
+        for (int o = 0; o < kOut; ++o) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                *reinterpret_cast<i32x2*>(own + col * 2 * kWidth + 16 * key_place<kWidth>(col, 4 * o + i) + 8 * h) =
+                    i32x2{pack2<kHalf>(acc[o][4 * i] * inv, acc[o][4 * i + 1] * inv), pack2<kHalf>(acc[o][4 * i + 2] * inv, acc[o][4 * i + 3] * inv)};
+        }
+        wave_sync();
+        each_line([&](int i, int token, int head, int d) {
+            *reinterpret_cast<i32x4*>(p.out + (static_cast<int64_t>(token) * p.q_heads + head) * p.width + d) =
+                *reinterpret_cast<const i32x4*>(own + 1024 * i + 16 * lane);
+        });
+        return;
+    }
+    if (!busy) return;
+    float* const to = place_of<kWidth, kRows>(p, blockIdx.x);
 #pragma unroll
     for (int o = 0; o < kOut; ++o) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const f32x4 v = {acc[o][4 * i], acc[o][4 * i + 1], acc[o][4 * i + 2], acc[o][4 * i + 3]};
-            const int d = 32 * o + 8 * i + 4 * h;
-            if (p.splits == 1) {
-                store_row<kHalf>(p, at, d, v, total, any);
-            } else {
-                const int64_t places = static_cast<int64_t>(p.tokens) * p.q_heads;
-                *reinterpret_cast<f32x4*>(p.work + (split * places + at) * kWidth + d) = v;
-                if (d == 0)
-                    *reinterpret_cast<f32x2*>(p.work + p.splits * places * kWidth + 2 * (split * places + at)) =
-                        f32x2{any ? (bound > 0.0f ? ref : kNoScore) : -__builtin_inff(), total};
-            }
-        }
+        for (int i = 0; i < 4; ++i)
+            reinterpret_cast<f32x4*>(to)[(4 * kOut * wave + 4 * o + i) * 64 + lane] =
+                f32x4{acc[o][4 * i], acc[o][4 * i + 1], acc[o][4 * i + 2], acc[o][4 * i + 3]};
+    }
+    if (h == 0)
+        reinterpret_cast<f32x2*>(to + kRows * kWidth)[32 * wave + col] =
+            f32x2{any ? (bound > 0.0f ? ref : kNoScore) : -__builtin_inff(), total};
+}
+
+// Joins a tile's parts, one a split: a workgroup the 32 rows of one wave, in the order in which it left them.
+template <int kWidth, int kWaves>
+__global__ __launch_bounds__(256) void cross_join_kernel(CrossAttend p) {
+    constexpr int kRows = 32 * kWaves, kOut = kWidth / 32;
+    const int lane = threadIdx.x & 63, side = threadIdx.x >> 6, wave = blockIdx.x % kWaves;
+    const int id = blockIdx.x / kWaves, kv = id % p.kv_heads, col = lane & 31, h = lane >> 5;
+    int request, tile, found;
+    if (!find_tile<kRows>(p, id / p.kv_heads, request, tile, found)) {
+        clear_rest(p, found * p.kv_heads * kWaves);
+        return;
+    }
+    const Rows of = rows_of(p, request);
+    const int row = kRows * tile + 32 * wave + col;
+    if (row >= of.count * p.group) return;
+    float most = -__builtin_inff(), total = 0.0f;
+    f32x4 v[kOut];
+#pragma unroll
+    for (int o = 0; o < kOut; ++o) v[o] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 2
+    for (int split = 0; split < p.splits; ++split) {
+        const float* from = place_of<kWidth, kRows>(p, (id / p.kv_heads * p.splits + split) * p.kv_heads + kv);
+        const f32x2 rest = reinterpret_cast<const f32x2*>(from + kRows * kWidth)[32 * wave + col];
+        f32x4 one[kOut];
+#pragma unroll
+        for (int o = 0; o < kOut; ++o) one[o] = reinterpret_cast<const f32x4*>(from)[(4 * kOut * wave + kOut * side + o) * 64 + lane];
+        const float up = nan_max(most, rest[0]);
+        // Nothing seen so far, and here: minus infinity less itself is no reference.
+        const float old = most == up ? 1.0f : __builtin_amdgcn_exp2f(most - up), factor = rest[0] == up ? 1.0f : __builtin_amdgcn_exp2f(rest[0] - up);
+        total = total * old + rest[1] * factor;
+#pragma unroll
+        for (int o = 0; o < kOut; ++o) v[o] = v[o] * old + one[o] * factor;
+        most = up;
+    }
+    const int64_t at = static_cast<int64_t>(of.first + row / p.group) * p.q_heads + kv * p.group + row % p.group;
+    const bool some = most != -__builtin_inff();
+#pragma unroll
+    for (int o = 0; o < kOut; ++o) {
+        const int chunk = kOut * side + o, d = 32 * (chunk / 4) + 8 * (chunk % 4) + 4 * h;
+        if (p.half) store_row<true>(p, at, d, v[o], total, some);
+        else store_row<false>(p, at, d, v[o], total, some);
     }
 }
 
@@ -375,14 +503,6 @@ __device__ __forceinline__ f32x4 mfma16(const i32x4& a, const i32x4& b, f32x4 c)
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
     else
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-}
-
-// LDS accesses of the wave's own lanes, before and after: done, and in that order.
-__device__ __forceinline__ void wave_sync() {
-    fence();
-    wait_lgkmcnt0();
-    __builtin_amdgcn_wave_barrier();
-    fence();
 }
 
 // The eight XCDs take workgroups in turn: one share's heads begin further on than the last one's, so that each XCD reads
@@ -761,35 +881,6 @@ __global__ __launch_bounds__(256) void cross_few_join_kernel(CrossAttend p) {
     }
 }
 
-// Joins a row's parts, kWidth / 4 threads a row: Σ sums · 2^(ref − most) over Σ totals · 2^(ref − most).
-template <int kWidth>
-__global__ __launch_bounds__(256) void cross_join_kernel(CrossAttend p) {
-    constexpr int kEach = kWidth / 4;
-    const int64_t places = static_cast<int64_t>(p.tokens) * p.q_heads;
-    const int64_t at = static_cast<int64_t>(blockIdx.x) * (256 / kEach) + threadIdx.x / kEach;
-    const int d = 4 * (threadIdx.x % kEach);
-    if (at >= places || d >= p.width) return;
-    const int token = static_cast<int>(at / p.q_heads);
-    const Rows last = rows_of(p, p.requests - 1);
-    f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (token >= rows_of(p, 0).first && token < last.first + last.count) {
-        const float* parts = p.work + p.splits * places * kWidth;
-        float most = -__builtin_inff();
-        for (int i = 0; i < p.splits; ++i) most = nan_max(most, parts[2 * (i * places + at)]);
-        if (most != -__builtin_inff()) {
-            float total = 0.0f;
-            for (int i = 0; i < p.splits; ++i) {
-                const float factor = __builtin_amdgcn_exp2f(parts[2 * (i * places + at)] - most);
-                total += parts[2 * (i * places + at) + 1] * factor;
-                v += *reinterpret_cast<const f32x4*>(p.work + (i * places + at) * kWidth + d) * factor;
-            }
-            v *= 1.0f / total;
-        }
-    }
-    *reinterpret_cast<i32x2*>(p.out + at * p.width + d) =
-        i32x2{static_cast<int32_t>(narrow2(v[0], v[1], p.half)), static_cast<int32_t>(narrow2(v[2], v[3], p.half))};
-}
-
 constexpr int padded(int width) { return width <= 64 ? 64 : width <= 128 ? 128 : 256; }
 constexpr int waves_of(int width) { return width == 256 ? 4 : 8; }
 
@@ -837,7 +928,7 @@ Shape shape_of(int64_t tokens, int group, int requests, int kv_heads, int states
         const int64_t step = step_of(padded(width)), steps = (states + step - 1) / step;
         const int64_t splits = min(256 / (a.tiles * kv_heads), steps / 4);
         a.splits = static_cast<int>(splits < 1 ? 1 : splits > 64 ? 64 : splits);
-        if (a.splits > 1) a.floats = a.splits * tokens * group * kv_heads * (padded(width) + 2);
+        if (a.splits > 1) a.floats = a.tiles * a.splits * kv_heads * a.rows * (padded(width) + 2);
     }
     return a;
 }
@@ -859,11 +950,7 @@ hipError_t attend(const CrossAttend& p, const Shape& a, hipStream_t s) {
     constexpr int kWaves = waves_of(kWidth);
     const unsigned groups = static_cast<unsigned>(a.tiles * p.kv_heads * p.splits);
     cross_kernel<kWidth, kWaves, kHalf><<<groups, 64 * kWaves, 0, s>>>(p);
-    if (p.splits > 1) {
-        const int64_t rows = static_cast<int64_t>(p.tokens) * p.q_heads;
-        constexpr int kEach = 256 / (kWidth / 4);
-        cross_join_kernel<kWidth><<<static_cast<unsigned>((rows + kEach - 1) / kEach), 256, 0, s>>>(p);
-    }
+    if (p.splits > 1) cross_join_kernel<kWidth, kWaves><<<static_cast<unsigned>(a.tiles * p.kv_heads * kWaves), 256, 0, s>>>(p);
     return hipGetLastError();
 }
 
