@@ -17,8 +17,11 @@ namespace cozyq {
 namespace {
 
 constexpr int kThreads = 256;
-// Waves from which on a wave takes more than one run of heads.
-constexpr int kManyWaves = 8192;
+// Waves from which on a wave takes more than one run of heads: a token's cosines and sines are then read fewer times,
+// up to once for all of its heads. 8191 tokens of 40 heads on three axes take 34.8 us so and 45.2 at a run a wave, 4173
+// of 20 and 20 of 64 14.5 and 16.1; but 24 tokens, all heads a wave, 7.3 for 3.8. (From 8192 on: 39.6 and 16.1; 8191
+// tokens on one axis, one launch after another, 36.8 for 37.6.)
+constexpr int kManyWaves = 2048;
 
 // The tables' row of a position, the nearest one where there is none.
 __device__ __forceinline__ int64_t table_row(const HeadRows& r, int position) {
@@ -29,7 +32,10 @@ __device__ __forceinline__ int64_t table_row(const HeadRows& r, int position) {
 // the rotated part holds both elements of eight pairs, so that a rotation needs no other lane: for
 // halves the chunks u and u + rotated/16 of eight elements, otherwise the neighbours 2u and 2u + 1.
 // A wave takes 64 / lanes heads of one token at a time, `runs` times: a lane's cosines and sines are the same for
-// all of them and are read once.
+// all of them and are read once. On several axes a lane reads every axis' rows and keeps, of each pair, its own axis':
+// whole lines that the token's other lanes share, rather than a gather a pair.
+// Bound by memory and the vector unit (168 MB of those 8191 tokens at 4.8 TB/s, where a large copy reaches 5.6; VALU
+// 77% busy), small calls by the launch.
 template <bool kHalf>
 __global__ __launch_bounds__(kThreads) void norm_rope_kernel(HeadRows r, int parts) {
     const int lane = threadIdx.x & 63, u = lane & (r.lanes - 1), slots = 64 / r.lanes;
