@@ -35,7 +35,7 @@ __device__ __forceinline__ int64_t table_row(const HeadRows& r, int position) {
 // all of them and are read once. On several axes a lane reads every axis' rows and keeps, of each pair, its own axis':
 // whole lines that the token's other lanes share, rather than a gather a pair.
 // Bound by memory and the vector unit (168 MB of those 8191 tokens at 4.8 TB/s, where a large copy reaches 5.6; VALU
-// 77% busy), small calls by the launch.
+// 68% busy), small calls by the launch.
 template <bool kHalf>
 __global__ __launch_bounds__(kThreads) void norm_rope_kernel(HeadRows r, int parts) {
     const int lane = threadIdx.x & 63, u = lane & (r.lanes - 1), slots = 64 / r.lanes;
