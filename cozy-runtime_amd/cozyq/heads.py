@@ -29,7 +29,8 @@ def norm_rope(torch: Any, q: Tensor, k: Tensor | None, q_gain: Tensor | None, k_
     to 256. With `sections` a token has a position on each of two to four axes (time, height and width of images and
     video): `positions` is int32 `[axes, T]`, and pair j turns by row positions[axis of j, t] of the tables' column j.
     `sections[a]` of the R/2 pairs belong to axis a, in runs, axis 0's first; or `cycled`, in turns: axis a > 0 has
-    pairs a, a + axes, a + 2·axes, .., all below R/2, and axis 0 the others. q and k may be views (of one QKV buffer, say) whose last axis is dense and whose other
-    strides and address are multiples of 16 bytes; the results are new and contiguous."""
+    pairs a, a + axes, a + 2·axes, .., all below R/2, and axis 0 the others. q and k may be views (of one QKV buffer,
+    say) whose last axis is dense and whose other strides and address are multiples of 16 bytes; the results are new and
+    contiguous."""
     return _dispatch.library(_dispatch.card(OP, q)).head_norm_rope(q, k, q_gain, k_gain, cos, sin, positions, eps, interleaved,
                                                                    sections, cycled)  # fmt: skip

@@ -256,6 +256,33 @@ def test_cross_past_32_bit_offsets(attention, rows):
     check(attention.cross(torch, q, k, v, starts=counts(rows), lengths=n, most=max(rows)), q, k, v, counts(rows), n)
 
 
+@pytest.mark.parametrize("masked", [False, True], ids=["whole", "masked"])
+@pytest.mark.parametrize("rows", [[1, 0, 2], [130, 0, 40]], ids=["few", "many"])
+def test_cross_rows_of_no_request_beside_shared_out_states(attention, rows, masked):
+    """Rows before the first request's and after the last's, where requests' states are shared out over workgroups."""
+    q, k, v = inputs(sum(rows) + 50, 3, 2500, 4, 2, 64, BF16, 16)
+    starts, n = ints([20 + sum(rows[:i]) for i in range(4)]), ints([2500, 2500, 700])
+    mask = torch.rand(3, 2500, device=DEV) < 0.7 if masked else None
+    torch.cuda.empty_cache()
+    junk = [torch.full(q.shape, math.nan, dtype=BF16, device=DEV) for _ in range(4)]
+    where = {x.data_ptr() for x in junk}
+    del junk
+    got = attention.cross(torch, q, k, v, starts=starts, lengths=n, mask=mask, most=max(rows))
+    assert got.data_ptr() in where
+    check(got, q, k, v, starts, n, mask)
+    assert not got[:20].any() and not got[20 + sum(rows) :].any()
+
+
+@pytest.mark.parametrize("masked", [False, True], ids=["whole", "masked"])
+def test_cross_many_steps_of_one_workgroup(attention, masked):
+    """Tiles enough that none's states are shared out, over more than 256 steps of 64 of them."""
+    q, k, v = inputs(557, 2, 16900, 64, 64, 8, FP16, 17)
+    starts, n = counts([300, 257]), ints([16900, 16385])
+    mask = torch.rand(2, 16900, device=DEV) < 0.5 if masked else None
+    got = attention.cross(torch, q, k, v, starts=starts, lengths=n, mask=mask, most=300)
+    check(got, q, k, v, starts, n, mask)
+
+
 @pytest.mark.parametrize("rows", [[1, 1, 1], [30, 1, 200]], ids=["few", "many"])
 def test_cross_is_the_same_every_time_on_another_stream_and_in_a_graph(attention, rows):
     """A captured call, replayed over changing lengths, masks and rows with eager work between, equals the eager one."""
