@@ -175,6 +175,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         [c_int, _P, c_int, c_int64, c_int, c_int64, c_int64, _P, _P, c_int, c_int, c_int, c_int, c_int64, c_int64,
          c_int64, c_int64, c_int64, c_int64, _P, _P, _P, c_int64, c_int64, c_float, _P, _P, _P],
     ),
+    "cozyq_host_cross_runs": (c_int, [c_int64, c_int, c_int, c_int, c_int, c_int, c_int64, _P, _P, _P]),
     "cozyq_host_e4m3": (None, [_P, _P, c_int64]),
     "cozyq_host_mx_byte": (None, [_P, _P, c_int64]),
     "cozyq_probe_div": (c_int, [c_int, _P, _P, _P, c_int64, _P]),

@@ -923,6 +923,22 @@ int cozyq_cross_attend(int device, const void* q, int half, int64_t tokens, int 
                                most, on(stream));
 }
 
+int cozyq_host_cross_runs(int64_t tokens, int q_heads, int requests, int states, int kv_heads, int width, int64_t most,
+                          const int* starts, const int* lengths, int* out) {
+    if (!cross_shape(tokens, q_heads, requests, states, kv_heads, width, most) || !starts || !lengths || !out) return -1;
+    cozyq::CrossAttend p{};
+    p.starts = starts;
+    p.lengths = lengths;
+    p.tokens = static_cast<int>(tokens);
+    p.requests = requests;
+    p.states = states;
+    p.kv_heads = kv_heads;
+    p.q_heads = q_heads;
+    p.group = q_heads / kv_heads;
+    p.width = width;
+    return cozyq::cross_runs(p, most, out);
+}
+
 void cozyq_host_e4m3(const float* in, uint8_t* out, int64_t n) {
     for (int64_t i = 0; i < n; ++i) out[i] = cozyq::e4m3_rn(in[i]);
 }

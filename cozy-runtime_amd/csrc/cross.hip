@@ -61,7 +61,7 @@ struct Rows {
     int first, count, length;
 };
 
-__device__ __forceinline__ Rows rows_of(const CrossAttend& p, int b) {
+__host__ __device__ __forceinline__ Rows rows_of(const CrossAttend& p, int b) {
     Rows r;
     if (p.starts) {
         r.first = min(max(p.starts[b], 0), p.tokens);
@@ -78,23 +78,26 @@ __device__ __forceinline__ Rows rows_of(const CrossAttend& p, int b) {
 // index past its request.
 constexpr int kMany = 1 << 30;
 
+// Two numbers of up to kMany, added up.
+__host__ __device__ __forceinline__ int add_up(int a, int b) {
+    const uint32_t sum = static_cast<uint32_t>(a) + static_cast<uint32_t>(b);
+    return sum < kMany ? static_cast<int>(sum) : kMany;
+}
+
 // x from the lane that DPP control kCtrl names, 0 where it names none or the row is masked out.
 template <int kCtrl, int kRowMask>
-__device__ __forceinline__ uint32_t dpp_or_zero(uint32_t x) {
-    return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), kCtrl, kRowMask, 0xF, false));
+__device__ __forceinline__ int dpp_or_zero(int x) {
+    return __builtin_amdgcn_update_dpp(0, x, kCtrl, kRowMask, 0xF, false);
 }
 
 // Inclusive sums over a wave of numbers of up to kMany: within rows of 16 lanes, then a row's last sum into the next.
 __device__ __forceinline__ int wave_prefix(int n) {
-    const uint32_t most = kMany;
-    uint32_t x = static_cast<uint32_t>(n);
-    x = min(x + dpp_or_zero<0x111, 0xF>(x), most);  // row_shr:1
-    x = min(x + dpp_or_zero<0x112, 0xF>(x), most);  // row_shr:2
-    x = min(x + dpp_or_zero<0x114, 0xF>(x), most);  // row_shr:4
-    x = min(x + dpp_or_zero<0x118, 0xF>(x), most);  // row_shr:8
-    x = min(x + dpp_or_zero<0x142, 0xA>(x), most);  // row_bcast:15 into rows 1 and 3
-    x = min(x + dpp_or_zero<0x143, 0xC>(x), most);  // row_bcast:31 into rows 2 and 3
-    return static_cast<int>(x);
+    n = add_up(n, dpp_or_zero<0x111, 0xF>(n));  // row_shr:1
+    n = add_up(n, dpp_or_zero<0x112, 0xF>(n));  // row_shr:2
+    n = add_up(n, dpp_or_zero<0x114, 0xF>(n));  // row_shr:4
+    n = add_up(n, dpp_or_zero<0x118, 0xF>(n));  // row_shr:8
+    n = add_up(n, dpp_or_zero<0x142, 0xA>(n));  // row_bcast:15 into rows 1 and 3
+    return add_up(n, dpp_or_zero<0x143, 0xC>(n));  // row_bcast:31 into rows 2 and 3
 }
 
 // The tile number `id` of all requests' row tiles of kRows rows, one request after another; false past the last.
@@ -107,16 +110,16 @@ __device__ bool find_tile(const CrossAttend& p, int id, int& request, int& tile,
         if (base + lane < p.requests)
             tiles = static_cast<int>((static_cast<int64_t>(rows_of(p, base + lane).count) * p.group + kRows - 1) / kRows);
         const int sum = wave_prefix(tiles);
-        const uint64_t past = __ballot(min(before, kMany) - id > -sum);
+        const uint64_t past = __ballot(before - id > -sum);
         if (past) {
             const int at = __ffsll(static_cast<unsigned long long>(past)) - 1;
             request = base + at;
             tile = id - before - (__builtin_amdgcn_readlane(sum, at) - __builtin_amdgcn_readlane(tiles, at));
             return true;
         }
-        before = min(before, kMany) + __builtin_amdgcn_readlane(sum, 63);
+        before = add_up(before, __builtin_amdgcn_readlane(sum, 63));
     }
-    count = min(before, kMany);
+    count = before;
     return false;
 }
 
@@ -528,7 +531,7 @@ struct Extent {
 };
 
 template <int kRows>
-__device__ __forceinline__ Extent extent_of(const CrossAttend& p, int b) {
+__host__ __device__ __forceinline__ Extent extent_of(const CrossAttend& p, int b) {
     if (b >= p.requests) return {0, 0, {0, 0, 0}};
     const Rows r = rows_of(p, b);
     const int steps = max(1, (r.length + kFewStep - 1) / kFewStep);
@@ -548,10 +551,30 @@ __device__ __forceinline__ Extent extent_at(const CrossAttend& p, const Cuts& c,
     return base == 0 ? c.first : extent_of<kRows>(p, base + static_cast<int>(threadIdx.x & 63));
 }
 
+// A request's runs of p.cut steps, if none holds two tiles' steps.
+__host__ __device__ __forceinline__ int runs_of(const CrossAttend& p, const Extent& e) { return e.tiles * ((e.steps + p.cut - 1) / p.cut); }
+
+// Cuts `total` steps in all (kMany: or more), of `runs` such runs; `longer`: whether a tile has more than kWholeSteps.
+// run * shares > total, so that every step is of one of the runs.
+__host__ __device__ __forceinline__ void cut(const CrossAttend& p, int total, int runs, bool longer, Cuts& c) {
+    c.apart = runs <= p.shares;
+    c.run = c.apart ? (longer ? p.cut : kWholeSteps) : max(p.cut, total / p.shares + 1);
+}
+
 // A tile's steps as they are counted.
-__device__ __forceinline__ int counted(const Extent& e, const Cuts& c) {
+__host__ __device__ __forceinline__ int counted(const Extent& e, const Cuts& c) {
     return c.apart ? (e.steps + c.run - 1) / c.run * c.run : e.steps;
 }
+
+// The first step of tile `tile` of a request's `tiles` of `one` steps each, the last of which ends at `end`.
+__host__ __device__ __forceinline__ int first_step(int end, int tiles, int tile, int one) { return end - (tiles - tile) * one; }
+
+// The runs that a tile's steps are in, from the first to the last.
+struct Runs {
+    int first, last;
+};
+
+__host__ __device__ __forceinline__ Runs runs_of(int start, int steps, int run) { return {start / run, (start + steps - 1) / run}; }
 
 template <int kRows>
 __device__ Cuts cuts_of(const CrossAttend& p) {
@@ -565,11 +588,10 @@ __device__ Cuts cuts_of(const CrossAttend& p) {
     for (int base = 0; base < p.requests; base += 64) {
         const Extent e = extent_at<kRows>(p, c, base);
         longer |= __any(e.steps > kWholeSteps);
-        total = min(total, kMany) + __builtin_amdgcn_readlane(wave_prefix(e.tiles * e.steps), 63);
-        runs = min(runs, kMany) + __builtin_amdgcn_readlane(wave_prefix(e.tiles * ((e.steps + p.cut - 1) / p.cut)), 63);
+        total = add_up(total, __builtin_amdgcn_readlane(wave_prefix(e.tiles * e.steps), 63));
+        runs = add_up(runs, __builtin_amdgcn_readlane(wave_prefix(runs_of(p, e)), 63));
     }
-    c.apart = runs <= p.shares;
-    c.run = c.apart ? (longer ? p.cut : kWholeSteps) : max(p.cut, min(total, kMany) / p.shares + 1);
+    cut(p, total, runs, longer, c);
     return c;
 }
 
@@ -588,18 +610,18 @@ __device__ bool find_item(const CrossAttend& p, const Cuts& c, int id, Item& out
         const int one = p.cut ? counted(e, c) : 0;
         const int steps = wave_prefix(e.tiles * one), tiles = wave_prefix(e.tiles);
         const int ids = kByStep ? steps : tiles;
-        const uint64_t past = __ballot(min(ids_before, kMany) - id > -ids);
+        const uint64_t past = __ballot(ids_before - id > -ids);
         if (past) {
             const int at = __ffsll(static_cast<unsigned long long>(past)) - 1;
             const int n = __builtin_amdgcn_readlane(one, at), t = __builtin_amdgcn_readlane(e.tiles, at);
             const int from = id - ids_before - __builtin_amdgcn_readlane(ids, at) + (kByStep ? t * n : t);
             const int tile = kByStep ? from / n : from;
-            out = {base + at, tile, steps_before + __builtin_amdgcn_readlane(steps, at) - (t - tile) * n, __builtin_amdgcn_readlane(e.steps, at),
+            out = {base + at, tile, first_step(steps_before + __builtin_amdgcn_readlane(steps, at), t, tile, n), __builtin_amdgcn_readlane(e.steps, at),
                    {__builtin_amdgcn_readlane(e.of.first, at), __builtin_amdgcn_readlane(e.of.count, at), __builtin_amdgcn_readlane(e.of.length, at)}};
             return true;
         }
-        ids_before = min(ids_before, kMany) + __builtin_amdgcn_readlane(ids, 63);
-        steps_before = min(steps_before, kMany) + __builtin_amdgcn_readlane(steps, 63);
+        ids_before = add_up(ids_before, __builtin_amdgcn_readlane(ids, 63));
+        steps_before = add_up(steps_before, __builtin_amdgcn_readlane(steps, 63));
     }
     return false;
 }
@@ -832,7 +854,8 @@ __global__ __launch_bounds__(256) void cross_few_join_kernel(CrossAttend p) {
     const int run = cuts.run;
     Item item;
     if (!find_item<kRows, false>(p, cuts, blockIdx.x / p.kv_heads, item)) return;
-    const int first = item.start / run, last = (item.start + item.steps - 1) / run;
+    const Runs parts = runs_of(item.start, item.steps, run);
+    const int first = parts.first, last = parts.last;
     if (first == last) return;  // whole
     const Rows of = item.of;
     const int row0 = kRows * item.tile, count = min(kRows, of.count * p.group - row0);
@@ -963,6 +986,56 @@ hipError_t attend(const CrossAttend& p, const Shape& a, hipStream_t s) {
 
 int64_t cross_attend_work(int64_t tokens, int group, int requests, int kv_heads, int states, int width, int64_t most) {
     return 4 * shape_of(tokens, group, requests, kv_heads, states, width, most).floats;
+}
+
+// What cuts_of and find_item come to, 64 requests after another: the same sums and rules.
+template <int kRows>
+static void host_runs(const CrossAttend& p, int tiles, int* out) {
+    Cuts c = {extent_of<kRows>(p, 0), 1, false};
+    int total = 0, runs = 0;
+    bool longer = false;
+    for (int base = 0; base < p.requests; base += 64) {
+        int all = 0, cut_up = 0;
+        for (int b = base; b < base + 64; ++b) {
+            const Extent e = extent_of<kRows>(p, b);
+            longer |= e.steps > kWholeSteps;
+            all = add_up(all, e.tiles * e.steps);
+            cut_up = add_up(cut_up, runs_of(p, e));
+        }
+        total = add_up(total, all);
+        runs = add_up(runs, cut_up);
+    }
+    cut(p, total, runs, longer, c);
+    int least = 0, most = 0, steps_before = 0;
+    for (int base = 0, id = 0; base < p.requests; base += 64) {
+        int steps = 0;
+        for (int b = base; b < base + 64; ++b) {
+            const Extent e = extent_of<kRows>(p, b);
+            const int one = counted(e, c);
+            steps = add_up(steps, e.tiles * one);
+            for (int tile = 0; tile < e.tiles && id < tiles; ++tile, ++id) {
+                const Runs of = runs_of(first_step(steps_before + steps, e.tiles, tile, one), e.steps, c.run);
+                least = min(least, of.first);
+                most = max(most, of.last);
+            }
+        }
+        steps_before = add_up(steps_before, steps);
+    }
+    out[0] = total;
+    out[1] = c.run;
+    out[2] = p.shares;
+    out[3] = least;
+    out[4] = most;
+}
+
+bool cross_runs(CrossAttend p, int64_t most, int* out) {
+    const Shape a = shape_of(p.tokens, p.group, p.requests, p.kv_heads, p.states, p.width, most);
+    if (!a.cut) return false;
+    p.cut = a.cut;
+    p.shares = a.shares;
+    if (a.rows == 16) host_runs<16>(p, static_cast<int>(a.tiles), out);
+    else host_runs<32>(p, static_cast<int>(a.tiles), out);
+    return true;
 }
 
 hipError_t cross_attend(CrossAttend p, int64_t most, hipStream_t s) {

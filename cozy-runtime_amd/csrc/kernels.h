@@ -360,6 +360,8 @@ struct CrossAttend {
 // Bytes of workspace; `most`: the most rows a request has, as far as the caller knows (0: not at all).
 int64_t cross_attend_work(int64_t tokens, int group, int requests, int kv_heads, int states, int width, int64_t most);
 hipError_t cross_attend(CrossAttend p, int64_t most, hipStream_t s);
+// How few rows' steps are cut, from `starts` and `lengths` in host memory (cozyq_host_cross_runs); false where they are not.
+bool cross_runs(CrossAttend p, int64_t most, int* out);
 
 // The most rows, table rows or cache slots that the head and cache kernels index: int32 with room.
 constexpr int kMostTokens = 1 << 30;
