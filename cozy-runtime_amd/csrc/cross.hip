@@ -25,9 +25,15 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 LdsFour;
 
 constexpr float kLog2e = 1.44269504f;
-// A row's weights are taken up to 2^6 at first and up to 2^15 before their reference moves, so that f16 holds those
-// down to 2^-30 of the largest.
-constexpr float kLift = 6.0f, kBound = 15.0f;
+// A row's weights are taken up to 2^kLift at first and 2^kSlack times that, 2^kMost at the most, before their reference
+// moves. f16: up to 2^6 and 2^15, so that it holds those down to 2^-30 of the largest. bf16, whose values may be as
+// large as float32's: up to 2^-24 and 2^-16, so that the sums of 2^16 states' finite values stay finite before they are
+// divided; values from 2^-102 on still come out of float32's subnormals' reach.
+template <bool kHalf>
+constexpr float kLift = kHalf ? 6.0f : -24.0f;
+template <bool kHalf>
+constexpr float kSlack = kHalf ? 9.0f : 8.0f;
+constexpr float kMost = 15.0f;
 // Below any reference: that of a row without a finite score.
 constexpr float kNoScore = -1e30f;
 constexpr int kStage = 256;  // steps whose seen states are staged at a time
@@ -55,6 +61,19 @@ __device__ __forceinline__ int32_t pack2(float a, float b) {
 
 // Keeps a branch a branch: without it the compiler works out both sides and selects.
 __device__ __forceinline__ void rarely() { asm volatile(""); }
+
+// Moves a row's reference for exponents of up to `most`, if they pass `bound` (minus infinity: there is no reference yet):
+// `up` is how far, and the result what sums so far are to be taken times. Where scores are so large that float32 has no
+// kLift more or less of them, the bound is of the weight that comes of it.
+template <bool kHalf>
+__device__ __forceinline__ float move(float most, float& ref, float& bound, float& up) {
+    const bool over = most > bound;
+    up = over ? most - kLift<kHalf> : 0.0f;
+    const float shrink = bound > -__builtin_inff() ? __builtin_amdgcn_exp2f(-up) : 0.0f;
+    if (over) bound = fminf(most - up + kSlack<kHalf>, kMost);
+    ref += up;
+    return shrink;
+}
 
 // Request b's rows of the call, in order and never past its last: [first, first + count), and how many states it has.
 struct Rows {
@@ -362,10 +381,8 @@ __global__ __launch_bounds__(64 * kWaves, kWidth == 256 ? 1 : 2) void cross_kern
         for (int i = 0; i < kScores; ++i) most = fmaxf(most, s[i / 16][i % 16]);
         if (__any(most > bound)) {
             most = fmaxf(most, __shfl_xor(most, 32));
-            const float up = most > bound ? most - kLift : 0.0f;
-            const float shrink = bound > 0.0f ? __builtin_amdgcn_exp2f(-up) : 0.0f;
-            if (most > bound) bound = kBound;
-            ref += up;
+            float up;
+            const float shrink = move<kHalf>(most, ref, bound, up);
             total *= shrink;
 #pragma unroll
             for (int i = 0; i < kScores; ++i) s[i / 16][i % 16] -= up;
@@ -452,7 +469,7 @@ __global__ __launch_bounds__(64 * kWaves, kWidth == 256 ? 1 : 2) void cross_kern
     }
     if (h == 0)
         reinterpret_cast<f32x2*>(to + kRows * kWidth)[32 * wave + col] =
-            f32x2{any ? (bound > 0.0f ? ref : kNoScore) : -__builtin_inff(), total};
+            f32x2{any ? (bound > -__builtin_inff() ? ref : kNoScore) : -__builtin_inff(), total};
 }
 
 // Joins a tile's parts, one a split: a workgroup the 32 rows of one wave, in the order in which it left them.
@@ -775,10 +792,8 @@ __global__ __launch_bounds__(256, kWidth * kTiles > 128 ? 1 : kWidth * kTiles ==
                 if (__any(most > bound[n])) {
                     most = fmaxf(most, __shfl_xor(most, 16));
                     most = fmaxf(most, __shfl_xor(most, 32));
-                    const float up = most > bound[n] ? most - kLift : 0.0f;
-                    const float shrink = bound[n] > 0.0f ? __builtin_amdgcn_exp2f(-up) : 0.0f;
-                    if (most > bound[n]) bound[n] = kBound;
-                    ref[n] += up;
+                    float up;
+                    const float shrink = move<kHalf>(most, ref[n], bound[n], up);
                     total[n] *= shrink;
 #pragma unroll
                     for (int i = 0; i < 8; ++i) x[i] -= up;
@@ -811,7 +826,7 @@ __global__ __launch_bounds__(256, kWidth * kTiles > 128 ? 1 : kWidth * kTiles ==
             total[n] += __shfl_xor(total[n], 16);
             total[n] += __shfl_xor(total[n], 32);
             if (g == 0) {
-                tops[wave][col] = bound[n] > 0.0f ? ref[n] : kNoScore;
+                tops[wave][col] = bound[n] > -__builtin_inff() ? ref[n] : kNoScore;
                 totals[wave][col] = total[n];
             }
 #pragma unroll
