@@ -34,8 +34,8 @@ constexpr float kLift = kHalf ? 6.0f : -24.0f;
 template <bool kHalf>
 constexpr float kSlack = kHalf ? 9.0f : 8.0f;
 constexpr float kMost = 15.0f;
-// Below any reference: that of a row without a finite score.
-constexpr float kNoScore = -1e30f;
+// Below any reference, as the lowest finite number: that of a row without a finite score.
+constexpr float kNoScore = -3.40282347e38f;
 constexpr int kStage = 256;  // steps whose seen states are staged at a time
 // States taken at a time: 64, or 32 of wide heads, whose accumulators leave fewer registers.
 constexpr int step_of(int width) { return width == 256 ? 32 : 64; }

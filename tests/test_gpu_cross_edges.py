@@ -1,13 +1,15 @@
-"""Attention to an encoder's states (`cozyq.attention.cross`) at the ends of its types, against `oracle/layer.py`; bars
-as in test_gpu_cross.py."""
+"""Attention to an encoder's states (`cozyq.attention.cross`) at the ends of its types and at scores far from zero,
+against `oracle/layer.py`; bars as in test_gpu_cross.py."""
 
 from __future__ import annotations
+
+import math
 
 import pytest
 import torch
 
-from test_gpu_cross import BF16, check, counts, inputs
-from test_gpu_kv_cache import DEV, ints
+from test_gpu_cross import BF16, FP16, check, counts, inputs
+from test_gpu_kv_cache import DEV, UNIT, ints
 
 pytestmark = pytest.mark.gpu
 
@@ -38,3 +40,26 @@ def test_cross_values_of_any_size(attention, rows, states, power):
     for x in (q, torch.zeros_like(q)):
         got = attention.cross(torch, x, k, v, starts=counts(rows), lengths=ints(lengths), most=max(rows))
         check(got, x, k, v, counts(rows), ints(lengths))
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("beside", [False, True], ids=["alone", "beside minus infinity"])
+@pytest.mark.parametrize("rows", ROWS, ids=str)
+def test_cross_scores_far_below_zero(attention, rows, beside, dtype):
+    """Ten states that all score -2^106, and nothing else seen, or nothing but scores of minus infinity: their values'
+    mean. Scores that are equal are off alike, so that only the weights' and the output's roundings count."""
+    requests, width, states = len(rows), 64, 4100
+    scale = 2.0**96 if dtype is FP16 else 2.0**-10
+    q = torch.full((sum(rows), 2, width), 16.0 if dtype is FP16 else 2.0**55, dtype=dtype, device=DEV)
+    _, _, v = inputs(1, requests, states, 2, 2, width, dtype, 4)
+    for at in (0, 710, 4080):
+        k = torch.full((requests, states, 2, width), -math.inf, dtype=dtype, device=DEV)
+        k[:, at : at + 10] = -1.0 if dtype is FP16 else -(2.0**55)
+        mask = None
+        if not beside:
+            mask = torch.zeros(requests, states, dtype=torch.bool, device=DEV)
+            mask[:, at : at + 10] = True
+        got = attention.cross(torch, q, k, v, starts=counts(rows), mask=mask, most=max(rows), scale=scale).double()
+        want = v[:, at : at + 10].double().mean(1).repeat_interleave(ints(rows), 0)
+        size = v[:, at : at + 10].double().abs().mean(1).repeat_interleave(ints(rows), 0)
+        assert ((got - want).abs() <= UNIT[dtype] * want.abs() + (UNIT[dtype] + 2.0**-20) * size).all(), at
