@@ -30,8 +30,8 @@ typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 constexpr float kLog2e = 1.44269504f;
-// Below any finite score: an all-masked row's maximum, so that 2^(−inf − m) is 0 and not NaN.
-constexpr float kNoScore = -1e30f;
+// Below any reference, as the lowest finite number: an all-masked row's maximum, so that 2^(−inf − m) is 0 and not NaN.
+constexpr float kNoScore = -3.40282347e38f;
 // A row's weights are taken up to 2^6 at first (the denominator alike), so that f16 holds those down to
 // 2^-30 of the largest; no more, because of scores so large that float32 steps by 16: six less then
 // rounds to no change, ten less would round to 2^16, which f16 has not.
