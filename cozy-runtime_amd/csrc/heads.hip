@@ -17,59 +17,72 @@ namespace cozyq {
 namespace {
 
 constexpr int kThreads = 256;
-// Waves from which on a wave takes more than one run of heads: a token's cosines and sines are then read fewer times,
-// up to once for all of its heads. 8191 tokens of 40 heads on three axes take 34.8 us so and 45.2 at a run a wave, 4173
-// of 20 and 20 of 64 14.5 and 16.1; but 24 tokens, all heads a wave, 7.3 for 3.8. (From 8192 on: 39.6 and 16.1; 8191
-// tokens on one axis, one launch after another, 36.8 for 37.6.)
-constexpr int kManyWaves = 2048;
+// From so many waves of one run each on, a wave takes several, one after another, of one token: its cosines and sines are
+// then read fewer times, but with fewer waves there is less to hide a wave's waiting behind. On one axis, one run and up
+// to three a wave, us (bf16, cold): 8500 waves (1700 tokens of 32 + 8 heads of 128) 12.8 / 12.6, 12500 15.6 / 15.8, 16500
+// 19.8 / 18.5, 40955 40.1 / 37.5; 9900 of 12 + 12 13.7 / 13.4, 24573 27.3 / 24.2; 12519 of 20 + 20 of 64 14.2 / 15.1,
+// 24573 23.6 / 22.8. On three axes, whose tables are three times as much, one and up to four: 6000 waves of 32 + 8 10.9 /
+// 11.9, 8500 14.4 / 13.9, 40955 48.5 / 40.5; 7500 of 12 + 12 13.7 / 12.8, 24573 31.3 / 26.5; 7500 of 20 + 20 of 64 11.3 /
+// 12.2, 12519 16.0 / 16.4, 18000 21.8 / 20.0.
+constexpr int kWaves = 16384, kRuns = 3, kAxesWaves = 7168, kAxesRuns = 4;
 
 // The tables' row of a position, the nearest one where there is none.
 __device__ __forceinline__ int64_t table_row(const HeadRows& r, int position) {
     return position < 0 ? 0 : (position < r.table_rows ? position : r.table_rows - 1);
 }
 
+// The cosines and sines of eight pairs from 8 * u on, of a token. On several axes a lane reads every axis' rows and keeps,
+// of each pair, its own axis': whole lines that the token's other lanes share, rather than a gather a pair.
+template <bool kAxes>
+__device__ __forceinline__ void turns_of(const HeadRows& r, int token, int u, float* c, float* s) {
+    const int64_t row = table_row(r, r.positions ? r.positions[token] : token) * (r.rotated / 2) + 8 * u;
+    load8f(r.cos + row, c);
+    load8f(r.sin + row, s);
+    if constexpr (!kAxes) return;
+    const uint32_t axis = r.axis_of[u];
+    for (int a = 1; a < r.axes; ++a) {
+        const int64_t other = table_row(r, r.positions[static_cast<int64_t>(a) * r.tokens + token]) * (r.rotated / 2) + 8 * u;
+        float ca[8], sa[8];
+        load8f(r.cos + other, ca);
+        load8f(r.sin + other, sa);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const bool mine = ((axis >> (2 * i)) & 3) == static_cast<uint32_t>(a);
+            c[i] = mine ? ca[i] : c[i];
+            s[i] = mine ? sa[i] : s[i];
+        }
+    }
+}
+
 // A head is width/16 units of 16 elements, one a lane, on `lanes` lanes (a power of two). A unit of
 // the rotated part holds both elements of eight pairs, so that a rotation needs no other lane: for
 // halves the chunks u and u + rotated/16 of eight elements, otherwise the neighbours 2u and 2u + 1.
-// A wave takes 64 / lanes heads of one token at a time, `runs` times: a lane's cosines and sines are the same for
-// all of them and are read once. On several axes a lane reads every axis' rows and keeps, of each pair, its own axis':
-// whole lines that the token's other lanes share, rather than a gather a pair.
-// Bound by memory and the vector unit (168 MB of those 8191 tokens at 4.8 TB/s, where a large copy reaches 5.6; VALU
-// 68% busy), small calls by the launch.
-template <bool kHalf>
+// A wave takes the next 64 / lanes heads, of whatever tokens; or (kRuns) 64 / lanes heads of one token at a time, `runs`
+// times: a lane's cosines and sines are then the same for all of them and are read once.
+template <bool kHalf, bool kAxes, bool kRuns>
 __global__ __launch_bounds__(kThreads) void norm_rope_kernel(HeadRows r, int parts) {
     const int lane = threadIdx.x & 63, u = lane & (r.lanes - 1), slots = 64 / r.lanes;
     const int64_t wave = static_cast<int64_t>(blockIdx.x) * (kThreads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int token = static_cast<int>(wave / parts), part = static_cast<int>(wave - static_cast<int64_t>(token) * parts);
-    if (token >= r.tokens) return;
     const int heads = r.q_heads + r.k_heads;
+    int token, head;
+    if constexpr (kRuns) {
+        token = static_cast<int>(wave / parts);
+        head = static_cast<int>(wave - static_cast<int64_t>(token) * parts) * r.runs * slots + lane / r.lanes;
+    } else {
+        const int64_t slot = wave * slots + lane / r.lanes;
+        token = static_cast<int>(slot / heads);
+        head = static_cast<int>(slot - static_cast<int64_t>(token) * heads);
+    }
+    if (token >= r.tokens) return;  // with all of its head's lanes
     const int units = r.width / 16, turning = r.rotated / 16;
     int at_a = 16 * u, at_b = 16 * u + 8;
-    float c[8], s[8];
-    if (u < turning) {
-        if (!r.interleaved) {
-            at_a = 8 * u;
-            at_b = 8 * u + r.rotated / 2;
-        }
-        const int64_t row = table_row(r, r.positions ? r.positions[token] : token) * (r.rotated / 2) + 8 * u;
-        load8f(r.cos + row, c);
-        load8f(r.sin + row, s);
-        const uint32_t axis = r.axes > 1 ? r.axis_of[u] : 0;
-        for (int a = 1; a < r.axes; ++a) {
-            const int64_t other = table_row(r, r.positions[static_cast<int64_t>(a) * r.tokens + token]) * (r.rotated / 2) + 8 * u;
-            float ca[8], sa[8];
-            load8f(r.cos + other, ca);
-            load8f(r.sin + other, sa);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const bool mine = ((axis >> (2 * i)) & 3) == static_cast<uint32_t>(a);
-                c[i] = mine ? ca[i] : c[i];
-                s[i] = mine ? sa[i] : s[i];
-            }
-        }
+    if (!r.interleaved && u < turning) {
+        at_a = 8 * u;
+        at_b = 8 * u + r.rotated / 2;
     }
-    int head = part * r.runs * slots + lane / r.lanes;
-    for (int run = 0; run < r.runs; ++run, head += slots) {
+    float c[8], s[8];
+    if (kRuns && u < turning) turns_of<kAxes>(r, token, u, c, s);
+    for (int run = 0; run < (kRuns ? r.runs : 1); ++run, head += slots) {
         const bool live = head < heads && u < units;
         float a[8], b[8];
         uint16_t* out = nullptr;
@@ -116,6 +129,7 @@ __global__ __launch_bounds__(kThreads) void norm_rope_kernel(HeadRows r, int par
         }
         if (!live) continue;
         if (u < turning) {
+            if (!kRuns) turns_of<kAxes>(r, token, u, c, s);
             if (r.interleaved) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
@@ -139,6 +153,15 @@ __global__ __launch_bounds__(kThreads) void norm_rope_kernel(HeadRows r, int par
     }
 }
 
+template <bool kHalf, bool kAxes>
+void launch(const HeadRows& rows, int most, hipStream_t s) {
+    const int heads = rows.q_heads + rows.k_heads, slots = 64 / rows.lanes, parts = (most + rows.runs - 1) / rows.runs;
+    const int64_t waves = rows.runs > 1 ? static_cast<int64_t>(rows.tokens) * parts : (static_cast<int64_t>(rows.tokens) * heads + slots - 1) / slots;
+    const unsigned groups = static_cast<unsigned>((waves + kThreads / 64 - 1) / (kThreads / 64));
+    if (rows.runs > 1) norm_rope_kernel<kHalf, kAxes, true><<<groups, kThreads, 0, s>>>(rows, parts);
+    else norm_rope_kernel<kHalf, kAxes, false><<<groups, kThreads, 0, s>>>(rows, 1);
+}
+
 }  // namespace
 
 hipError_t head_norm_rope(HeadRows rows, hipStream_t s) {
@@ -146,13 +169,12 @@ hipError_t head_norm_rope(HeadRows rows, hipStream_t s) {
     while (rows.lanes * 16 < rows.width) rows.lanes *= 2;
     const int slots = 64 / rows.lanes, heads = rows.q_heads + rows.k_heads, most = (heads + slots - 1) / slots;
     if (rows.tokens == 0 || heads == 0) return hipSuccess;
-    const int64_t waves = static_cast<int64_t>(rows.tokens) * most;
-    rows.runs = static_cast<int>(waves / kManyWaves < 1 ? 1 : waves / kManyWaves < most ? waves / kManyWaves : most);
-    const int parts = (most + rows.runs - 1) / rows.runs;
-    const int64_t needed = static_cast<int64_t>(rows.tokens) * parts;
-    const unsigned groups = static_cast<unsigned>((needed + kThreads / 64 - 1) / (kThreads / 64));
-    if (rows.half) norm_rope_kernel<true><<<groups, kThreads, 0, s>>>(rows, parts);
-    else norm_rope_kernel<false><<<groups, kThreads, 0, s>>>(rows, parts);
+    const bool axes = rows.axes > 1;
+    // The same number of runs for every wave of a token, but for the last one's.
+    const int up_to = axes ? kAxesRuns : kRuns, parts = (most + up_to - 1) / up_to;
+    rows.runs = static_cast<int64_t>(rows.tokens) * most >= (axes ? kAxesWaves : kWaves) ? (most + parts - 1) / parts : 1;
+    if (rows.half) axes ? launch<true, true>(rows, most, s) : launch<true, false>(rows, most, s);
+    else axes ? launch<false, true>(rows, most, s) : launch<false, false>(rows, most, s);
     return hipGetLastError();
 }
 
