@@ -910,8 +910,8 @@ int cozyq_cross_attend(int device, const void* q, int half, int64_t tokens, int 
         (states && (!k || !v || !aligned16(k) || !aligned16(v))) || k_request % 8 || k_state % 8 || k_head % 8 ||
         v_request % 8 || v_state % 8 || v_head % 8)
         return hipErrorInvalidValue;
-    if (!workspace && cozyq_cross_attend_workspace_bytes(tokens, q_heads, requests, states, kv_heads, width, most))
-        return hipErrorInvalidValue;
+    const int64_t bytes = cozyq_cross_attend_workspace_bytes(tokens, q_heads, requests, states, kv_heads, width, most);
+    if (bytes < 0 || (bytes && !workspace)) return hipErrorInvalidValue;
     const OnDevice guard(device);
     if (guard.error() != hipSuccess) return guard.error();
     return cozyq::cross_attend({static_cast<const uint16_t*>(q), static_cast<const uint16_t*>(k),

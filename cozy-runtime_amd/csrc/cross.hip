@@ -943,11 +943,12 @@ struct Shape {
     int splits;     // many rows: workgroups of a tile
     int cut, shares;  // few rows: a run's steps at the least (0: runs are tiles), runs at the most
     int64_t floats;
+    int64_t threads;  // of the larger launch
 };
 
 Shape shape_of(int64_t tokens, int group, int requests, int kv_heads, int states, int width, int64_t most) {
     const int64_t rows = (most > 0 && most < tokens ? most : tokens) * group;
-    Shape a = {rows <= few_rows(width), 0, 0, 1, 0, 0, 0};
+    Shape a = {rows <= few_rows(width), 0, 0, 1, 0, 0, 0, 0};
     if (a.few) {
         a.rows = rows > 16 ? 32 : 16;
         a.tiles = tokens * group / a.rows + requests;
@@ -959,14 +960,17 @@ Shape shape_of(int64_t tokens, int group, int requests, int kv_heads, int states
             a.shares = static_cast<int>(min(runs, shares));
             a.floats = 2ll * a.shares * kv_heads * a.rows * (padded(width) + 2);
         }
+        a.threads = 256 * kv_heads * (a.shares > a.tiles ? a.shares : a.tiles);
     }
     if (!a.few) {
-        a = {false, 32 * waves_of(padded(width)), 0, 1, 0, 0, 0};
+        const int waves = waves_of(padded(width));
+        a = {false, 32 * waves, 0, 1, 0, 0, 0, 0};
         a.tiles = (tokens * group + a.rows - 1) / a.rows + requests;
         const int64_t step = step_of(padded(width)), steps = (states + step - 1) / step;
         const int64_t splits = min(256 / (a.tiles * kv_heads), steps / 4);
         a.splits = static_cast<int>(splits < 1 ? 1 : splits > 64 ? 64 : splits);
         if (a.splits > 1) a.floats = a.tiles * a.splits * kv_heads * a.rows * (padded(width) + 2);
+        a.threads = a.tiles * kv_heads * waves * (a.splits > 4 ? 64 * a.splits : a.splits > 1 ? 256 : 64);
     }
     return a;
 }
@@ -1000,7 +1004,8 @@ hipError_t attend(const CrossAttend& p, const Shape& a, hipStream_t s) {
 }  // namespace
 
 int64_t cross_attend_work(int64_t tokens, int group, int requests, int kv_heads, int states, int width, int64_t most) {
-    return 4 * shape_of(tokens, group, requests, kv_heads, states, width, most).floats;
+    const Shape a = shape_of(tokens, group, requests, kv_heads, states, width, most);
+    return a.threads < (1ll << 32) ? 4 * a.floats : -1;
 }
 
 // What cuts_of and find_item come to, 64 requests after another: the same sums and rules.

@@ -357,7 +357,8 @@ struct CrossAttend {
     float* work;
     int splits, cut, shares;
 };
-// Bytes of workspace; `most`: the most rows a request has, as far as the caller knows (0: not at all).
+// Bytes of workspace, -1 for calls of more threads than a launch has (2^32 - 1); `most`: the most rows a request has, as
+// far as the caller knows (0: not at all).
 int64_t cross_attend_work(int64_t tokens, int group, int requests, int kv_heads, int states, int width, int64_t most);
 hipError_t cross_attend(CrossAttend p, int64_t most, hipStream_t s);
 // How few rows' steps are cut, from `starts` and `lengths` in host memory (cozyq_host_cross_runs); false where they are not.

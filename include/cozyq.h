@@ -594,7 +594,8 @@ int cozyq_cache_attend(int device, int fp8, const void* q, int half, int64_t tok
  * softmax(scale · q·k) · v over what is seen; 0 where nothing is and for a row of no request. Nothing of a state that
  * is not seen reaches a result, whatever it holds. `most`: the most rows a request has, as far as the caller knows
  * (0: not at all); it sets the launch's shape and speed, never its results. The workspace is of
- * cozyq_cross_attend_workspace_bytes bytes, uninitialised (NULL where that is 0; -1 for a bad argument). */
+ * cozyq_cross_attend_workspace_bytes bytes, uninitialised (NULL where that is 0; -1 for a bad argument, or more rows,
+ * heads and requests together than a launch has threads for). */
 int64_t cozyq_cross_attend_workspace_bytes(int64_t tokens, int q_heads, int requests, int states, int kv_heads, int width,
                                            int64_t most);
 int cozyq_cross_attend(int device, const void* q, int half, int64_t tokens, int q_heads, int64_t q_token, int64_t q_head,

@@ -66,3 +66,16 @@ def test_ascending_and_shuffled_starts(seed):
         assert found[0] == steps
         rng.shuffle(starts)
         held(runs(tokens, kv_heads * group, states, kv_heads, width, most, starts, lengths))
+
+
+def test_calls_of_more_threads_than_a_launch_has_are_refused():
+    """2^32 threads: 256 a tile of 16 rows and key head, and 512 one of 256."""
+    size = _lib.load().cozyq_cross_attend_workspace_bytes
+    assert size(65535, 4096, 65535, 10, 4096, 64, 1) == -1
+    assert size(65535, 256, 65535, 10, 256, 64, 1) == -1 and size(65535, 128, 65535, 10, 128, 64, 1) == 0
+    assert size(1 << 23, 256, 1, 10, 256, 8, 0) == -1 and size(1 << 22, 256, 1, 10, 256, 8, 0) == 0
+    one, at = np.zeros(32, dtype=np.float32), np.zeros(1, dtype=np.int32)
+    p = one.ctypes.data + -one.ctypes.data % 16
+    call = _lib.load().cozyq_cross_attend
+    assert call(0, p, 0, 65535, 4096, 64, 64, p, p, 65535, 10, 4096, 64, 64, 64, 64, 64, 64, 64, at.ctypes.data, None, None, 0, 1,
+                1.0, p, None, None) == 1  # fmt: skip
