@@ -67,7 +67,8 @@ __device__ __forceinline__ float block_total(float v, float* places) {
 template <bool kHalf, bool kFp8, int kRuns>
 __global__ __launch_bounds__(1024) void add_rms_kernel(AddRms p) {
     __shared__ float sums[2][16], tops[16];
-    const int64_t row = blockIdx.x;
+    const int64_t row = static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x;
+    if (row >= p.rows) return;
     const int thread = threadIdx.x, waves = blockDim.x >> 6;
     const uint16_t* x = p.x + row * p.width;
     const uint16_t* r = p.residual ? p.residual + row * p.width : nullptr;
@@ -172,8 +173,11 @@ __global__ __launch_bounds__(1024) void add_rms_kernel(AddRms p) {
 template <bool kHalf, bool kFp8>
 hipError_t launch(const AddRms& p, hipStream_t s) {
     const int lanes = (p.width / 16 + 63) / 64 * 64;
-    if (lanes <= 1024) add_rms_kernel<kHalf, kFp8, 1><<<p.rows, lanes, 0, s>>>(p);
-    else add_rms_kernel<kHalf, kFp8, 2><<<p.rows, (lanes / 2 + 63) / 64 * 64, 0, s>>>(p);
+    // A dimension of a grid has fewer than 2^32 threads: lines of 2^21 rows, of up to 1024 threads each.
+    constexpr int kLine = 1 << 21;
+    const dim3 grid(p.rows < kLine ? p.rows : kLine, (p.rows + kLine - 1) / kLine);
+    if (lanes <= 1024) add_rms_kernel<kHalf, kFp8, 1><<<grid, lanes, 0, s>>>(p);
+    else add_rms_kernel<kHalf, kFp8, 2><<<grid, (lanes / 2 + 63) / 64 * 64, 0, s>>>(p);
     return hipGetLastError();
 }
 
