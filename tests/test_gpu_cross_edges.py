@@ -1,5 +1,5 @@
-"""Attention to an encoder's states (`cozyq.attention.cross`) at the ends of its types and at scores far from zero,
-against `oracle/layer.py`; bars as in test_gpu_cross.py."""
+"""Attention to an encoder's states (`cozyq.attention.cross`) where every state counts, at the ends of its types and at
+scores far from zero, against counts and `oracle/layer.py`; bars as in test_gpu_cross.py."""
 
 from __future__ import annotations
 
@@ -23,6 +23,34 @@ def attention():
 
 # One row and a few, two tiles of few rows, part of a tile of many, more than one.
 ROWS = [[1, 2], [20], [60, 1], [130, 1], [300]]
+
+
+@pytest.mark.parametrize("width,dtype", [(64, FP16), (128, FP16), (256, BF16), (256, FP16)])
+@pytest.mark.parametrize("rows", ROWS, ids=str)
+def test_cross_every_state_counts_once(attention, rows, width, dtype):
+    """Keys of zeros and values of one channel each, state t's the channel t % D: the result is how many of a request's n
+    states have the channel, over n. Weights (2^6 or 2^-24) and their sums (below 2^15 states) are exact, so that the
+    quotient's two roundings in float32 and the output's one are all there is: u + 2^-22. A state lost or taken twice
+    moves its channel's count of 16385 states by one in 64, 128 or 256 (D 256, 128, 64), that is by eight times u or more
+    in fp16 and by four times in bf16, and fewer states' by more."""
+    for states in (1, 31, 32, 33, 64, 65, 127, 255, 257, 767, 769, 1025, 4096, 4097, 16385):
+        requests = len(rows)
+        q, _, _ = inputs(sum(rows), requests, 1, 2, 1, width, dtype, states)
+        k = torch.zeros(requests, states, 1, width, dtype=dtype, device=DEV)
+        t = torch.arange(states, device=DEV)
+        channel = torch.nn.functional.one_hot(t % width, width)
+        v = channel.to(dtype)[None, :, None].expand(requests, -1, -1, -1)
+        lengths = [states, max(1, states - 2)][:requests]
+        gen = torch.Generator(DEV).manual_seed(states)
+        mask = torch.rand(requests, states, generator=gen, device=DEV) < 0.8
+        mask[:, ::97] = True
+        for shown in (None, mask):
+            got = attention.cross(torch, q, k, v, starts=counts(rows), lengths=ints(lengths), mask=shown, most=max(rows))
+            for r, n in enumerate(lengths):
+                seen = t < n if shown is None else (t < n) & shown[r]
+                want = channel[seen].sum(0).double() / int(seen.sum())
+                mine = got[sum(rows[:r]) : sum(rows[: r + 1])].double()
+                assert ((mine - want).abs() <= (UNIT[dtype] + 2.0**-22) * want).all(), (states, r)
 
 
 @pytest.mark.parametrize("states", [40, 450, 5000])
