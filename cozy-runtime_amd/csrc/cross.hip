@@ -153,13 +153,25 @@ __device__ void clear_rest(const CrossAttend& p, int busy) {
         reinterpret_cast<i32x4*>(p.out)[i < from ? i : i - from + after] = i32x4{0, 0, 0, 0};
 }
 
+// The inputs' type's largest number, and a finite result within it: a mean is no larger than its values, but where weights
+// were rounded up and their sum was not, the quotient may be.
+template <bool kHalf>
+constexpr float kLargest = kHalf ? 65504.0f : 0x1.fep127f;
+template <bool kHalf>
+__device__ __forceinline__ float within(float x) {
+    const float bounded = fminf(fmaxf(x, -kLargest<kHalf>), kLargest<kHalf>);
+    return __builtin_fabsf(x) < __builtin_inff() ? bounded : x;
+}
+
 // Four elements of a row's result from d on, of the sums v with the denominator `total`. `some`: whether a state was
 // seen; nothing seen is 0, nothing but scores of minus infinity the quotient 0 / 0.
 template <bool kHalf>
 __device__ __forceinline__ void store_row(const CrossAttend& p, int64_t at, int d, f32x4 v, float total, bool some) {
     if (d >= p.width) return;
     const float inv = some ? 1.0f / total : 0.0f;
-    *reinterpret_cast<i32x2*>(p.out + at * p.width + d) = i32x2{pack2<kHalf>(v[0] * inv, v[1] * inv), pack2<kHalf>(v[2] * inv, v[3] * inv)};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = within<kHalf>(v[i] * inv);
+    *reinterpret_cast<i32x2*>(p.out + at * p.width + d) = i32x2{pack2<kHalf>(v[0], v[1]), pack2<kHalf>(v[2], v[3])};
 }
 
 // A view of `left` rows (none below 1) of `width` 16-bit elements, `stride` apart, from `base` on: what lies past them
@@ -444,12 +456,28 @@ __global__ __launch_bounds__(64 * kWaves, kWidth == 256 ? 1 : 2) void cross_kern
     if (p.splits == 1) {
         __syncthreads();
         const float inv = any ? 1.0f / total : 0.0f;
+        float largest = 0.0f;
+        const auto leave = [&](auto&& number) {
 #pragma unroll
-        for (int o = 0; o < kOut; ++o) {
+            for (int o = 0; o < kOut; ++o) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                *reinterpret_cast<i32x2*>(own + col * 2 * kWidth + 16 * key_place<kWidth>(col, 4 * o + i) + 8 * h) =
-                    i32x2{pack2<kHalf>(acc[o][4 * i] * inv, acc[o][4 * i + 1] * inv), pack2<kHalf>(acc[o][4 * i + 2] * inv, acc[o][4 * i + 3] * inv)};
+                for (int i = 0; i < 4; ++i) {
+                    float x[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) x[j] = number(acc[o][4 * i + j]);
+                    *reinterpret_cast<i32x2*>(own + col * 2 * kWidth + 16 * key_place<kWidth>(col, 4 * o + i) + 8 * h) =
+                        i32x2{pack2<kHalf>(x[0], x[1]), pack2<kHalf>(x[2], x[3])};
+                }
+            }
+        };
+        leave([&](float sum) {
+            const float x = sum * inv;
+            largest = fmaxf(largest, __builtin_fabsf(x));
+            return x;
+        });
+        if (__any(largest > kLargest<kHalf>)) {
+            rarely();
+            leave([&](float sum) { return within<kHalf>(sum * inv); });
         }
         wave_sync();
         each_line([&](int i, int token, int head, int d) {

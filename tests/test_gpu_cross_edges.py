@@ -91,3 +91,22 @@ def test_cross_scores_far_below_zero(attention, rows, beside, dtype):
         want = v[:, at : at + 10].double().mean(1).repeat_interleave(ints(rows), 0)
         size = v[:, at : at + 10].double().abs().mean(1).repeat_interleave(ints(rows), 0)
         assert ((got - want).abs() <= UNIT[dtype] * want.abs() + (UNIT[dtype] + 2.0**-20) * size).all(), at
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("states", [33, 450, 5000])
+@pytest.mark.parametrize("rows", ROWS, ids=str)
+def test_cross_values_that_are_all_the_type_s_largest(attention, rows, states, dtype):
+    """Their mean is the type's largest too: no rounding of weights takes it past that."""
+    most = torch.finfo(dtype).max
+    q, k, v = inputs(sum(rows), len(rows), states, 4, 2, 64, dtype, states)
+    v = torch.full_like(v, most)
+    v[..., ::3] *= -1
+    got = attention.cross(torch, q, k, v, starts=counts(rows), most=max(rows)).double()
+    want = v[0, 0].double().repeat_interleave(2, 0)
+    # A weight is off by half a step at the most, and their sum, as a share of it, no more; then the output's half step.
+    assert ((got - want).abs() <= (2 * UNIT[dtype] + 2.0**-18) * most).all() and got.isfinite().all()
+    # An infinity among them is the mean, and beside one of the other sign NaN.
+    v[:, states // 2, 0, 0], v[:, 5, 1, 1], v[:, 6, 1, 1] = math.inf, math.inf, -math.inf
+    got = attention.cross(torch, torch.zeros_like(q), k, v, starts=counts(rows), most=max(rows))
+    assert (got[:, :2, 0] == math.inf).all() and got[:, 2:, 1].isnan().all() and got[:, :2, 1:].isfinite().all()
