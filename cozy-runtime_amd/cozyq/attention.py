@@ -25,7 +25,9 @@ def cross(torch: Any, q: Tensor, k: Tensor, v: Tensor, *, starts: Tensor | None 
     seen; None: all); where that is none, or of a row of no request, the result is 0. What is not seen reaches no
     result, whatever it holds. `starts`, `lengths` and `mask` are read on the GPU, so that a step may be captured into a
     HIP graph and replayed over others. `most`: the most rows a request has, as far as the host knows (0: not at all);
-    kernels are chosen by it, and any value is right. D is a multiple of 8 up to 256. q, k and v may be views (of one
+    kernels are chosen by it, and any value is right, but 0 beside `starts` takes all rows for one request's: single
+    tokens of 24 requests over up to 1600 states then take 37 us instead of 29. Scores, the softmax and sums are float32
+    (scores past its range are infinities); each state's weight is rounded to q's type before it multiplies v. D is a multiple of 8 up to 256. q, k and v may be views (of one
     projection's buffer, say) whose last axis is dense and whose other strides and address are multiples of 16 bytes.
     A workspace comes from torch's allocator where states are split over workgroups. Results carry no gradient."""
     index = _dispatch.card(OP, q)

@@ -62,7 +62,7 @@ __device__ __forceinline__ float block_total(float v, float* places) {
 // sixteenth of a rotation's block: two of its four stages stay in the lane, the others move by DPP, and nothing but the
 // two reductions passes through LDS.
 // Bound by the vector unit and memory alike where there is a rotation (6001 rows of 4096: 172 MB in 32.6 us, 5.3 TB/s of a
-// large copy's 5.6; VALU 96% busy), by memory without (1531 rows of 12288 to E4M3: 132 MB in 25.3 us, 5.2 TB/s); few rows by
+// large copy's 5.6; VALU 94% busy), by memory without (1531 rows of 12288 to E4M3: 132 MB in 25.3 us, 5.2 TB/s); few rows by
 // the launch and one row's chain of reductions (one row 3.6 us, 48 of 5120 4.4).
 template <bool kHalf, bool kFp8, int kRuns>
 __global__ __launch_bounds__(1024) void add_rms_kernel(AddRms p) {

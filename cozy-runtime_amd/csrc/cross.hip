@@ -7,8 +7,10 @@
 //
 // Both products run on the matrix unit in the inputs' type, transposed (Sᵀ = K·Qᵀ, Oᵀ = Vᵀ·Pᵀ), so that a row is a
 // column of both results and a lane holds 16 scores of one row for every 32 states. Weights are rounded to the inputs'
-// type for the second product alone: float32 runs at a sixteenth of the rate there. Scores, maxima, sums and
-// accumulators are float32. States that are not seen are zeros by the time they are in LDS, whatever memory holds.
+// type for the second product alone: float32 runs at a sixteenth of the rate there. (Against 64 bits the result is off
+// by 0.0021 of its size in bf16 and 0.00024 in fp16 over 30000 states, where weights of 32 bits leave 0.0017 and 0.00021,
+// the output's rounding.) Scores, maxima, sums and accumulators are float32. States that are not seen are zeros by the
+// time they are in LDS, whatever memory holds.
 #include <hip/hip_runtime.h>
 
 #include "common.h"
@@ -223,9 +225,10 @@ __device__ __forceinline__ float* place_of(const CrossAttend& p, int64_t group) 
 // written 8 and 16 bytes a row at a time they took 18000 rows of 24 heads of 128 over 512 states from 131 to 152 us.
 // Where tiles are fewer than CUs a tile's states are split (301 rows of 28 heads over 30000 states: six ways, 154 us, and
 // 746 in one), and cross_join_kernel adds the parts.
-// Bound by the matrix and vector units in turn: of a step's 2.0 us (256 rows, 64 states, 128 wide) the scores take 0.5,
-// their exponentials and the second product 0.75, of which the products alone 0.95 together, waiting for states 0.25,
-// writing them to LDS and the barrier 0.15. Two waves a SIMD are all that its registers hold. Tried and not faster: the
+// Bound by no unit alone (matrix unit 28 to 39% of the cycles, vector unit 35 to 45%, a wave waits 33 to 39% of its life):
+// of a step's 2.0 us (256 rows, 64 states, 128 wide) the products alone take 0.95. Left out one at a time, the scores
+// are 0.5 of it, their exponentials and the second product 0.75, waiting for states 0.25, writing them to LDS and the
+// barrier 0.15; the other 0.35 is no single part's. Two waves a SIMD are all that its registers hold. Tried and not faster: the
 // next step's scores over this one's exponentials; half of the waves half a step late; 4 waves of 64 rows (copies
 // between register files, +50%); 4 waves of 32, two workgroups a CU (states read twice as often, +12%); equal runs of
 // steps as few rows have them (+5%: their parts' traffic, and requests' states no longer shared in L2).
@@ -951,7 +954,10 @@ constexpr int padded(int width) { return width <= 64 ? 64 : width <= 128 ? 128 :
 constexpr int waves_of(int width) { return width == 256 ? 4 : 8; }
 
 // Requests of up to so many rows a key head are cross_few_kernel's: two tiles of 16, whose accumulators fit the registers
-// up to 128 wide.
+// up to 128 wide. By that alone; cross_few_kernel / cross_kernel, us, requests of so many rows each: 24 requests over 1600
+// states, 8 key heads of 128, 16 rows 34.4 / 37.7, 20 rows 35.7 / 37.4, 32 rows 35.1 / 38.0, 20 key heads of 64 40.8 /
+// 56.5, 41.4 / 56.8, 40.3 / 55.1; but 4 requests, whose steps are cut, 16 rows 24.9 / 17.8, 20 rows 29.7 / 18.0, 32 rows
+// 38.9 / 18.7, of 64 20.7 / 19.9, 26.2 / 20.1, 31.5 / 20.9.
 constexpr int64_t few_rows(int width) { return width > 128 ? 16 : 32; }
 
 // Whether few rows' steps are cut into equal runs, which costs a second launch and a workgroup's search for its tiles,

@@ -591,7 +591,8 @@ int cozyq_cache_attend(int device, int fp8, const void* q, int half, int64_t tok
  * multiple of 8 up to 256. Request b's rows are starts[b] .. starts[b + 1] − 1 (int32 [requests + 1], ascending; NULL:
  * tokens / requests each); it sees the first lengths[b] of its states (int32 [requests]; NULL: all) that mask has
  * (bytes [requests, states], mask_request apart, nonzero: seen; NULL: all). out [tokens, q_heads, width], contiguous:
- * softmax(scale · q·k) · v over what is seen; 0 where nothing is and for a row of no request. Nothing of a state that
+ * softmax(scale · q·k) · v over what is seen, scores, softmax and sums in float32 and each weight rounded to the type
+ * before it multiplies v; 0 where nothing is seen and for a row of no request. Nothing of a state that
  * is not seen reaches a result, whatever it holds. `most`: the most rows a request has, as far as the caller knows
  * (0: not at all); it sets the launch's shape and speed, never its results. The workspace is of
  * cozyq_cross_attend_workspace_bytes bytes, uninitialised (NULL where that is 0; -1 for a bad argument, or more rows,
