@@ -29,7 +29,7 @@ ROWS = [[1, 2], [20], [60, 1], [130, 1], [300]]
 @pytest.mark.parametrize("rows", ROWS, ids=str)
 def test_cross_every_state_counts_once(attention, rows, width, dtype):
     """Keys of zeros and values of one channel each, state t's the channel t % D: the result is how many of a request's n
-    states have the channel, over n. Weights (2^6 or 2^-24) and their sums (below 2^15 states) are exact, so that the
+    states have the channel, over n. Weights (2^6 or 2^-14) and their sums (below 2^15 states) are exact, so that the
     quotient's two roundings in float32 and the output's one are all there is: u + 2^-22. A state lost or taken twice
     moves its channel's count of 16385 states by one in 64, 128 or 256 (D 256, 128, 64), that is by eight times u or more
     in fp16 and by four times in bf16, and fewer states' by more."""
@@ -55,10 +55,14 @@ def test_cross_every_state_counts_once(attention, rows, width, dtype):
 
 @pytest.mark.parametrize("states", [40, 450, 5000])
 @pytest.mark.parametrize("rows", ROWS, ids=str)
-@pytest.mark.parametrize("power", [126, 60, -100])
+@pytest.mark.parametrize("power", [126, 60, -100, -120, -126])
 def test_cross_values_of_any_size(attention, rows, states, power):
     """bf16 values near the type's ends: their weighted means are as large, whatever their sums would be. Scores grow
-    along the states, so that the largest is met late."""
+    along the states, so that the largest is met late. Sums of the smallest are in steps of 2^-149, half of which every
+    16 states (a matrix instruction) may cost over weights of 2^-14 and more: 2^-131 of the mean for 450, below the bars'
+    2^-130, and for 5000 2^-128, below their 2^-127 at 2^-120."""
+    if power == -126 and states > 450:
+        pytest.skip("past what float32's smallest steps allow")
     q, k, v = inputs(sum(rows), len(rows), states, 4, 2, 64, BF16, states)
     gen = torch.Generator(DEV).manual_seed(3)
     k = (k.float() * torch.linspace(0, 2, states, device=DEV)[None, :, None, None]).to(BF16)
