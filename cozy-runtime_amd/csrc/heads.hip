@@ -24,7 +24,7 @@ constexpr int kThreads = 256;
 // 24573 23.6 / 22.8. On three axes, whose tables are three times as much, one and up to four: 6000 waves of 32 + 8 10.9 /
 // 11.9, 8500 14.4 / 13.9, 40955 48.5 / 40.5; 7500 of 12 + 12 13.7 / 12.8, 24573 31.3 / 26.5; 7500 of 20 + 20 of 64 11.3 /
 // 12.2, 12519 16.0 / 16.4, 18000 21.8 / 20.0.
-constexpr int kWaves = 16384, kRuns = 3, kAxesWaves = 7168, kAxesRuns = 4;
+constexpr int kManyWaves = 16384, kMostRuns = 3, kManyAxesWaves = 7168, kMostAxesRuns = 4;
 
 // The tables' row of a position, the nearest one where there is none.
 __device__ __forceinline__ int64_t table_row(const HeadRows& r, int position) {
@@ -176,8 +176,8 @@ hipError_t head_norm_rope(HeadRows rows, hipStream_t s) {
     if (rows.tokens == 0 || heads == 0) return hipSuccess;
     const bool axes = rows.axes > 1;
     // The same number of runs for every wave of a token, but for the last one's.
-    const int up_to = axes ? kAxesRuns : kRuns, parts = (most + up_to - 1) / up_to;
-    rows.runs = static_cast<int64_t>(rows.tokens) * most >= (axes ? kAxesWaves : kWaves) ? (most + parts - 1) / parts : 1;
+    const int up_to = axes ? kMostAxesRuns : kMostRuns, parts = (most + up_to - 1) / up_to;
+    rows.runs = static_cast<int64_t>(rows.tokens) * most >= (axes ? kManyAxesWaves : kManyWaves) ? (most + parts - 1) / parts : 1;
     if (rows.half) axes ? launch<true, true>(rows, most, s) : launch<true, false>(rows, most, s);
     else axes ? launch<false, true>(rows, most, s) : launch<false, false>(rows, most, s);
     return hipGetLastError();

@@ -605,14 +605,15 @@ int cozyq_cross_attend(int device, const void* q, int half, int64_t tokens, int 
                        const int* starts, const int* lengths, const void* mask, int64_t mask_request, int64_t most,
                        float scale, void* out, void* workspace, void* stream);
 
-/* Test entries (no reference counterpart): the kernels' scalar conversions run on the host,
- * so CPU tests can hold the device code's arithmetic against torch without a GPU. */
-/* How cozyq_cross_attend cuts the steps of requests of few rows (starts [requests + 1], lengths [requests], in host
- * memory), by the kernels' own sums and rules: 1, and out [5] the steps in all (2^30: or more), a run's steps, how many
- * runs the workspace has places for, and the first and the last run that joining any tile reads; 0 where steps are not
- * cut, -1 for a bad argument. */
+/* Test entry (no reference counterpart): how cozyq_cross_attend cuts the steps of requests of few rows (starts
+ * [requests + 1], lengths [requests], in host memory), by the kernels' own sums and rules: 1, and out [5] the steps in
+ * all (2^30: or more), a run's steps, how many runs the workspace has places for, and the first and the last run that
+ * joining any tile reads; 0 where steps are not cut, -1 for a bad argument. */
 int cozyq_host_cross_runs(int64_t tokens, int q_heads, int requests, int states, int kv_heads, int width, int64_t most,
                           const int* starts, const int* lengths, int* out);
+
+/* Test entries (no reference counterpart): the kernels' scalar conversions run on the host,
+ * so CPU tests can hold the device code's arithmetic against torch without a GPU. */
 void cozyq_host_e4m3(const float* in, uint8_t* out, int64_t n);
 void cozyq_host_mx_byte(const float* amax, uint8_t* out, int64_t n);
 
